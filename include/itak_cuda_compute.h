@@ -473,6 +473,149 @@ int itk_decode_attention_noalloc(const void* k_layer, const void* v_layer, uint3
                                  const uint32_t* kv_len, const float* d_q, float* d_out, uint32_t splits,
                                  void* cuda_stream, char* error_text, size_t error_text_len);
 
+/* ---- the paged cache: rotation, append and attention over pages ------------------------- */
+
+/* A second form of the resident cache, for callers that keep the K and V rows of many sequences in one pool of
+ * fixed-size pages: the pools, the page tables and the lengths are the caller's, on the device, so a step captured
+ * into a graph follows them from replay to replay.  No counterpart in the reference, whose cache is one slot per
+ * session (crates/wgpu-compute/src/session.rs:235-249).  Like itk_draft_attention these calls take no backend handle:
+ * they queue work on `cuda_stream` (NULL = the default stream of `device`), allocate nothing, keep nothing between
+ * calls, may be captured, and report a refusal through error_text.  They run on the device the structure names,
+ * whichever is current.  Head rows are head_dim contiguous elements; strides count elements.
+ *
+ * Element types of rows: f32 rows go with f16 pages (rounded to nearest even on append, NaN -> sign|0x7e00), f16 rows
+ * with f16 pages, bf16 rows with bf16 pages. */
+typedef enum itk_row_dtype { ITK_ROW_F32 = 0, ITK_ROW_F16 = 1, ITK_ROW_BF16 = 2 } itk_row_dtype;
+
+/* The rotation's frequencies: angle of pair i at position p = p * inv_freq[i], inv_freq[i] = base^(-2i / rotary_dim)
+ * scaled for contexts longer than the trained one:
+ *   ITK_ROPE_PLAIN   as it is
+ *   ITK_ROPE_LINEAR  every frequency / factor (positions interpolated)
+ *   ITK_ROPE_BASE    base * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair as with LINEAR, the fastest kept
+ *   ITK_ROPE_BANDS   by turns over the original context, t_i = original_context * inv_freq[i] / 2 pi: pairs of more
+ *                    than `high` turns kept, of fewer than `low` divided by factor, between them mixed in t_i
+ *   ITK_ROPE_RAMP    by pair number: kept up to the pair of `high` turns (rounded down), divided by factor from the
+ *                    pair of `low` turns (rounded up), mixed linearly between; magnitude 0.1 ln(factor) + 1
+ *   ITK_ROPE_PAIRS   inv_freq[i] / pair_factors[i]
+ * `magnitude` multiplies sine and cosine; 0 asks for the scaling's own (1 except for RAMP).  Host arithmetic in f64, no
+ * device needed; inv_freq receives rotary_dim / 2 values, which the caller copies to the device once. */
+typedef enum itk_rope_scaling {
+    ITK_ROPE_PLAIN = 0, ITK_ROPE_LINEAR = 1, ITK_ROPE_BASE = 2, ITK_ROPE_BANDS = 3, ITK_ROPE_RAMP = 4, ITK_ROPE_PAIRS = 5
+} itk_rope_scaling;
+typedef struct itk_rope_config {
+    const float* pair_factors; /* PAIRS: rotary_dim / 2 host values, finite and > 0; else unused */
+    uint32_t rotary_dim;       /* even, 2..256 */
+    int32_t scaling;           /* itk_rope_scaling */
+    float base;                /* finite, > 1 */
+    float factor;              /* LINEAR, BASE, BANDS, RAMP: finite, >= 1 */
+    float original_context;    /* BANDS, RAMP: finite, > 0 */
+    float low, high;           /* BANDS, RAMP: turns, 0 < low < high */
+    float magnitude;           /* finite, >= 0 */
+} itk_rope_config;
+int itk_rope_table(const itk_rope_config* cfg, double* inv_freq, float* magnitude, char* error_text, size_t error_text_len);
+
+/* Rotates `rows` x `heads` head rows, row r at positions[r]: as itk_rope_rows, for rows of all three types, any strides,
+ * a frequency table, and the gradient.  Pair i joins channels (2i, 2i + 1) (pairing 0) or (i, i + rotary_dim / 2)
+ * (pairing 1); channels from rotary_dim on are copied.  With inverse != 0 the angle is negated: the map from the
+ * gradient of `out` to the gradient of `x`.  Angles in f64, reduced to a turn before sine and cosine are taken in f32;
+ * products in f32; one rounding to the rows' type.  out may be x (same strides); else the two share no element.
+ * head_dim up to 256, even. */
+typedef struct itk_rope_desc {
+    const void* x;             /* device, element (row, head, channel) at row * x_row_stride + head * x_head_stride + channel */
+    void* out;                 /* device, likewise */
+    const uint32_t* positions; /* device [rows] */
+    const double* inv_freq;    /* device [rotary_dim / 2] */
+    uint64_t x_row_stride, x_head_stride, out_row_stride, out_head_stride;
+    uint32_t rows, heads, head_dim, rotary_dim;
+    uint32_t pairing, inverse;
+    int32_t dtype; /* itk_row_dtype */
+    int32_t device;
+    float magnitude;
+} itk_rope_desc;
+int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* error_text, size_t error_text_len);
+
+/* The pools: element (page, head, row, channel) of K at page * page_stride + head * head_stride + row * row_stride +
+ * channel, V alike.  Both [page][kv_head][row][D] and [page][row][kv_head][D] are such layouts.  Pools start on a
+ * 16-byte boundary and strides are multiples of 8. */
+typedef struct itk_paged_kv {
+    void* k;
+    void* v;
+    uint64_t page_stride, head_stride, row_stride;
+    uint32_t n_pages;
+    uint32_t page_size; /* rows of a page: a power of two up to 65536 */
+    uint32_t kv_heads;
+    uint32_t head_dim; /* a multiple of 8, up to 256 */
+    int32_t dtype;     /* ITK_ROW_F16 or ITK_ROW_BF16 */
+    int32_t device;
+} itk_paged_kv;
+
+/* A ragged batch.  Sequence s owns the packed rows [row_start[s], row_start[s + 1]) and kv_len[s] keys, its new rows
+ * included: its row i sits at position kv_len[s] - rows + i.  The key of position p is row p % page_size of page
+ * table[s * table_stride + p / page_size].  All arrays are on the device and read when the work runs.
+ * Contents are checked there: a page number outside the pool is never followed (its keys read as zeros, a row that
+ * would be stored there is dropped) and raises bit 0 of *status; a length that the table has no columns for is cut to
+ * them (bit 1); new rows that reach before position 0 see nothing and are not stored (bit 2); starts that run backwards
+ * or past total_rows are cut (bit 3).  Bit 4: a wait inside the tensor-core kernel ran out and the call's outputs are
+ * not valid.  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] are neither
+ * read nor written. */
+typedef struct itk_paged_batch {
+    const uint32_t* table;     /* [n_seqs][table_stride], table_width columns used */
+    const uint32_t* row_start; /* [n_seqs + 1] */
+    const uint32_t* kv_len;    /* [n_seqs] */
+    uint32_t* status;
+    uint32_t n_seqs; /* up to 1024 */
+    uint32_t table_width, table_stride;
+    uint32_t total_rows; /* rows the packed tensors hold */
+} itk_paged_batch;
+
+/* Stores the batch's new K and V rows into their pages, K rotated at its rows' positions (inv_freq NULL or rotary_dim 0:
+ * stored as it is), and, where q is not NULL, writes the batch's Q rows rotated alike to q_out - one launch for all that
+ * stands between a layer's projection and its attention.  A token's heads are contiguous; the three row strides let q,
+ * k and v be parts of one projection's output.  q_out may be q.  Two rows must not share a place in the pool. */
+typedef struct itk_paged_append_desc {
+    const void* q;     /* [total_rows][q_heads][head_dim] or NULL */
+    void* q_out;       /* as q */
+    const void* k_new; /* [total_rows][kv_heads][head_dim] */
+    const void* v_new;
+    const double* inv_freq; /* device [rotary_dim / 2] or NULL */
+    uint64_t q_row_stride, q_out_row_stride, k_row_stride, v_row_stride;
+    uint32_t q_heads; /* 0 without q */
+    uint32_t rotary_dim, pairing;
+    int32_t dtype; /* of the rows */
+    float magnitude;
+} itk_paged_append_desc;
+int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* batch, const itk_paged_append_desc* d,
+                     void* cuda_stream, char* error_text, size_t error_text_len);
+
+/* Grouped-query attention of the batch's rows over their sequences' pages: a row at position p sees the keys
+ * kp <= p (and kp > p - window when window != 0) of its own sequence; out = softmax(scale * q k^T) v, and where lse is
+ * not NULL the natural logarithm of each row's sum of exponentials.  A row that sees nothing gives zeros and -infinity.
+ * Any number of rows per sequence: one (decode), a few (a block to verify) or a prompt's chunk; max_rows is the caller's
+ * bound of it and only chooses between kernels - results hold whatever the device-side row counts are.
+ * Head dimensions, page sizes and row types as above.  Queries of f32 rows stay below 65504 in magnitude.
+ * A value that is not finite in a visible V row may reach every row of the batch block it is visible to some of;
+ * what lies outside a sequence's keys never reaches a result.
+ *
+ * `workspace`: device memory of itk_paged_attention_workspace() bytes, 256-byte aligned, that must be zero before its
+ * first use; every call leaves what it needs of it zero again.  Calls that may run at the same time need one each. */
+typedef struct itk_paged_attention_desc {
+    const void* q; /* [total_rows][q_heads][head_dim] */
+    void* out;     /* as q, same type */
+    float* lse;    /* [total_rows][q_heads] or NULL */
+    void* workspace;
+    uint64_t workspace_bytes;
+    uint64_t q_row_stride, out_row_stride;
+    uint32_t q_heads; /* a multiple of kv_heads */
+    uint32_t max_rows;
+    uint32_t window;
+    int32_t dtype; /* of the rows */
+    float scale;
+} itk_paged_attention_desc;
+int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch* batch, const itk_paged_attention_desc* d,
+                        void* cuda_stream, char* error_text, size_t error_text_len);
+/* Bytes of workspace that serve every itk_paged_attention call on `device` whatever its batch; 0 without a device. */
+uint64_t itk_paged_attention_workspace(int32_t device);
+
 /* ---- the persistent prefix store ------------------------------------------------ */
 
 /* PrefixStore (crates/itak-kv/src/store.rs): one file per entry under `root`, keyed by token prefix, bounded by

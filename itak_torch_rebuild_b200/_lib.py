@@ -47,6 +47,19 @@ ERR_INVALID_SLOT = 103
 KV_F32 = 0
 KV_F16 = 1
 
+# itk_row_dtype
+ROW_F32 = 0
+ROW_F16 = 1
+ROW_BF16 = 2
+
+# itk_rope_scaling
+ROPE_PLAIN = 0
+ROPE_LINEAR = 1
+ROPE_BASE = 2
+ROPE_BANDS = 3
+ROPE_RAMP = 4
+ROPE_PAIRS = 5
+
 
 class Config(C.Structure):
     _fields_ = [
@@ -92,6 +105,107 @@ class Stats(C.Structure):
         ("prefix_captures", C.c_uint64),
         ("prefix_restores", C.c_uint64),
         ("last_splits", C.c_uint64),
+    ]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [
+        ("pair_factors", C.POINTER(C.c_float)),
+        ("rotary_dim", C.c_uint32),
+        ("scaling", C.c_int32),
+        ("base", C.c_float),
+        ("factor", C.c_float),
+        ("original_context", C.c_float),
+        ("low", C.c_float),
+        ("high", C.c_float),
+        ("magnitude", C.c_float),
+    ]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("out", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("x_row_stride", C.c_uint64),
+        ("x_head_stride", C.c_uint64),
+        ("out_row_stride", C.c_uint64),
+        ("out_head_stride", C.c_uint64),
+        ("rows", C.c_uint32),
+        ("heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("rotary_dim", C.c_uint32),
+        ("pairing", C.c_uint32),
+        ("inverse", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("device", C.c_int32),
+        ("magnitude", C.c_float),
+    ]
+
+
+class PagedKv(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("page_stride", C.c_uint64),
+        ("head_stride", C.c_uint64),
+        ("row_stride", C.c_uint64),
+        ("n_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("device", C.c_int32),
+    ]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p),
+        ("row_start", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("status", C.c_void_p),
+        ("n_seqs", C.c_uint32),
+        ("table_width", C.c_uint32),
+        ("table_stride", C.c_uint32),
+        ("total_rows", C.c_uint32),
+    ]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_new", C.c_void_p),
+        ("v_new", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("q_row_stride", C.c_uint64),
+        ("q_out_row_stride", C.c_uint64),
+        ("k_row_stride", C.c_uint64),
+        ("v_row_stride", C.c_uint64),
+        ("q_heads", C.c_uint32),
+        ("rotary_dim", C.c_uint32),
+        ("pairing", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("magnitude", C.c_float),
+    ]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("q_row_stride", C.c_uint64),
+        ("out_row_stride", C.c_uint64),
+        ("q_heads", C.c_uint32),
+        ("max_rows", C.c_uint32),
+        ("window", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
     ]
 
 
@@ -166,6 +280,12 @@ SIGNATURES = {
                                           C.POINTER(_sz)]),
     "itk_prefix_store_stats": (C.c_int, [_vp, _u64p, _u64p, _u64p]),
     "itk_prefix_store_entry": (C.c_int, [_vp, _u64, C.c_char_p, _sz, _u64p, _u64p, _u64p, _u64p, _u64p]),
+    "itk_rope_table": (C.c_int, [C.POINTER(RopeConfig), _vp, C.POINTER(C.c_float), C.c_char_p, _sz]),
+    "itk_rope_apply": (C.c_int, [C.POINTER(RopeDesc), _vp, C.c_char_p, _sz]),
+    "itk_paged_append": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(PagedAppendDesc), _vp, C.c_char_p, _sz]),
+    "itk_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(PagedAttentionDesc), _vp,
+                                      C.c_char_p, _sz]),
+    "itk_paged_attention_workspace": (_u64, [C.c_int32]),
     "itk_rope_rows": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_float, _vp, C.c_char_p, _sz]),
     "itk_decode_attention_noalloc": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32p, _u32p, _vp, _vp, _u32, _vp,
                                                C.c_char_p, _sz]),

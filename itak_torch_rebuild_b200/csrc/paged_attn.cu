@@ -1,0 +1,97 @@
+// Host side of attention over pages: refusals, the workspace, and which kernel takes a call.
+#include <math.h>
+
+#include <atomic>
+
+#include "paged.cuh"
+
+namespace itk {
+namespace paged {
+namespace {
+
+// Multiprocessors of a device, asked for once.
+cudaError_t multiprocessors(int device, uint32_t* sms) {
+    static std::atomic<uint32_t> known[64];
+    if (device >= 0 && device < 64 && (*sms = known[device].load(std::memory_order_relaxed)) != 0) return cudaSuccess;
+    int n = 0;
+    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    *sms = static_cast<uint32_t>(n);
+    if (device >= 0 && device < 64) known[device].store(*sms, std::memory_order_relaxed);
+    return cudaSuccess;
+}
+
+constexpr uint64_t kAlign = 256;
+uint64_t round_up(uint64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+// The workspace: tickets (one per persistent CTA), then the parts' (maximum, sum) pairs, then their outputs.  A CTA
+// leaves at most two parts: of the cell its run begins in and of the one it ends in.
+struct Layout {
+    uint64_t ml, o, bytes;
+};
+Layout layout_of(uint32_t sms) {
+    Layout l;
+    const uint64_t stream_parts = 2ull * stream_ctas(sms, 128);  // above 128 channels: half the CTAs, twice the width
+    l.ml = round_up(sizeof(unsigned int) * 2ull * sms);
+    l.o = l.ml + round_up(stream_parts * kStreamRows * 2 * sizeof(float));
+    l.bytes = l.o + round_up(stream_parts * kStreamRows * 128 * sizeof(float));
+    return l;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace itk
+
+extern "C" uint64_t itk_paged_attention_workspace(int32_t device) {
+    uint32_t sms = 0;
+    if (itk::paged::multiprocessors(device, &sms) != cudaSuccess) return 0;
+    return itk::paged::layout_of(sms).bytes;
+}
+
+extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch* batch, const itk_paged_attention_desc* d,
+                                   void* cuda_stream, char* error_text, size_t error_text_len) {
+    using namespace itk::paged;
+    const ErrorText e(error_text, error_text_len);
+    AttnParams p{};
+    if (int rc = check_pool(kv, e, &p.pool)) return rc;
+    if (int rc = check_batch(batch, e, &p.batch)) return rc;
+    if (!d) return e.invalid("null pointer argument");
+    if (int rc = check_row_dtype(d->dtype, kv->dtype, e)) return rc;
+    if (d->q_heads == 0) return e.refuse(ITK_ERR_ZERO_DIMENSION, "num_q_heads must be positive, got 0");
+    if (d->q_heads % kv->kv_heads != 0)
+        return e.refuse(ITK_ERR_NON_DIVISIBLE_HEADS, "%llu query heads do not divide evenly across %llu KV heads", d->q_heads, kv->kv_heads);
+    if (static_cast<uint64_t>(batch->total_rows) * d->q_heads > 0x7fffffffull)
+        return e.invalid("total_rows x q_heads = %llu is too large", static_cast<uint64_t>(batch->total_rows) * d->q_heads);
+    if (!isfinite(d->scale)) return e.invalid("the scale must be finite");
+    if (!d->q || !d->out || !d->workspace) return e.invalid("null pointer argument");
+    if (!aligned16(d->q) || !aligned16(d->out)) return e.invalid("q and out must start on a 16-byte boundary");
+    const uint64_t width = static_cast<uint64_t>(d->q_heads) * kv->head_dim;
+    if (d->q_row_stride % 8 != 0 || d->out_row_stride % 8 != 0 || d->q_row_stride >= kMaxStride || d->out_row_stride >= kMaxStride)
+        return e.invalid("row strides must be multiples of 8 elements, got %llu and %llu", d->q_row_stride, d->out_row_stride);
+    if (batch->total_rows > 1 && d->out_row_stride < width)
+        return e.invalid("rows of out overlap (row stride %llu, %llu elements)", d->out_row_stride, width);
+    if (reinterpret_cast<uintptr_t>(d->workspace) % kAlign != 0) return e.invalid("the workspace must start on a 256-byte boundary");
+    const DeviceScope scope(kv->device);
+    if (scope.err != cudaSuccess) return e.cuda("paged attention: the device cannot be used", scope.err);
+    uint32_t sms = 0;
+    const cudaError_t known = multiprocessors(kv->device, &sms);
+    if (known != cudaSuccess) return e.cuda("paged attention: the device cannot be used", known);
+    const Layout l = layout_of(sms);
+    if (d->workspace_bytes < l.bytes) return e.refuse(ITK_ERR_CAPACITY, "the workspace holds %llu bytes, %llu are needed", d->workspace_bytes, l.bytes);
+    if (batch->total_rows == 0) return 0;
+    p.q = d->q;
+    p.out = d->out;
+    p.lse = d->lse;
+    p.q_row = d->q_row_stride;
+    p.out_row = d->out_row_stride;
+    p.q_heads = d->q_heads;
+    p.group = d->q_heads / kv->kv_heads;
+    p.window = d->window;
+    p.scale_log2 = static_cast<float>(static_cast<double>(d->scale) * 1.4426950408889634074);
+    unsigned char* ws = static_cast<unsigned char*>(d->workspace);
+    p.tickets = reinterpret_cast<unsigned int*>(ws);
+    p.part_ml = reinterpret_cast<float*>(ws + l.ml);
+    p.part_o = reinterpret_cast<float*>(ws + l.o);
+    const cudaError_t err = launch_stream(p, d->dtype, sms, static_cast<cudaStream_t>(cuda_stream));
+    return err == cudaSuccess ? 0 : e.cuda("paged attention launch failed", err);
+}

@@ -1,0 +1,596 @@
+// Attention of a ragged batch over the pages of its sequences, for calls with few (row, head) pairs per KV head: decode
+// steps and short verify blocks - and, at any cost in speed, every shape the tensor-memory kernel does not take.
+//
+// For one row at position p and one head:  out = sum_k w_k v_k / sum_k w_k,  w_k = 2^(c q.k - m),  c = scale * log2(e),
+// over the keys p - window < k <= p, with the running maximum m and the sums kept in f32 in one pass over the keys.
+//
+// Bound: HBM.  Every K and V row of a (sequence, KV head) is read once for all the pairs of the KV head's group (up to
+// 16), which makes 16 multiply-adds per byte at most: the mma.sync path is enough, and its 16-row operand is filled
+// where a 128-row tile would be padding.
+//
+//   work    The launch's 64-key tiles, laid end to end over all cells (sequence, KV head, block of pairs), are cut into
+//           equal runs, one per persistent CTA, from lengths that only the device knows: every CTA sums up the batch by
+//           itself.  A cell that several CTAs share leaves one partial (maximum, sum, output) per CTA; the CTA that
+//           takes the cell's last ticket joins them.  No CTA waits for another.
+//   tiles   A warp owns 16 keys of every tile with a cp.async ring of its own, so that no barrier stands between tiles;
+//           page numbers are fetched one tile ahead of the copies that need them.  Rows outside the block's keys are
+//           never read: their shared-memory rows are zeros and their scores -infinity, whatever the page holds there.
+//   pairs   16-bit rows: the 16 rows of the score product are 16 pairs, products exact, weights rounded to the pages'
+//           type (half a step of the output's own type, and averaged over the keys).  f32 rows: x = h + l with two
+//           halfs, so that 8 pairs take the 16 rows and scores and outputs come out f32-grade.
+#include <type_traits>
+
+#include "attn_common.cuh"
+#include "paged.cuh"
+
+namespace itk {
+namespace paged {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr uint32_t kTile = 64;   // keys of a tile, 16 per warp
+constexpr uint32_t kMinRun = 2;  // tiles a CTA takes at least
+constexpr float kRescaleStep = 8.f;  // log2 of the growth of a maximum that triggers a rescale
+constexpr int kJoinBatch = 8;        // parts requested at a time when a cell is joined
+
+template <typename T>
+struct RowTraits;  // PAIRS: (row, head) pairs of a block
+template <>
+struct RowTraits<float> {
+    using Page = __half;
+    static constexpr uint32_t kPairs = 8;
+};
+template <>
+struct RowTraits<__half> {
+    using Page = __half;
+    static constexpr uint32_t kPairs = 16;
+};
+template <>
+struct RowTraits<__nv_bfloat16> {
+    using Page = __nv_bfloat16;
+    static constexpr uint32_t kPairs = 16;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename P>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<P, __half>::value)
+        mma_16816(c, a, b0, b1);
+    else
+        mma_bf16(c, a, b0, b1);
+}
+__device__ __forceinline__ uint32_t pack2(__half, float x, float y) { return pack_half2(__float2half_rn(x), __float2half_rn(y)); }
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A sequence as the walk over the batch sees it.
+struct SeqInfo {
+    uint32_t row0, rows, len;
+};
+
+// Where a walk over a CTA's run stands: a cell and, inside it, the 64-key tiles [t, t_end) that are left to do.
+struct Cursor {
+    uint64_t pos, next;    // run position of the cell's first tile here, and of what follows it
+    uint32_t s, kvh, b;    // sequence, KV head, block of pairs
+    uint32_t blocks, T;    // of the sequence: blocks of pairs, tiles reserved for each cell
+    uint32_t tile0;        // (reserved tile number the run enters the cell at)
+    uint32_t row0, rows, len;
+    uint32_t t, t_end;
+    uint32_t lo, hi;  // keys any row of the block sees
+    bool fresh, done;
+};
+
+template <int D, int STAGES>
+__host__ __device__ constexpr size_t pipe_bytes() {
+    return static_cast<size_t>(STAGES) * kWarps * 2 * 16 * D * 2;
+}
+template <int D, int STAGES>
+size_t smem_bytes(uint32_t n_seqs) {
+    return pipe_bytes<D, STAGES>() + 2 * kWarps * 16 * sizeof(float) + 32 + (n_seqs + 1) * sizeof(uint64_t) + n_seqs * sizeof(SeqInfo);
+}
+
+template <typename T, int D, int STAGES>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kernel(const __grid_constant__ AttnParams p) {
+    using P = typename RowTraits<T>::Page;
+    constexpr uint32_t PB = RowTraits<T>::kPairs;
+    constexpr bool SPLIT = PB == 8;  // two-term f32 rows
+    constexpr uint32_t kRowBytes = D * 2, kSlice = 16 * kRowBytes;
+    constexpr uint32_t CH = D / 8;            // 16-byte chunks of a row
+    constexpr uint32_t kPassRows = 32 / CH;   // rows a warp copies at a time
+    constexpr uint32_t kPasses = 16 / kPassRows;
+    constexpr int KS = D / 16, NT = D / 8;
+
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* wm = reinterpret_cast<float*>(smem + pipe_bytes<D, STAGES>());  // [warp][16]
+    float* wl = wm + kWarps * 16;
+    uint32_t* s_flag = reinterpret_cast<uint32_t*>(wl + kWarps * 16);
+    uint64_t* s_warp = reinterpret_cast<uint64_t*>(s_flag + 8);
+    uint64_t* prefix = s_warp;  // [n_seqs + 1]; its head doubles as the scan's scratch before it is filled
+    SeqInfo* info = reinterpret_cast<SeqInfo*>(prefix + p.batch.n_seqs + 1);
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    const uint32_t n_seqs = p.batch.n_seqs, G = gridDim.x, cta = blockIdx.x;
+    const uint32_t group = p.group, head_dim = p.pool.head_dim, shift = p.pool.page_shift;
+
+    // ---- the batch summed up: prefix[s] = tiles reserved before sequence s -----------------------------------------
+    // A cell's block of pairs reserves the tiles of its whole sequence (of its first row's window to its last key);
+    // tiles that the block does not see are passed over in the walk.
+    auto geometry = [&](uint32_t rows, uint32_t len, uint32_t& lo_t, uint32_t& tiles, uint32_t& blocks) {
+        const int32_t pos0 = static_cast<int32_t>(len) - static_cast<int32_t>(rows);
+        lo_t = p.window != 0 && pos0 >= 0 && static_cast<uint32_t>(pos0) >= p.window ? (pos0 + 1 - p.window) / kTile : 0u;
+        const uint32_t hi_t = (len + kTile - 1) / kTile;
+        tiles = hi_t > lo_t ? hi_t - lo_t : 1u;
+        blocks = (rows * group + PB - 1) / PB;
+    };
+    const uint32_t each = (n_seqs + kThreads - 1) / kThreads;
+    uint64_t mine = 0;
+    for (uint32_t i = 0; i < each; ++i) {
+        const uint32_t s = tid * each + i;
+        if (s >= n_seqs) break;
+        Batch b = p.batch;
+        if (cta != 0) b.status = nullptr;  // one CTA reports
+        const Seq q = seq_of(b, s, shift);
+        info[s] = SeqInfo{q.row0, q.rows, q.len};
+        uint32_t lo_t, tiles, blocks;
+        geometry(q.rows, q.len, lo_t, tiles, blocks);
+        mine += static_cast<uint64_t>(tiles) * blocks * p.pool.kv_heads;
+    }
+    uint64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= static_cast<uint32_t>(d)) incl += o;
+    }
+    uint64_t* const wsum = reinterpret_cast<uint64_t*>(wm);  // [4], before the walk needs it
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    uint64_t before = incl - mine, W = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        if (w < warp) before += wsum[w];
+        W += wsum[w];
+    }
+    for (uint32_t i = 0; i < each; ++i) {
+        const uint32_t s = tid * each + i;
+        if (s >= n_seqs) break;
+        prefix[s] = before;
+        uint32_t lo_t, tiles, blocks;
+        geometry(info[s].rows, info[s].len, lo_t, tiles, blocks);
+        before += static_cast<uint64_t>(tiles) * blocks * p.pool.kv_heads;
+    }
+    if (tid == 0) prefix[n_seqs] = W;
+    __syncthreads();
+    uint64_t per = (W + G - 1) / G;
+    if (per < kMinRun) per = kMinRun;
+    const uint64_t run0 = cta * per, run1 = min(W, run0 + per);
+    if (run0 >= run1) return;
+
+    // ---- the walk ----------------------------------------------------------------------------------------------------
+    auto open_seq = [&](Cursor& c) {
+        const SeqInfo q = info[c.s];
+        c.row0 = q.row0;
+        c.rows = q.rows;
+        c.len = q.len;
+        uint32_t lo_t;
+        geometry(q.rows, q.len, lo_t, c.T, c.blocks);
+    };
+    auto open_cell = [&](Cursor& c, uint32_t tile) {  // entered at reserved tile `tile`
+        uint32_t lo_t, tiles, blocks;
+        geometry(c.rows, c.len, lo_t, tiles, blocks);
+        const uint32_t n = static_cast<uint32_t>(min(run1 - c.pos, static_cast<uint64_t>(c.T - tile)));
+        c.next = c.pos + n;
+        c.tile0 = tile;
+        const uint32_t r0 = c.b * PB / group, r1 = (min(c.rows * group, (c.b + 1) * PB) - 1) / group;
+        const int32_t pos0 = static_cast<int32_t>(c.len) - static_cast<int32_t>(c.rows);
+        const int32_t first = pos0 + static_cast<int32_t>(r0), last = pos0 + static_cast<int32_t>(r1);
+        c.hi = last >= 0 ? static_cast<uint32_t>(last) + 1u : 0u;
+        c.lo = p.window != 0 && first >= 0 && static_cast<uint32_t>(first) >= p.window ? first + 1 - p.window : 0u;
+        c.t = max(lo_t + tile, c.lo / kTile);
+        c.t_end = min(lo_t + tile + n, (c.hi + kTile - 1) / kTile);
+        if (c.t >= c.t_end) {  // nothing to see here: one empty step, so that the cell is still finished
+            c.t = 0;
+            c.t_end = 1;
+            c.lo = c.hi = 0;
+        }
+        c.fresh = true;
+    };
+    auto step = [&](Cursor& c) {
+        c.fresh = false;
+        if (++c.t < c.t_end) return;
+        c.pos = c.next;
+        if (c.pos >= run1) {
+            c.done = true;
+            return;
+        }
+        if (c.pos >= prefix[c.s + 1]) {
+            do ++c.s;
+            while (c.pos >= prefix[c.s + 1]);
+            c.kvh = c.b = 0;
+            open_seq(c);
+        } else if (++c.b == c.blocks) {
+            c.b = 0;
+            ++c.kvh;
+        }
+        open_cell(c, 0);
+    };
+    Cursor C;
+    {
+        uint32_t lo = 0, hi = n_seqs;  // the last sequence that begins at or before run0 and is not empty
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (prefix[mid] <= run0)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        C.s = lo;
+        C.pos = run0;
+        C.done = false;
+        open_seq(C);
+        const uint64_t in = run0 - prefix[lo];
+        const uint64_t cell = in / C.T;
+        C.kvh = static_cast<uint32_t>(cell / C.blocks);
+        C.b = static_cast<uint32_t>(cell % C.blocks);
+        open_cell(C, static_cast<uint32_t>(in % C.T));
+    }
+    Cursor L = C;  // the copies' walk, STAGES - 1 tiles ahead
+
+    // ---- copies ------------------------------------------------------------------------------------------------------
+    const uint32_t pipe = smem_u32(smem) + warp * (STAGES * 2 * kSlice);
+    const uint32_t chunk = lane % CH, prow = lane / CH;
+    const bool live_chunk = chunk * 8 < head_dim;
+    const P* const kc = static_cast<const P*>(p.pool.k) + chunk * 8;
+    const P* const vc = static_cast<const P*>(p.pool.v) + chunk * 8;
+    const uint32_t row_mask = (1u << shift) - 1u;
+    // The number of the page that holds row (lane % 16) of the slice at L, one step ahead of its use.
+    auto page_of = [&]() -> uint32_t {
+        const uint32_t key = L.t * kTile + warp * 16 + (lane & 15);
+        const uint32_t inside = min(max(key, L.lo), L.hi - 1u);  // rows outside the block's keys are not read
+        if (L.done || L.hi == 0) return 0u;
+        return __ldg(p.batch.table + static_cast<size_t>(L.s) * p.batch.table_stride + (inside >> shift));
+    };
+    uint32_t page = page_of();
+    auto request = [&](uint32_t stage) {
+        const uint32_t key0 = L.t * kTile + warp * 16;
+        const uint32_t a = L.lo > key0 ? min(L.lo - key0, 16u) : 0u, b = L.hi > key0 ? min(L.hi - key0, 16u) : 0u;
+        if (a < b) {  // rows [a, b) of the slice are read, the others become zeros
+            const bool bad = page >= p.pool.n_pages;
+            if (bad) raise(p.batch, kBadPage);
+            const uint32_t ks = pipe + stage * (2 * kSlice), vs = ks + kSlice;
+            const uint64_t head = static_cast<uint64_t>(L.kvh) * p.pool.head_stride;
+            if (shift >= 4) {  // a slice lies in one page
+                const uint64_t base = bad ? 0u : page * p.pool.page_stride + (key0 & row_mask) * p.pool.row_stride + head;
+                const uint64_t jump = bad ? 0u : p.pool.row_stride;
+#pragma unroll
+                for (uint32_t i = 0; i < kPasses; ++i) {
+                    const uint32_t r = prow + i * kPassRows;
+                    const uint32_t n = live_chunk && !bad && r >= a && r < b ? 16u : 0u;
+                    const uint64_t off = n ? base + r * jump : 0u;
+                    const uint32_t so = r * kRowBytes + ((chunk ^ (r & 7)) << 4);
+                    cp_async16(ks + so, kc + off, n);
+                    cp_async16(vs + so, vc + off, n);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kPasses; ++i) {
+                    const uint32_t r = prow + i * kPassRows;
+                    const uint32_t pg = __shfl_sync(0xffffffffu, page, r);
+                    const uint32_t n = live_chunk && pg < p.pool.n_pages && r >= a && r < b ? 16u : 0u;
+                    const uint64_t off = n ? pg * p.pool.page_stride + ((key0 + r) & row_mask) * p.pool.row_stride + head : 0u;
+                    const uint32_t so = r * kRowBytes + ((chunk ^ (r & 7)) << 4);
+                    cp_async16(ks + so, kc + off, n);
+                    cp_async16(vs + so, vc + off, n);
+                }
+            }
+        }
+        step(L);
+        page = page_of();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < STAGES - 1; ++i) {
+        if (!L.done) request(i);
+        cp_async_commit();
+    }
+
+    // ---- the pass over the run -----------------------------------------------------------------------------------------
+    uint32_t qf[KS][4];
+    float o[NT][4];
+    float m[2], l[2];       // rows g and g + 8 of the score product (f32 rows: row g alone)
+    int32_t at[2];          // their positions; below zero: sees nothing
+    uint32_t stage = 0;
+    while (!C.done) {
+        const int32_t pos0 = static_cast<int32_t>(C.len) - static_cast<int32_t>(C.rows);
+        if (C.fresh) {
+            const uint32_t pairs = C.rows * group;
+            const T* qp[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t pair = C.b * PB + g + (SPLIT ? 0 : 8 * j);
+                const bool has = pair < pairs;
+                const uint32_t row = has ? pair / group : 0u;
+                at[j] = has ? pos0 + static_cast<int32_t>(row) : -1;
+                qp[j] = has ? static_cast<const T*>(p.q) + static_cast<uint64_t>(C.row0 + row) * p.q_row +
+                                  (C.kvh * group + pair % group) * head_dim
+                            : nullptr;
+                m[j] = -INFINITY;
+                l[j] = 0.f;
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // channels 16 ks + 8 e + 2 tq and the next
+                    const uint32_t d = 16 * ks + 8 * e + 2 * tq;
+                    if constexpr (SPLIT) {
+                        float2 x = make_float2(0.f, 0.f);
+                        if (qp[0] && d < head_dim) x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(qp[0]) + d);
+                        __half h0, l0, h1, l1;
+                        split_half(x.x, h0, l0);
+                        split_half(x.y, h1, l1);
+                        qf[ks][2 * e] = pack_half2(h0, h1);
+                        qf[ks][2 * e + 1] = pack_half2(l0, l1);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            qf[ks][2 * e + j] = qp[j] && d < head_dim ? *reinterpret_cast<const uint32_t*>(qp[j] + d) : 0u;
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        }
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        if (!L.done) request(stage == 0 ? STAGES - 1 : stage - 1);
+        cp_async_commit();
+
+        const uint32_t key0 = C.t * kTile + warp * 16;
+        if (key0 < C.hi && key0 + 16 > C.lo) {
+            const uint32_t ks0 = pipe + stage * (2 * kSlice), vs0 = ks0 + kSlice;
+            float sc[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t kb[4];
+                const uint32_t r = ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
+                ldmatrix_x4(kb, ks0 + r * kRowBytes + ((c ^ (r & 7)) << 4));
+                mma<P>(sc[0], qf[ks], kb[0], kb[1]);
+                mma<P>(sc[1], qf[ks], kb[2], kb[3]);
+            }
+            // w[j][n][e]: row g + 8 j, key 8 n + 2 tq + e of the slice
+            constexpr int J = SPLIT ? 1 : 2;
+            float w[J][2][2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (SPLIT) {
+                        w[0][n][e] = (sc[n][e] + sc[n][e + 2]) * p.scale_log2;
+                    } else {
+                        w[0][n][e] = sc[n][e] * p.scale_log2;
+                        w[1][n][e] = sc[n][e + 2] * p.scale_log2;
+                    }
+                }
+            bool grows = false;
+            float top[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int32_t low = p.window != 0 ? at[j] - static_cast<int32_t>(min(p.window, 0x7fffffffu)) : -1;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int32_t key = static_cast<int32_t>(key0 + 8 * n + 2 * tq + e);
+                        if (key > at[j] || key <= low) w[j][n][e] = -INFINITY;
+                    }
+                top[j] = fmaxf(fmaxf(w[j][0][0], w[j][0][1]), fmaxf(w[j][1][0], w[j][1][1]));
+                top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+                top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
+                grows = grows || top[j] > m[j] + kRescaleStep || (m[j] == -INFINITY && top[j] != -INFINITY);
+            }
+            if (__any_sync(0xffffffffu, grows)) {
+                float f[2];
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const float to = fmaxf(m[j], top[j]);
+                    f[j] = m[j] == -INFINITY ? 0.f : fast_exp2(m[j] - to);
+                    m[j] = to;
+                    l[j] *= f[j];
+                }
+                if constexpr (SPLIT) f[1] = f[0];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[n][0] *= f[0];
+                    o[n][1] *= f[0];
+                    o[n][2] *= f[1];
+                    o[n][3] *= f[1];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float base = m[j] == -INFINITY ? 0.f : m[j];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[j][n][e] = fast_exp2(w[j][n][e] - base);
+                        l[j] += w[j][n][e];
+                    }
+            }
+            uint32_t pa[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                if constexpr (SPLIT) {
+                    __half h0, l0, h1, l1;
+                    split_half(w[0][n][0], h0, l0);
+                    split_half(w[0][n][1], h1, l1);
+                    pa[2 * n] = pack_half2(h0, h1);
+                    pa[2 * n + 1] = pack_half2(l0, l1);
+                } else {
+                    pa[2 * n] = pack2(P(), w[0][n][0], w[0][n][1]);
+                    pa[2 * n + 1] = pack2(P(), w[1][n][0], w[1][n][1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t vb[4];
+                const uint32_t r = lane & 15, c = n + (lane >> 4);
+                ldmatrix_x4_trans(vb, vs0 + r * kRowBytes + ((c ^ (r & 7)) << 4));
+                mma<P>(o[n], pa, vb[0], vb[1]);
+                mma<P>(o[n + 1], pa, vb[2], vb[3]);
+            }
+        }
+
+        if (C.t + 1 == C.t_end) {
+            // ---- the run's part of the cell is complete: join the warps ----------------------------------------------
+            // The stage just used (of every warp) holds the warp's output rows, PB x D floats; columns are twisted by
+            // the row so that the eight rows a warp writes at a time spread over the banks.
+            __syncwarp();
+            float* const ex = reinterpret_cast<float*>(smem + warp * (STAGES * 2 * kSlice) + stage * (2 * kSlice));
+#pragma unroll
+            for (int j = 0; j < (SPLIT ? 1 : 2); ++j) {
+                l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+                l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+                if (tq == 0) {
+                    wm[warp * 16 + g + 8 * j] = m[j];
+                    wl[warp * 16 + g + 8 * j] = l[j];
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float2 x = make_float2(o[n][2 * j], o[n][2 * j + 1]);
+                    if constexpr (SPLIT) x = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+                    *reinterpret_cast<float2*>(ex + (g + 8 * j) * D + ((8 * n + 2 * tq) ^ (8 * (g & 7)))) = x;
+                }
+            }
+            __syncthreads();
+            const uint32_t pairs = min(C.rows * group - C.b * PB, PB);
+            const bool whole = C.tile0 == 0 && C.next - C.pos == C.T;  // no other CTA has a part of the cell
+            const uint64_t cell0 = C.pos - C.tile0;
+            const uint32_t first = whole ? cta : static_cast<uint32_t>(cell0 / per);
+            const uint32_t last = whole ? cta : static_cast<uint32_t>((cell0 + C.T - 1) / per);
+            const uint32_t part = C.tile0 == 0 ? 2 * cta + 1 : 2 * cta;
+            const uint32_t cols = head_dim / 4;
+            auto write = [&](uint32_t pair, uint32_t c4, float4 v, float top, float sum) {
+                const uint32_t abs_pair = C.b * PB + pair;
+                const uint32_t row = abs_pair / group, head = C.kvh * group + abs_pair % group;
+                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                T* dst = static_cast<T*>(p.out) + static_cast<uint64_t>(C.row0 + row) * p.out_row + head * head_dim + 4 * c4;
+                const float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+                if constexpr (SPLIT) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                } else {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(P(), x[0], x[1]), pack2(P(), x[2], x[3]));
+                }
+                if (c4 == 0 && p.lse)
+                    p.lse[static_cast<uint64_t>(C.row0 + row) * p.q_heads + head] =
+                        sum > 0.f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+            };
+            for (uint32_t i = tid; i < pairs * cols; i += kThreads) {
+                const uint32_t pair = i / cols, c4 = i % cols;
+                float top = wm[pair];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, wm[w * 16 + pair]);
+                float sum = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float f = wm[w * 16 + pair] == -INFINITY ? 0.f : fast_exp2(wm[w * 16 + pair] - top);
+                    sum += f * wl[w * 16 + pair];
+                    const float4 x = *reinterpret_cast<const float4*>(
+                        reinterpret_cast<const float*>(smem + w * (STAGES * 2 * kSlice) + stage * (2 * kSlice)) + pair * D +
+                        ((4 * c4) ^ (8 * (pair & 7))));
+                    v.x += f * x.x;
+                    v.y += f * x.y;
+                    v.z += f * x.z;
+                    v.w += f * x.w;
+                }
+                if (whole) {
+                    write(pair, c4, v, top, sum);
+                } else {
+                    reinterpret_cast<float4*>(p.part_o + (static_cast<size_t>(part) * 16 + pair) * D)[c4] = v;
+                    if (c4 == 0) reinterpret_cast<float2*>(p.part_ml)[part * 16 + pair] = make_float2(top, sum);
+                }
+            }
+            __syncthreads();  // the stage may be filled again, and every store of the part is done
+            if (!whole) {
+                if (tid == 0) {
+                    __threadfence();  // cumulative over the CTA's stores above (ordered before the barrier)
+                    const unsigned int ticket = atomicAdd(p.tickets + first, 1u);
+                    *s_flag = ticket == last - first ? 1u : 0u;
+                    if (ticket == last - first) p.tickets[first] = 0u;  // as the next launch wants it
+                }
+                __syncthreads();
+                if (*s_flag != 0u) {
+                    __threadfence();
+                    // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...
+                    for (uint32_t i = tid; i < pairs * cols; i += kThreads) {
+                        const uint32_t pair = i / cols, c4 = i % cols;
+                        float top = -INFINITY, sum = 0.f;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (uint32_t c0 = first; c0 <= last; c0 += kJoinBatch) {
+                            float2 ml[kJoinBatch];
+                            float4 x[kJoinBatch];
+#pragma unroll
+                            for (int u = 0; u < kJoinBatch; ++u) {
+                                const uint32_t c = min(c0 + u, last), slot = c == first ? 2 * c + 1 : 2 * c;
+                                ml[u] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot * 16 + pair);
+                                x[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (static_cast<size_t>(slot) * 16 + pair) * D) + c4);
+                            }
+                            float to = top;
+#pragma unroll
+                            for (int u = 0; u < kJoinBatch; ++u) to = fmaxf(to, ml[u].x);
+                            const float f0 = top == -INFINITY ? 0.f : fast_exp2(top - to);
+                            sum *= f0;
+                            v.x *= f0, v.y *= f0, v.z *= f0, v.w *= f0;
+                            top = to;
+#pragma unroll
+                            for (int u = 0; u < kJoinBatch; ++u) {
+                                const float f = c0 + u <= last && ml[u].x != -INFINITY ? fast_exp2(ml[u].x - top) : 0.f;
+                                sum += f * ml[u].y;
+                                v.x += f * x[u].x, v.y += f * x[u].y, v.z += f * x[u].z, v.w += f * x[u].w;
+                            }
+                        }
+                        write(pair, c4, v, top, sum);
+                    }
+                    __syncthreads();  // before s_flag is written again
+                }
+            }
+        }
+        step(C);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+}
+
+template <typename F>
+cudaError_t by_shape(uint32_t head_dim, int32_t row_dtype, F&& f) {
+    auto by_dim = [&](auto row) {
+        using T = decltype(row);
+        if (head_dim <= 64) return f(paged_stream_kernel<T, 64, 4>, smem_bytes<64, 4>);
+        if (head_dim <= 128) return f(paged_stream_kernel<T, 128, 3>, smem_bytes<128, 3>);
+        return f(paged_stream_kernel<T, 256, 3>, smem_bytes<256, 3>);
+    };
+    if (row_dtype == ITK_ROW_F32) return by_dim(float());
+    if (row_dtype == ITK_ROW_F16) return by_dim(__half());
+    return by_dim(__nv_bfloat16());
+}
+
+}  // namespace
+
+cudaError_t launch_stream(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s) {
+    return by_shape(p.pool.head_dim, row_dtype, [&](auto kernel, auto bytes_of) {
+        const size_t bytes = bytes_of(p.batch.n_seqs);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes_of(kMaxSeqs)));
+        if (e != cudaSuccess) return e;
+        kernel<<<stream_ctas(sms, p.pool.head_dim), kThreads, bytes, s>>>(p);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace paged
+}  // namespace itk

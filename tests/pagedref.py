@@ -1,0 +1,148 @@
+"""The paged operators from their definitions, in 64 bits on the host, one row and head at a time, and how far a device
+result may be from them.
+
+Rounding one value to a type t is off by at most u = eps(t) / 2 of it (bf16 2^-8, f16 2^-11, f32 2^-24)."""
+import math
+
+import numpy as np
+import torch
+
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+PAGE = {torch.float32: torch.float16, torch.float16: torch.float16, torch.bfloat16: torch.bfloat16}
+
+
+def rotate(x, positions, inv_freq, pairing, magnitude=1.0, inverse=False):
+    """x [rows][heads][D] f64 tensor, as complex pairs times magnitude * exp(+-i angle)."""
+    x = x.double().clone()
+    n = len(inv_freq)
+    a = torch.arange(n) * (2 if pairing == 0 else 1)
+    b = a + (1 if pairing == 0 else n)
+    angle = torch.as_tensor(positions, dtype=torch.float64)[:, None] * torch.as_tensor(np.asarray(inv_freq), dtype=torch.float64)
+    z = torch.complex(x[..., a], x[..., b]) * torch.polar(torch.full_like(angle, magnitude), -angle if inverse else angle)[:, None]
+    x[..., a], x[..., b] = z.real, z.imag
+    return x
+
+
+def rotation_bound(x, inv_freq, pairing, magnitude, t):
+    """|x_a cos - x_b sin| in f32: sine and cosine are within 2^-24 * pi (the reduced angle's rounding, at most half a
+    turn of half turns) + 2 * 2^-24 (sincospif, 1 ulp-grade, and the product with the magnitude) of the exact ones; two products and a sum
+    round 3 times more: 9 * 2^-24 of |x_a| + |x_b| covers it.  Then one rounding to t."""
+    n = len(inv_freq)
+    a = torch.arange(n) * (2 if pairing == 0 else 1)
+    b = a + (1 if pairing == 0 else n)
+    size = x.double().abs().clone()
+    both = (x.double()[..., a].abs() + x.double()[..., b].abs()) * abs(magnitude)
+    size[..., a], size[..., b] = both, both
+    extra = torch.zeros(x.shape[-1], dtype=torch.float64)
+    extra[a], extra[b] = 9 * 2.0 ** -24, 9 * 2.0 ** -24
+    return size * extra, size
+
+
+def within(got, want, err, t):
+    """|got - want| <= err + one rounding to t (and t's subnormal step)."""
+    got, want = got.double().cpu(), want.double()
+    tiny = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[t]
+    off = (got - want).abs()
+    bound = err * (1 + U[t]) + U[t] * want.abs() + tiny
+    bad = off > bound
+    assert not bool(bad.any()) and bool(torch.isfinite(got).all()), (
+        f"{int(bad.sum())} of {bad.numel()} values off, worst {float((off - bound).max()):.3e} over a bound of "
+        f"{float(bound.reshape(-1)[int((off - bound).argmax())]):.3e}")
+
+
+def attend(q, keys, values, pos0, scale, window):
+    """One sequence: q [rows][Hq][D], keys / values [n][Hkv][D] (f64): (out, lse, mean, slack).  mean = sum of weight *
+    |value|: what the rounding of weights and sums is proportional to; slack = the f32 score's error bound."""
+    rows, hq, d = q.shape
+    n, hkv, _ = keys.shape
+    out = torch.zeros(rows, hq, d, dtype=torch.float64)
+    lse = torch.full((rows, hq), -math.inf, dtype=torch.float64)
+    mean, slack = torch.zeros_like(out), torch.zeros(rows, hq, dtype=torch.float64)
+    for r in range(rows):
+        p = pos0 + r
+        lo, hi = (max(0, p - window + 1) if window else 0), p + 1
+        if p < 0 or hi <= lo:
+            continue
+        for h in range(hq):
+            k, v = keys[lo:hi, h // (hq // hkv)], values[lo:hi, h // (hq // hkv)]
+            s = k @ q[r, h] * scale
+            top = s.max()
+            w = torch.exp(s - top)
+            lse[r, h] = top + w.sum().log()
+            out[r, h] = (w / w.sum()) @ v
+            mean[r, h] = (w / w.sum()) @ v.abs()
+            slack[r, h] = (k.abs() @ q[r, h].abs()).max() * abs(scale)
+    return out, lse, mean, slack
+
+
+def attend_bound(mean, slack, n, d, t):
+    """How far an output may be, before its own rounding: scores are sums of d products in f32 (and, for f32 rows, of
+    products good to 2^-21 of their size), so a weight is off by the factor 1 +- 2 e with e = (d + 16) 2^-24 * slack; the
+    weight itself is rounded to the pages' type for 16-bit rows (u) and to two halfs for f32 rows (2^-21, and 2^-23 of
+    the exponential); sums over n keys run in f32 in steps of 16 keys; joins and the quotient add a few roundings."""
+    weight = 2.0 ** -21 if t is torch.float32 else U[t]
+    e = 2 * ((d + 16) * 2.0 ** -24 + (2.0 ** -21 if t is torch.float32 else 0.0)) * slack
+    return mean * (weight + (n / 16 + 64) * 2.0 ** -24 + e[..., None])
+
+
+class Batch:
+    """A ragged batch on the device with its host copies: ``rows`` and ``lens`` per sequence, pages scattered over the pool
+    whose unused rows hold NaN."""
+
+    def __init__(self, rows, lens, hq, hkv, d, t, page, layout, seed=0, extra_rows=0, spare=2, width=None, device="cuda"):
+        g = torch.Generator().manual_seed(seed)
+        self.rows, self.lens, self.hq, self.hkv, self.d, self.t, self.page, self.layout = rows, lens, hq, hkv, d, t, page, layout
+        pt = PAGE[t]
+        held = [-(-n // page) for n in lens]
+        self.n_pages = sum(held) + spare
+        self.width = max(1, max(held)) if width is None else width
+        order = torch.randperm(self.n_pages, generator=g).tolist()
+        table = torch.full((len(rows), self.width), -1, dtype=torch.int32)
+        i = 0
+        for s, n in enumerate(held):
+            table[s, :n] = torch.tensor(order[i:i + n], dtype=torch.int32)
+            i += n
+        self.table_h = table
+        self.keys = [torch.randn(n, hkv, d, generator=g).to(pt) for n in lens]
+        self.values = [torch.randn(n, hkv, d, generator=g).to(pt) for n in lens]
+        shape = (self.n_pages, hkv, page, d) if layout == "head" else (self.n_pages, page, hkv, d)
+        self.k_h, self.v_h = (torch.full(shape, math.nan, dtype=pt) for _ in range(2))
+        for s, n in enumerate(lens):
+            for p in range(n):
+                for pool, src in ((self.k_h, self.keys), (self.v_h, self.values)):
+                    self.cell(pool, int(table[s, p // page]), p % page).copy_(src[s][p])
+        starts = [0]
+        for r in rows:
+            starts.append(starts[-1] + r)
+        self.total = starts[-1] + extra_rows
+        self.starts = starts
+        self.q_h = torch.randn(self.total, hq, d, generator=g).to(t)
+        self.k = self.k_h.to(device)
+        self.v = self.v_h.to(device)
+        self.table = table.to(device)
+        self.row_start = torch.tensor(starts, dtype=torch.int32, device=device)
+        self.kv_len = torch.tensor(lens, dtype=torch.int32, device=device)
+        self.q = self.q_h.to(device)
+
+    def cell(self, pool, page, row):
+        """[kv_heads][D] view of one row of one page."""
+        return pool[page, :, row] if self.layout == "head" else pool[page, row]
+
+    def check(self, out, lse=None, scale=None, window=0, only=None):
+        scale = 1.0 / math.sqrt(self.d) if scale is None else scale
+        scale = float(np.float32(scale))
+        for s, (r, n) in enumerate(zip(self.rows, self.lens)):
+            if r == 0 or (only is not None and s not in only):
+                continue
+            lo = self.starts[s]
+            want, want_lse, mean, slack = attend(self.q_h[lo:lo + r].double(), self.keys[s].double(), self.values[s].double(),
+                                                 n - r, scale, window)
+            err = attend_bound(mean, slack, n, self.d, self.t)
+            within(out[lo:lo + r], want, err, self.t)
+            if lse is not None:
+                got = lse[lo:lo + r].double().cpu()
+                seen = torch.isfinite(want_lse)
+                assert torch.equal(torch.isfinite(got), seen) and bool((got[~seen] == -math.inf).all())
+                # the score's error, the sum's, and log2 and its product in f32
+                tol = (self.d + 16) * 2.0 ** -24 * slack + 2.0 ** -20 * slack + (n / 16 + 64) * 2.0 ** -24 + 8 * 2.0 ** -24 * want_lse.abs()
+                assert bool(((got - want_lse).abs()[seen] <= tol[seen]).all()), float((got - want_lse).abs()[seen].max())

@@ -1,0 +1,597 @@
+"""The paged operators on the device against their definitions in 64 bits (``pagedref``), with tolerances derived there."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from itak_torch_rebuild_b200 import CudaComputeError, _lib, paged
+from pagedref import PAGE, U, Batch, rotate, rotation_bound, within
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+NAN = math.nan
+
+
+def table(rot, dev="cuda", **kw):
+    f, m = paged.rope_table(rot, 10000.0, **kw)
+    return f, torch.from_numpy(f).to(dev), m
+
+
+# ---- rotation ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pairing", [0, 1])
+@pytest.mark.parametrize("rows,heads,d,rot", [(1, 1, 2, 2), (3, 5, 64, 64), (7, 3, 96, 32), (2, 33, 128, 128), (5, 2, 80, 62),
+                                              (4, 2, 256, 256), (2, 2, 10, 6), (1, 64, 128, 48), (2, 300, 64, 2)])
+def test_rotation(t, pairing, rows, heads, d, rot):
+    g = torch.Generator().manual_seed(rows * 100 + d)
+    x = torch.randn(rows, heads, d, generator=g).to(t)
+    pos = torch.randint(0, 1 << 20, (rows,), generator=g, dtype=torch.int32)
+    pos[0] = 0
+    f, fd, _ = table(rot)
+    got = paged.rope_apply(x.cuda(), pos.cuda(), fd, pairing=pairing, magnitude=1.25)
+    extra, _ = rotation_bound(x, f, pairing, 1.25, t)
+    within(got, rotate(x, pos, f, pairing, 1.25), extra, t)
+    if rot < d:
+        assert torch.equal(got[..., rot:].cpu(), x[..., rot:])
+    inplace = x.cuda()
+    assert paged.rope_apply(inplace, pos.cuda(), fd, pairing=pairing, magnitude=1.25, out=inplace) is inplace
+    assert torch.equal(inplace, got)
+
+
+def test_rotation_at_position_zero_and_far_away():
+    f, fd, _ = table(128)
+    x = torch.randn(4, 2, 128)
+    pos = torch.tensor([0, 1, 2 ** 24 + 1, 2 ** 31 - 1], dtype=torch.int32)
+    got = paged.rope_apply(x.cuda(), pos.cuda(), fd)
+    assert torch.equal(got[0].cpu(), x[0])
+    extra, _ = rotation_bound(x, f, 0, 1.0, F32)
+    # an f64 product p * f is off by 2^-53 of up to 2^31 radians, on both sides: 2^-21 of the pair
+    size = x.double().abs().sum(-1, keepdim=True)
+    within(got, rotate(x, pos, f, 0), extra + 2.0 ** -21 * size, F32)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pairing", [0, 1])
+def test_rotation_of_strided_rows(t, pairing):
+    """Q inside a projection's output; heads outermost; rows that sixteen-byte words cannot address; a broadcast row."""
+    f, fd, _ = table(64)
+    pos = torch.arange(5, dtype=torch.int32) * 77
+    whole = torch.randn(5, 9, 64).to(t).cuda()
+    out = torch.full((5, 9, 64), NAN, dtype=t, device="cuda")
+    views = [(whole[:, 2:6], out[:, 2:6]), (whole.transpose(0, 1).contiguous().transpose(0, 1)[:, :4], torch.empty(4, 5, 64, dtype=t, device="cuda").transpose(0, 1)),
+             (torch.randn(5, 4, 67).to(t).cuda()[..., 1:65], torch.empty(5, 4, 66, dtype=t, device="cuda")[..., :64]),
+             (whole[:1].expand(5, 9, 64)[:, 3:7], torch.empty(5, 4, 64, dtype=t, device="cuda"))]
+    for x, o in views:
+        paged.rope_apply(x, pos.cuda(), fd, pairing=pairing, out=o)
+        extra, _ = rotation_bound(x.cpu(), f, pairing, 1.0, t)
+        within(o, rotate(x.cpu(), pos, f, pairing), extra, t)
+    assert bool(torch.isnan(out[:, :2]).all()) and bool(torch.isnan(out[:, 6:]).all())
+
+
+@pytest.mark.parametrize("pairing", [0, 1])
+def test_gradient_against_the_formula_and_differences(pairing):
+    f, fd, m = table(24, scaling="ramp", factor=4.0, original_context=512.0, low=1.0, high=32.0)
+    x, gy = torch.randn(3, 2, 40), torch.randn(3, 2, 40)
+    pos = torch.tensor([5, 900, 0], dtype=torch.int32)
+    got = paged.rope_apply(gy.cuda(), pos.cuda(), fd, pairing=pairing, magnitude=m, inverse=True)
+    xa = x.double().requires_grad_()
+    a = torch.arange(12) * (2 if pairing == 0 else 1)
+    b = a + (1 if pairing == 0 else 12)
+    ang = pos.double()[:, None, None] * torch.from_numpy(f)
+    y0, y1 = m * (xa[..., a] * ang.cos() - xa[..., b] * ang.sin()), m * (xa[..., a] * ang.sin() + xa[..., b] * ang.cos())
+    loss = (y0 * gy.double()[..., a]).sum() + (y1 * gy.double()[..., b]).sum() + (xa[..., 24:] * gy.double()[..., 24:]).sum()
+    loss.backward()
+    extra, _ = rotation_bound(gy, f, pairing, m, F32)
+    within(got, xa.grad, extra, F32)
+    # differences: the map is linear, so f(x + e) - f(x) = f(e) up to rounding; one entry of every kind of channel
+    def value(z):
+        return float((paged.rope_apply(z.cuda(), pos.cuda(), fd, pairing=pairing, magnitude=m).double().cpu() * gy.double()).sum())
+    for r, h, c in [(0, 0, 0), (1, 1, 1), (1, 0, 13), (2, 1, 23), (0, 1, 39)]:
+        e = torch.zeros_like(x)
+        e[r, h, c] = 0.5
+        # two outputs of size <= 1.5 m |x + e| each rounded in f32, on both sides, times |gy|
+        slack = 8 * 16 * 2.0 ** -24 * m * float((x.abs().max() + 0.5) * gy.abs().max())
+        assert abs((value(x + e) - value(x - e)) - float(got[r, h, c])) <= slack
+
+
+def test_rotation_refuses_on_the_python_side():
+    f, fd, _ = table(64)
+    x, pos = torch.randn(4, 2, 64).cuda(), torch.zeros(4, dtype=torch.int32).cuda()
+    for bad in (dict(positions=pos.long()), dict(positions=pos[:3]), dict(inv_freq=fd.float()), dict(x=x.double()), dict(x=x.cpu()),
+                dict(out=torch.empty(4, 2, 64, dtype=F16, device="cuda")), dict(out=x[:2]), dict(inv_freq=torch.zeros(0, dtype=torch.float64, device="cuda")),
+                dict(x=x[..., ::2]), dict(x=x[:0], positions=pos[:0])):
+        kw = dict(x=x, positions=pos, inv_freq=fd)
+        kw.update(bad)
+        with pytest.raises(CudaComputeError):
+            paged.rope_apply(kw.pop("x"), kw.pop("positions"), kw.pop("inv_freq"), **kw)
+
+
+# ---- append -----------------------------------------------------------------------------------------------------------
+
+
+def check_append(b, k, v, q, f, pairing, q_out, status=None):
+    """Every page row is either one of the batch's new rows or untouched."""
+    pt = PAGE[b.t]
+    want_k, want_v = b.k_h.clone(), b.v_h.clone()
+    seen = torch.zeros(b.n_pages, b.page, dtype=torch.bool)
+    for s, (r, n) in enumerate(zip(b.rows, b.lens)):
+        lo = b.starts[s]
+        for i in range(r):
+            p = n - r + i
+            page = int(b.table_h[s, p // b.page]) if p >= 0 else -1
+            if p < 0 or not 0 <= page < b.n_pages:
+                continue
+            seen[page, p % b.page] = True
+            for pool, src, turned in ((b.k, k, True), (b.v, v, False)):
+                row = src[lo + i].cpu()
+                got = b.cell(pool.cpu(), page, p % b.page)
+                if turned and f is not None:
+                    extra, _ = rotation_bound(row[None], f, pairing, 1.0, pt)
+                    within(got[None], rotate(row[None], [p], f, pairing), extra, pt)
+                    assert torch.equal(got[..., 2 * len(f):], row[..., 2 * len(f):].to(pt))
+                else:
+                    assert torch.equal(got, row.to(pt))
+        if q is not None and r:
+            keep = [i for i in range(r) if n - r + i >= 0]
+            if keep:
+                rows = q[lo:lo + r].cpu()[keep]
+                pos = [n - r + i for i in keep]
+                if f is None:
+                    assert torch.equal(q_out[lo:lo + r].cpu()[keep], rows)
+                else:
+                    extra, _ = rotation_bound(rows, f, pairing, 1.0, b.t)
+                    within(q_out[lo:lo + r].cpu()[keep], rotate(rows, pos, f, pairing), extra, b.t)
+    for pool, was in ((b.k.cpu(), want_k), (b.v.cpu(), want_v)):
+        by_row = pool.transpose(1, 2) if b.layout == "head" else pool
+        was = was.transpose(1, 2) if b.layout == "head" else was
+        assert torch.equal(by_row[~seen].view(torch.int16), was[~seen].view(torch.int16)), "a row outside the batch was written"
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pairing,rot", [(0, 64), (1, 64), (1, 32), (0, 6), (1, 6), (0, 0)])
+@pytest.mark.parametrize("layout,page", [("head", 16), ("token", 8), ("head", 1), ("token", 64)])
+def test_append(t, pairing, rot, layout, page):
+    b = Batch([1, 0, 9, 3, 20], [1, 5, 9, 40, 21], 6, 2, 64, t, page, layout, extra_rows=3)
+    qkv = torch.randn(b.total, 10, 64).to(t).cuda()
+    q, k, v = qkv[:, :6], qkv[:, 6:8], qkv[:, 8:]
+    f, fd, _ = table(rot) if rot else (None, None, 1.0)
+    q_out = torch.full((b.total, 6, 64), 7.0, dtype=t, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    b.k_h, b.v_h = b.k.cpu(), b.v.cpu()
+    b.cell_was = None
+    assert b and PagedOf(b).append(k, v, b.table, b.row_start, b.kv_len, q=q, q_out=q_out, inv_freq=fd, pairing=pairing, status=status) is q_out
+    check_append(b, k, v, q, f, pairing, q_out)
+    assert int(status) == 0 and bool((q_out[b.starts[-1]:] == 7.0).all())
+
+
+def PagedOf(b):
+    return paged.PagedKv(b.k, b.v, layout=b.layout)
+
+
+@pytest.mark.parametrize("d,hkv", [(8, 1), (128, 8), (256, 3), (72, 5)])
+def test_append_without_q_and_other_widths(d, hkv):
+    b = Batch([4, 2], [30, 2], hkv, hkv, d, F32, 16, "token")
+    k, v = torch.randn(b.total, hkv, d).cuda(), torch.randn(b.total, hkv, d).cuda()
+    f, fd, _ = table(min(d, 8))
+    b.k_h, b.v_h = b.k.cpu(), b.v.cpu()
+    assert PagedOf(b).append(k, v, b.table, b.row_start, b.kv_len, inv_freq=fd, pairing=1) is None
+    check_append(b, k, v, None, f, 1, None)
+
+
+def test_append_keeps_bits_of_what_it_does_not_rotate():
+    """V and the channels behind the rotated part: infinities, NaN and signed zeros as they came (f32 NaN as an append
+    stores it: sign | 0x7e00)."""
+    for t in TYPES:
+        b = Batch([2], [2], 1, 1, 16, t, 8, "head")
+        odd = torch.tensor([math.inf, -math.inf, NAN, -0.0, 0.0, 65504.0, 1e-7, -1e-8, 1.0, 2.0, 3.0, 70000.0, -70000.0, 5.0, 6.0, 7.0])
+        v = odd.to(t).repeat(2, 1, 1).cuda()
+        _, fd, _ = table(8)
+        PagedOf(b).append(v, v, b.table, b.row_start, b.kv_len, inv_freq=fd)
+        page = int(b.table_h[0, 0])
+        want = odd.to(t).to(PAGE[t])
+        got_v, got_k = b.v.cpu()[page, 0, 0], b.k.cpu()[page, 0, 0]
+        for got, part in ((got_v, slice(0, 16)), (got_k, slice(8, 16))):
+            fine = ~torch.isnan(want[part])
+            assert torch.equal(got[part][fine].view(torch.int16), want[part][fine].view(torch.int16))
+            assert bool(torch.isnan(got[part][~fine]).all())
+
+
+def test_append_drops_what_the_pool_does_not_hold():
+    """A page number outside the pool, a sequence longer than its table, rows before position 0, starts that run backwards:
+    reported, nothing else touched."""
+    b = Batch([3, 2, 2], [20, 8, 40], 2, 1, 16, F16, 8, "head")
+    b.table[1, 0] = b.n_pages  # one past the end
+    b.table_h[1, 0] = b.n_pages
+    k = torch.randn(b.total, 1, 16).half().cuda()
+    b.k_h, b.v_h = b.k.cpu(), b.v.cpu()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, status=status)
+    assert int(status) == 1
+    check_append(b, k, k, None, None, 0, None)
+
+    b = Batch([3, 2], [20, 2], 2, 1, 16, F16, 8, "head")
+    k = torch.randn(b.total, 1, 16).half().cuda()
+    b.kv_len[0], b.kv_len[1] = 1000, 1  # longer than the table; two new rows in one key
+    before = b.k.clone()
+    status.zero_()
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, status=status)
+    assert int(status) == 2 | 4
+    b.kv_len[0], b.kv_len[1] = 20, 2
+    b.row_start.copy_(torch.tensor([3, 0, 5]))
+    status.zero_()
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, status=status)
+    assert int(status) & 8
+    b.row_start.copy_(torch.tensor([0, 3, 1000]))
+    status.zero_()
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, status=status)
+    assert int(status) & 8
+    assert before.shape == b.k.shape
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+
+
+def run_attention(b, window=0, scale=None, **kw):
+    out = torch.full((b.total, b.hq, b.d), 7.0, dtype=b.t, device="cuda")
+    lse = torch.full((b.total, b.hq), 7.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = paged.attention_workspace("cuda:0")
+    n_tickets = 4 * 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), window=window, scale=scale, out=out, lse=lse,
+                         status=status, workspace=ws, **kw)
+    b.check(out, lse, scale, window)
+    assert int(status) == 0
+    assert bool((ws[:n_tickets] == 0).all()), "the workspace's tickets are not zero again"
+    assert bool((out[b.starts[-1]:] == 7.0).all()) and bool((lse[b.starts[-1]:] == 7.0).all())
+    return out, lse
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 1, 128), (3, 3, 128), (2, 1, 96), (14, 2, 128), (2, 2, 256), (5, 1, 8), (32, 2, 64), (17, 1, 80)])
+@pytest.mark.parametrize("layout,page", [("head", 16), ("token", 32)])
+def test_decode(t, hq, hkv, d, layout, page):
+    run_attention(Batch([1] * 6, [1, 16, 17, 64, 65, 301], hq, hkv, d, t, page, layout, extra_rows=2))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 64, 256])
+@pytest.mark.parametrize("layout", ["head", "token"])
+def test_blocks_of_rows_over_all_page_sizes(t, page, layout):
+    run_attention(Batch([7, 0, 1, 5, 33, 2], [7, 3, 100, 64, 150, 2], 6, 2, 64, t, page, layout, extra_rows=1))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 128), (2, 2, 64), (7, 1, 64), (2, 1, 96), (2, 1, 256), (3, 1, 40)])
+@pytest.mark.parametrize("rows,lens", [([129], [129]), ([64, 1, 0, 200], [300, 77, 5, 256]), ([130, 31], [130, 500])])
+def test_chunks(t, hq, hkv, d, rows, lens):
+    run_attention(Batch(rows, lens, hq, hkv, d, t, 16, "head", extra_rows=3))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 128, 200, 100000, 2 ** 32 - 1])
+@pytest.mark.parametrize("rows,lens", [([1, 1, 1], [5, 64, 333]), ([9, 70, 140], [9, 290, 300])])
+def test_windows(t, window, rows, lens):
+    run_attention(Batch(rows, lens, 4, 2, 64, t, 16, "token"), window=window)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_pages_behind_the_window_may_be_gone(t):
+    """Pages that no row of the call can see are not followed: their table entries may hold anything."""
+    for rows, n, window in ((1, 300, 40), (5, 300, 40), (100, 300, 40)):
+        b = Batch([rows], [n], 4, 2, 64, t, 16, "head")
+        first = n - rows - window + 1
+        for j in range(first // 16):
+            page = int(b.table_h[0, j])
+            b.k[page], b.v[page] = NAN, NAN
+            b.table[0, j] = -7
+        run_attention(b, window=window)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-30])
+def test_scales(t, scale):
+    run_attention(Batch([1, 40], [77, 90], 4, 2, 64, t, 16, "head"), scale=scale)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_large_scores_rescale_the_accumulator(t):
+    """Maxima that keep growing along the keys: every tile raises the running maximum far beyond the lazy step."""
+    for rows, n in ((1, 400), (60, 400)):
+        b = Batch([rows], [n], 4, 2, 64, t, 16, "head")
+        ramp = torch.linspace(0.1, 12.0, n)[:, None, None]
+        q = torch.ones(b.total, 4, 64) * 0.5 + 0.01 * torch.randn(b.total, 4, 64)
+        b.q_h = q.to(t)
+        b.q.copy_(b.q_h)
+        b.keys[0] = (torch.ones(n, 2, 64) * ramp + 0.01 * torch.randn(n, 2, 64)).to(PAGE[t])
+        for p in range(n):
+            b.cell(b.k, int(b.table_h[0, p // 16]), p % 16).copy_(b.keys[0][p])
+        run_attention(b)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_rows_that_see_nothing(t, rows):
+    """More new rows than keys: the rows before position 0 give zeros and -infinity, and are reported."""
+    b = Batch([rows, 1, rows], [rows + 3, 0, rows + 9], 4, 2, 64, t, 16, "head")
+    out, lse = torch.full((b.total, 4, 64), 7.0, dtype=t, device="cuda"), torch.full((b.total, 4), 7.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows, out=out, lse=lse, status=status)
+    b.check(out, lse, only=(0, 2))
+    assert int(status) == 4
+    gone = out[b.starts[1]:b.starts[2]]
+    assert bool((gone == 0).all()) and bool((lse[b.starts[1]:b.starts[2]] == -math.inf).all())
+    # and a block that reaches before the start in part
+    b = Batch([rows + 5], [rows + 5], 4, 2, 64, t, 16, "head")
+    b.kv_len[0] = rows
+    out = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows + 5, lse=(lse := torch.empty(b.total, 4, device="cuda")))
+    assert bool((out[:5] == 0).all()) and bool((lse[:5] == -math.inf).all())
+    short = Batch([rows], [rows], 4, 2, 64, t, 16, "head")
+    short.q_h, short.keys, short.values = b.q_h[5:], [b.keys[0][:rows]], [b.values[0][:rows]]
+    short.check(out[5:], lse[5:])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [1, 50])
+def test_infinite_and_nan_keys_stay_with_the_rows_that_see_them(t, rows):
+    """A NaN key reaches the rows that see it, and a key of one sequence no row of another; the pool's unused rows are NaN
+    throughout these tests."""
+    b = Batch([rows, rows], [100, 100], 4, 2, 64, t, 16, "head")
+    p = 100 - (rows + 1) // 2  # rows from this position on see it
+    page = int(b.table_h[0, p // 16])
+    b.cell(b.k, page, p % 16).fill_(NAN)
+    out = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows)
+    b.check(out, only=(1,))
+    sees = torch.tensor([100 - rows + r >= p for r in range(rows)])
+    bad = torch.isnan(out[:rows]).all(-1).all(-1).cpu()
+    assert bool(bad[sees].all()) and not bool(torch.isnan(out[:rows].cpu()[~sees]).any())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_page_numbers_outside_the_pool_are_reported_and_not_followed(t, rows):
+    b = Batch([rows, rows], [200, 120], 4, 2, 64, t, 16, "head")
+    b.table[0, 3] = b.n_pages
+    b.table[0, 5] = -1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows, status=status)
+    assert int(status) == 1
+    b.check(out, only=(1,))
+    # their keys read as zeros
+    for s in (3, 5):
+        b.keys[0][16 * s:16 * s + 16] = 0
+        b.values[0][16 * s:16 * s + 16] = 0
+    b.check(out, only=(0,))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_malformed_batches_are_cut_and_reported(rows):
+    b = Batch([rows, rows], [100, 90], 4, 2, 64, F16, 16, "head")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    args = lambda: (b.q, b.table, b.row_start, b.kv_len)
+    b.kv_len[1] = 2 ** 31 - 1
+    PagedOf(b).attention(*args(), max_rows=rows, status=status)
+    assert int(status) & 2
+    b.kv_len[1] = 90
+    status.zero_()
+    b.row_start.copy_(torch.tensor([rows, 0, 2 * rows]))
+    PagedOf(b).attention(*args(), max_rows=rows, status=status)
+    assert int(status) & 8
+    status.zero_()
+    b.row_start.copy_(torch.tensor([0, rows, 1 << 30]))
+    out = PagedOf(b).attention(*args(), max_rows=rows, status=status)
+    assert int(status) & 8
+    b.check(out)  # cut to the rows there are
+
+
+def test_a_wrong_bound_of_the_rows_changes_nothing_but_the_kernel():
+    b = Batch([40, 1], [100, 300], 8, 2, 128, BF16, 16, "head")
+    for bound in (0, 1, 17, 10 ** 6):
+        out = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=bound)
+        b.check(out)
+
+
+@pytest.mark.parametrize("n,rows", [(1024, 1), (1000, 3), (300, 20)])
+def test_many_sequences(n, rows):
+    rng = np.random.default_rng(n)
+    lens = rng.integers(rows, 60, n).tolist()
+    r = [int(x) for x in rng.integers(0, rows + 1, n)]
+    b = Batch(r, lens, 2, 1, 64, BF16, 16, "token")
+    run_attention(b)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_strided_rows_and_pages(t):
+    """Q and out inside wider rows, pools that are slices of a layer-major allocation, a table with spare columns."""
+    b = Batch([1, 12], [90, 60], 4, 2, 64, t, 16, "head", width=9)
+    pools = torch.full((b.n_pages, 3, 2, 2, 16, 64), NAN, dtype=PAGE[t], device="cuda")  # [page][layer][K, V][head][row][D]
+    pools[:, 1, 0], pools[:, 1, 1] = b.k, b.v
+    wide = torch.full((b.total, 12, 64), NAN, dtype=t, device="cuda")
+    wide[:, 3:7] = b.q
+    out = torch.full((b.total, 6, 64), 7.0, dtype=t, device="cuda")
+    tab = torch.full((2, 20), -1, dtype=torch.int32, device="cuda")
+    tab[:, :9] = b.table
+    kv = paged.PagedKv(pools[:, 1, 0], pools[:, 1, 1])
+    kv.attention(wide[:, 3:7], tab[:, :9], b.row_start, b.kv_len, max_rows=12, out=out[:, 1:5])
+    b.check(out[:, 1:5])
+    assert bool((out[:, 0] == 7.0).all()) and bool((out[:, 5] == 7.0).all())
+
+
+def test_a_long_cache_is_addressed_past_32_bits():
+    """A pool whose last pages lie beyond 2^32 bytes and 2^31 elements: the same keys there and at its start."""
+    page, hkv, d = 64, 8, 128
+    n_pages = (1 << 32) // (page * hkv * d) + 8  # 2^32 elements and a little, 8 GiB each
+    k = torch.empty(n_pages, hkv, page, d, dtype=F16, device="cuda")
+    v = torch.empty_like(k)
+    b = Batch([1, 30], [200, 100], 16, hkv, d, F16, page, "head", spare=0)
+    far = torch.arange(b.n_pages, device="cuda") + (n_pages - b.n_pages)
+    k[far], v[far] = b.k, b.v
+    kv = paged.PagedKv(k, v)
+    high = torch.where(b.table >= 0, b.table + (n_pages - b.n_pages), b.table)
+    out = kv.attention(b.q, high, b.row_start, b.kv_len, max_rows=30)
+    b.check(out)
+    new = torch.randn(b.total, hkv, d).half().cuda()
+    kv.append(new, new, high, b.row_start, b.kv_len)
+    last = int(high[0, (200 - 1) // page])
+    assert torch.equal(v[last, :, (200 - 1) % page], new[0])
+
+
+def test_results_do_not_change_between_runs():
+    b = Batch([1] * 9, [700, 3, 900, 64, 65, 1, 512, 333, 128], 8, 2, 128, BF16, 16, "head")
+    first = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1)
+    for _ in range(3):
+        assert torch.equal(PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1), first)
+    b = Batch([70, 1, 300], [700, 33, 300], 8, 2, 128, BF16, 16, "head")
+    first = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=300)
+    for _ in range(3):
+        assert torch.equal(PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=300), first)
+
+
+# ---- streams, graphs, workspaces ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_another_stream_and_one_given_by_number(rows):
+    b = Batch([rows] * 3, [rows + 5, 200, 77], 4, 2, 64, F16, 16, "head")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        out = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows)
+    out2 = torch.empty_like(out)
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows, out=out2, stream=s.cuda_stream)
+    s.synchronize()
+    b.check(out)
+    assert torch.equal(out, out2)
+
+
+def test_two_streams_at_once():
+    b = [Batch([1] * 4, [900, 40, 333, 64], 8, 2, 128, F16, 16, "head", seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in b]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for x, s in zip(b, streams):
+            with torch.cuda.stream(s):
+                outs.append(PagedOf(x).attention(x.q, x.table, x.row_start, x.kv_len, max_rows=1))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, outs[i % 2])
+    b[0].check(outs[0])
+    b[1].check(outs[1])
+
+
+def test_a_captured_call_needs_a_workspace_of_its_own():
+    b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
+    out = torch.empty_like(b.q)
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(CudaComputeError) as e:
+            PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out)
+    assert "workspace" in e.value.msg
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
+    ws = paged.attention_workspace("cuda:0")
+    with pytest.raises(CudaComputeError) as e:
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, workspace=ws[:-256])
+    assert e.value.code == _lib.ERR_CAPACITY
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_the_operators_together_in_a_replayed_step(t):
+    """A prompt's chunk, then decode steps that a graph replays: each step rotates and stores its token and attends, the
+    lengths moving on the device.  Against the same run in 64 bits on the values that the pages hold."""
+    hq, hkv, d, page, n0, steps = 4, 2, 64, 16, 45, 5
+    f, fd, m = table(d, scaling="bands", factor=8.0, original_context=256.0, low=1.0, high=4.0)
+    seqs = 3
+    lens = [n0, 17, 1]
+    width = 6
+    g = torch.Generator().manual_seed(3)
+    pt = PAGE[t]
+    k_pool, v_pool = (torch.full((seqs * width, page, hkv, d), NAN, dtype=pt, device="cuda") for _ in range(2))
+    tab = torch.randperm(seqs * width, generator=g).to(torch.int32).view(seqs, width).cuda()
+    kv = paged.PagedKv(k_pool, v_pool, layout="token")
+    ws = paged.attention_workspace("cuda:0")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def host_rows(s, n):
+        ids = tab[s].cpu().long()
+        at = torch.arange(n)
+        return (p.cpu()[ids[at // page], at % page].double() for p in (k_pool, v_pool))
+
+    def check(qr, out, rows, lens):
+        b = Batch.__new__(Batch)
+        b.rows, b.lens, b.hq, b.hkv, b.d, b.t = rows, lens, hq, hkv, d, t
+        b.starts = np.cumsum([0] + rows).tolist()
+        b.q_h = qr.cpu()
+        pairs = [tuple(host_rows(s, n)) for s, n in enumerate(lens)]
+        b.keys, b.values = [p[0] for p in pairs], [p[1] for p in pairs]
+        b.check(out)
+
+    def layer(qkv, row_start, kv_len, q_rot, out, max_rows):
+        kv.append(qkv[:, hq:hq + hkv], qkv[:, hq + hkv:], tab, row_start, kv_len, q=qkv[:, :hq], q_out=q_rot, inv_freq=fd, pairing=1,
+                  magnitude=m, status=status)
+        kv.attention(q_rot, tab, row_start, kv_len, max_rows=max_rows, out=out, workspace=ws, status=status)
+
+    total = sum(lens)
+    qkv = torch.randn(total, hq + 2 * hkv, d, generator=g).to(t).cuda()
+    q_rot, out = (torch.empty(total, hq, d, dtype=t, device="cuda") for _ in range(2))
+    starts = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device="cuda")
+    layer(qkv, starts, torch.tensor(lens, dtype=torch.int32, device="cuda"), q_rot, out, max(lens))
+    check(q_rot, out, lens, lens)
+    for s, n in enumerate(lens):  # what the prompt left in the pages
+        k_row, _ = host_rows(s, n)
+        x = qkv[starts[s]:starts[s] + n, hq:hq + hkv].cpu()
+        extra, _ = rotation_bound(x, f, 1, m, pt)
+        within(k_row, rotate(x, torch.arange(n), f, 1, m), extra, pt)
+
+    kv_len = torch.tensor([n + 1 for n in lens], dtype=torch.int32, device="cuda")
+    one = torch.arange(seqs + 1, dtype=torch.int32, device="cuda")
+    step_in = torch.zeros(seqs, hq + 2 * hkv, d, dtype=t, device="cuda")
+    q1, out1 = (torch.empty(seqs, hq, d, dtype=t, device="cuda") for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(step_in, one, kv_len, q1, out1, 1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(step_in, one, kv_len, q1, out1, 1)
+        kv_len.add_(1)
+    for i in range(steps):
+        step_in.copy_(torch.randn(seqs, hq + 2 * hkv, d, generator=g).to(t))
+        graph.replay()
+        check(q1, out1, [1] * seqs, [n + 1 + i for n in lens])
+        want = rotate(step_in[:, :hq].cpu(), [n + i for n in lens], f, 1, m)
+        extra, _ = rotation_bound(step_in[:, :hq].cpu(), f, 1, m, t)
+        within(q1, want, extra, t)
+    assert int(status) == 0
+
+
+def test_pool_objects_refuse_what_they_cannot_describe():
+    k = torch.zeros(4, 2, 16, 64, dtype=F16, device="cuda")
+    for bad in (lambda: paged.PagedKv(k, k[:3]), lambda: paged.PagedKv(k.float(), k.float()), lambda: paged.PagedKv(k.cpu(), k.cpu()),
+                lambda: paged.PagedKv(k, k, layout="rows"), lambda: paged.PagedKv(k[..., ::2], k[..., ::2]), lambda: paged.PagedKv(k[0], k[0]),
+                lambda: paged.PagedKv(k, k.bfloat16())):
+        with pytest.raises(CudaComputeError):
+            bad()
+    kv = paged.PagedKv(k, k.clone())
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q, tab, st, ln = torch.zeros(2, 4, 64, dtype=F16, device="cuda"), torch.zeros(2, 3, **i32), torch.zeros(3, **i32), torch.zeros(2, **i32)
+    for kw in (dict(q=q.bfloat16()), dict(q=q[..., :32]), dict(q=q.float().double()), dict(tab=tab.long()), dict(tab=tab[:1]), dict(st=st[:2]), dict(ln=ln.cpu()),
+               dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), dict(out=q[:1]), dict(lse=torch.zeros(2, 3, device="cuda")), dict(window=-1),
+               dict(status=torch.zeros(1, device="cuda")), dict(workspace=torch.zeros(10, device="cuda")), dict(q=torch.zeros(2, 3, 64, dtype=F16, device="cuda"))):
+        a = dict(q=q, tab=tab, st=st, ln=ln)
+        a.update(kw)
+        with pytest.raises(CudaComputeError):
+            kv.attention(a.pop("q"), a.pop("tab"), a.pop("st"), a.pop("ln"), max_rows=1, **a)
+    assert kv.attention(q[:0], tab, st, ln, max_rows=0).shape == (0, 4, 64)
+    with pytest.raises(CudaComputeError):  # heads that are not contiguous, rows or not
+        kv.append(k[0, :, :0].transpose(0, 1), k[0, :, :0].transpose(0, 1), tab, st, ln)
+    assert kv.append(q[:0, :2], q[:0, 2:], tab, st, ln) is None
