@@ -220,6 +220,10 @@ int check_row_dtype(int32_t rows, int32_t pages, const ErrorText& e);
 constexpr uint32_t kStreamRows = 16;  // rows of one of its parts
 inline uint32_t stream_ctas(uint32_t sms, uint32_t head_dim) { return head_dim <= 128 ? 2 * sms : sms; }
 cudaError_t launch_stream(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s);
+// The tensor-memory kernel, for pools that it takes: head_dim up to 128, pages of at least 8 rows.
+constexpr uint32_t kTcRows = 256, kTcWidth = 128;  // rows and channels of one of its parts
+bool tc_takes(const Pool& pool);
+cudaError_t launch_tc(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace itk

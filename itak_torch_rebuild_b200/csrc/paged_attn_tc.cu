@@ -1,0 +1,896 @@
+// Attention of a ragged batch over the pages of its sequences on the 5th-generation tensor cores, for calls with many
+// (row, head) pairs per KV head: prompt chunks, and verify blocks beyond the streaming kernel's 16 pairs.
+//
+//   S = Q K^T,  P = 2^(c S - m),  O += P V,  out = O / sum P,   c = scale * log2(e), one pass over the keys.
+//
+// A cell is (sequence, KV head, block of 256 pairs); a pair is a query row and one of the heads of the KV head's group, so
+// that all heads of a group share the K and V tiles.  One CTA per SM walks an equal, contiguous run of the launch's
+// 128-key tiles laid end to end over all cells; a cell cut by the end of a run leaves a partial (maximum, sum, output), and
+// the CTA that takes the cell's last ticket joins them.  No CTA waits for another.
+//
+// Two streams keep the tensor core busy while a softmax runs: stream i has 128 accumulator rows (tensor-memory lanes), a
+// warpgroup whose thread r owns row r, and its own S and O in tensor memory:
+//   columns   0-127  S0, then in place its weights P0       columns 256-...  O0
+//   columns 128-255  S1, then P1                            columns 256 + D  O1
+//   more than 128 pairs: stream i holds pairs [128 i, 128 i + 128) of the block and takes every tile it sees;
+//   128 pairs or fewer:  both hold the same pairs, stream i takes every second tile, and the two are joined at the end -
+//                        otherwise the tensor core and the loads would wait for one softmax after every tile.
+// One thread issues all products, in the order O_i += P_i V(t), S_i = Q_i K(t + 1), the other stream's, ...: products
+// complete in order, so S may overwrite the weights of the tile before without a barrier of its own, and scores that are
+// complete vouch for every product issued before them.
+//
+// Warps 0-3 and 4-7: softmax of stream 0 and 1.  Warp 8: the products (one lane), tensor-memory allocation.  Warp 9: TMA
+// loads of K and V through one ring, K(t), V(t), K(t + 1), ...; a tile is fetched page by page, lane j taking one box
+// (64 channels of the rows that a page has in the tile), pages outside the keys of the block left out.  Score columns of
+// keys that a row does not see become -infinity whatever the tile holds there; V rows outside the block's keys are
+// overwritten with zeros in shared memory, since a weight of zero does not hide a NaN.
+//
+// 16-bit rows: products are exact, weights are rounded to the pages' type (half a step of the output's type, averaged over
+// the keys).  f32 rows: x = h + l with two halfs for queries and weights, twice the products, f32-grade results.
+//
+// The accumulator is rescaled in tensor memory only when a row's maximum grows by more than 2^8; until then the old
+// maximum is used for weights and sum alike, so nothing is lost.
+//
+// Bound: a 128 x 128 tile of both products takes 1024 clocks on the tensor core (D = 128) and its 16384 exponentials 1024
+// clocks on the special-function units.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "attn_common.cuh"
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace itk {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 384;  // two warpgroups of softmax, and one of product, load and two idle warps
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// Registers: the softmax threads hold a whole row of scores.  setmaxnreg moves registers between the warpgroups of a
+// block launched with kLaunchRegs a thread: 256 x 216 + 128 x 72 = 384 x 168.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "registers of the block");
+constexpr uint32_t kTile = 128;       // keys of a tile, and rows of a stream
+constexpr uint32_t kBlockPairs = 256;
+constexpr uint32_t kTmemCols = 512, kTmemO = 256;
+constexpr float kRescaleStep = 8.f;
+constexpr uint32_t kInfoSeqs = 32;  // sequences of a run kept in shared memory
+constexpr uint32_t kTailBytes = 1024;
+constexpr long long kWaitClocks = 2000000000ll;  // about a second
+
+template <typename T>
+struct RowTraits;
+template <>
+struct RowTraits<float> {
+    using Page = __half;
+    static constexpr bool kSplit = true;
+};
+template <>
+struct RowTraits<__half> {
+    using Page = __half;
+    static constexpr bool kSplit = false;
+};
+template <>
+struct RowTraits<__nv_bfloat16> {
+    using Page = __nv_bfloat16;
+    static constexpr bool kSplit = false;
+};
+
+template <typename T, int D>
+struct Shape {
+    static constexpr bool kSplit = RowTraits<T>::kSplit;
+    static constexpr uint32_t kPanel = kTile * 128;              // bytes of [128 rows][64 channels]
+    static constexpr uint32_t kStage = (D / 64) * kPanel;        // a K or V tile
+    static constexpr uint32_t kQ = (kSplit ? 2 : 1) * kStage;    // a stream's queries: (high) panels, then low ones
+    static constexpr uint32_t kStages = (232448u - 1024u - kTailBytes - 2 * kQ) / kStage;
+    static constexpr uint32_t kSmem = 2 * kQ + kStages * kStage + kTailBytes + 1024;
+    static_assert(kStages >= 3, "K(t), V(t) and K(t + 1)");
+    static_assert(kStages * kStage >= (2 * kMaxSeqs + 1) * 8, "the ring is the planning's scratch");
+    static_assert(kQ >= 2 * kTile * 8, "stream 1's query tile is the streams' exchange");
+};
+
+struct SeqInfo {
+    uint32_t row0, rows, len;
+};
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t channel, int32_t row, int32_t head,
+                                         int32_t page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(channel), "r"(row), "r"(head), "r"(page)
+        : "memory");
+}
+__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack2(__half, float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// The keys that pairs [p0, p1) of a sequence see, and the 128-key tiles that hold them (none: t0 == t1).
+struct KeyRange {
+    uint32_t lo, hi, t0, t1;
+};
+__device__ __forceinline__ KeyRange keys_of(const SeqInfo& q, uint32_t p0, uint32_t p1, uint32_t group, uint32_t window) {
+    const int32_t pos0 = static_cast<int32_t>(q.len) - static_cast<int32_t>(q.rows);
+    const int32_t first = pos0 + static_cast<int32_t>(p0 / group), last = pos0 + static_cast<int32_t>((p1 - 1) / group);
+    KeyRange r;
+    r.hi = last >= 0 ? static_cast<uint32_t>(last) + 1u : 0u;
+    r.lo = window != 0 && first >= 0 && static_cast<uint32_t>(first) >= window ? first + 1 - window : 0u;
+    if (r.hi == 0) r.lo = 0;
+    r.t0 = r.lo / kTile;
+    r.t1 = (r.hi + kTile - 1) / kTile;
+    return r;
+}
+// Tiles a cell takes in a run: at least one, so that a block that sees nothing is still written.
+__device__ __forceinline__ uint32_t cell_tiles(const SeqInfo& q, uint32_t block, uint32_t group, uint32_t window) {
+    const KeyRange r = keys_of(q, block * kBlockPairs, min(q.rows * group, (block + 1) * kBlockPairs), group, window);
+    return max(r.t1 - r.t0, 1u);
+}
+
+// One cell, or the part of one that falls into this CTA's run, as every role derives it for itself.
+struct Item {
+    SeqInfo q;
+    uint32_t s, kvh, block, blocks, pairs;  // pairs of the block
+    uint32_t T, off, n;                     // tiles of the cell, and of those this CTA's [off, off + n)
+    uint64_t pos;                           // of tile `off` in the launch's order
+    bool twin;
+    uint32_t lo, hi;        // keys of the block
+    uint32_t t0, t1;        // tiles to load
+    uint32_t a[2], e[2];    // stream i: tiles a[i], a[i] + step, ... below e[i]
+    uint32_t step;
+};
+
+struct Walk {
+    const AttnParams& p;
+    const SeqInfo* info;  // of the run's first kInfoSeqs sequences
+    uint32_t s_first;
+    uint64_t run1;
+    Item it;
+
+    __device__ __forceinline__ void open_seq() {
+        if (it.s - s_first < kInfoSeqs) {
+            it.q = info[it.s - s_first];
+        } else {
+            Batch b = p.batch;
+            b.status = nullptr;
+            const Seq q = seq_of(b, it.s, p.pool.page_shift);
+            it.q = SeqInfo{q.row0, q.rows, q.len};
+        }
+        it.blocks = (it.q.rows * p.group + kBlockPairs - 1) / kBlockPairs;
+    }
+    __device__ __forceinline__ void open_cell(uint32_t off) {
+        const uint32_t all = it.q.rows * p.group, p0 = it.block * kBlockPairs, p1 = min(all, p0 + kBlockPairs);
+        it.pairs = p1 - p0;
+        it.twin = it.pairs <= kTile;
+        const KeyRange r = keys_of(it.q, p0, p1, p.group, p.window);
+        it.T = max(r.t1 - r.t0, 1u);
+        it.off = off;
+        it.n = static_cast<uint32_t>(min(run1 - it.pos, static_cast<uint64_t>(it.T - off)));
+        it.lo = r.lo;
+        it.hi = r.hi;
+        it.t0 = min(r.t0 + off, r.t1);
+        it.t1 = min(it.t0 + it.n, r.t1);
+        if (it.twin) {
+            it.step = 2;
+            it.a[0] = it.t0;
+            it.a[1] = it.t0 + 1;
+            it.e[0] = it.e[1] = it.t1;
+        } else {
+            it.step = 1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const KeyRange k = keys_of(it.q, p0 + i * kTile, i == 0 ? p0 + kTile : p1, p.group, p.window);
+                it.a[i] = max(it.t0, k.t0);
+                it.e[i] = min(it.t1, k.t1);
+            }
+        }
+    }
+    __device__ __forceinline__ bool next() {
+        it.pos += it.n;
+        if (it.pos >= run1) return false;
+        if (++it.block == it.blocks) {
+            it.block = 0;
+            if (++it.kvh == p.pool.kv_heads) {
+                it.kvh = 0;
+                do {  // a sequence with rows follows, since the launch has tiles left
+                    if (++it.s >= p.batch.n_seqs) return false;
+                    open_seq();
+                } while (it.blocks == 0);
+            }
+        }
+        open_cell(0);
+        return true;
+    }
+    // How many streams use tile t (each reports the tile's stage as read).
+    __device__ __forceinline__ uint32_t users(uint32_t t) const {
+        if (it.twin) return 1u;
+        return (t >= it.a[0] && t < it.e[0] ? 1u : 0u) + (t >= it.a[1] && t < it.e[1] ? 1u : 0u);
+    }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                                                               const __grid_constant__ CUtensorMap vmap) {
+    using P = typename RowTraits<T>::Page;
+    using Sh = Shape<T, D>;
+    constexpr bool SPLIT = Sh::kSplit;
+    constexpr uint32_t NST = Sh::kStages;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* const smem =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const uint32_t qbuf = smem_u32(smem), ring = qbuf + 2 * Sh::kQ, tail = ring + NST * Sh::kStage;
+    unsigned char* const tail_ptr = smem + 2 * Sh::kQ + NST * Sh::kStage;
+    // mbarriers
+    const uint32_t bar_full = tail;                // [stage] the tile has landed
+    const uint32_t bar_empty = bar_full + 8 * 16;  // [stage] every product that reads it is complete
+    const uint32_t bar_s = bar_empty + 8 * 16;     // [stream] scores complete
+    const uint32_t bar_p = bar_s + 16;             // [stream] weights stored
+    const uint32_t bar_o = bar_p + 16;             // [stream] the cell's last product complete
+    const uint32_t bar_q = bar_o + 16;             // [stream] the cell's queries are in shared memory
+    const uint32_t bar_land = bar_q + 16;          // a V tile that needs zero rows has landed
+    const uint32_t bar_done = bar_land + 8;        // everything issued to the tensor core is complete
+    static_assert(NST <= 16, "stages");
+    uint32_t* const word = reinterpret_cast<uint32_t*>(tail_ptr + 400);  // [0] tensor memory, [1] joined flag, [2] abort
+    volatile uint32_t* const abort_flag = word + 2;
+    uint32_t* const plan = reinterpret_cast<uint32_t*>(tail_ptr + 424);  // where the run begins: sequence, KV head, block, tile
+    SeqInfo* const info = reinterpret_cast<SeqInfo*>(tail_ptr + 448);
+    static_assert(448 + kInfoSeqs * sizeof(SeqInfo) <= kTailBytes, "tail");
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t n_seqs = p.batch.n_seqs, group = p.group, window = p.window, cta = blockIdx.x;
+
+    // ---- set-up and the batch summed up --------------------------------------------------------------------------------
+    if (tid == 0) {
+        for (uint32_t i = 0; i < NST; ++i) {
+            tc::mbar_init(bar_full + 8 * i, 1);
+            tc::mbar_init(bar_empty + 8 * i, 2);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            tc::mbar_init(bar_s + 8 * i, 1);
+            tc::mbar_init(bar_p + 8 * i, 128);
+            tc::mbar_init(bar_o + 8 * i, 1);
+            tc::mbar_init(bar_q + 8 * i, 128);
+        }
+        tc::mbar_init(bar_land, 1);
+        tc::mbar_init(bar_done, 1);
+        *abort_flag = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == kMmaWarp) {
+        tc::tmem_alloc(smem_u32(word), kTmemCols);
+        tc::tmem_relinquish();
+    }
+    uint64_t* const prefix = reinterpret_cast<uint64_t*>(smem + 2 * Sh::kQ);  // [n_seqs + 1], scratch in the ring
+    uint64_t* const per_head = prefix + n_seqs + 1;  // [n_seqs] tiles of one KV head
+    constexpr uint64_t kLater = ~0ull;
+    constexpr uint32_t kOwnBlocks = 8;  // a sequence of more blocks is summed by a whole warp
+    for (uint32_t s = tid; s < n_seqs; s += kThreads) {
+        Batch b = p.batch;
+        if (cta != 0) b.status = nullptr;  // one CTA reports
+        const Seq sq = seq_of(b, s, p.pool.page_shift);
+        const SeqInfo q{sq.row0, sq.rows, sq.len};
+        const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
+        uint64_t sum = kLater;
+        if (blocks <= kOwnBlocks) {
+            sum = 0;
+            for (uint32_t i = 0; i < blocks; ++i) sum += cell_tiles(q, i, group, window);
+        }
+        per_head[s] = sum;
+    }
+    __syncthreads();
+    for (uint32_t s = warp; s < n_seqs; s += kThreads / 32) {
+        if (per_head[s] != kLater) continue;
+        Batch b = p.batch;
+        b.status = nullptr;
+        const Seq sq = seq_of(b, s, p.pool.page_shift);
+        const SeqInfo q{sq.row0, sq.rows, sq.len};
+        const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
+        uint64_t sum = 0;
+        for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        __syncwarp();
+        if (lane == 0) per_head[s] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {  // prefix sums, 32 sequences at a time
+        uint64_t base = 0;
+        for (uint32_t s0 = 0; s0 < n_seqs; s0 += 32) {
+            const uint32_t s = s0 + lane;
+            const uint64_t mine = s < n_seqs ? per_head[s] * p.pool.kv_heads : 0u;
+            uint64_t incl = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= static_cast<uint32_t>(d)) incl += o;
+            }
+            if (s < n_seqs) prefix[s] = base + incl - mine;
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) prefix[n_seqs] = base;
+    }
+    __syncthreads();
+    const uint64_t W = prefix[n_seqs];
+    const uint64_t per = max((W + gridDim.x - 1) / gridDim.x, static_cast<uint64_t>(1));
+    const uint64_t run0 = cta * per, run1 = min(W, run0 + per);
+    const bool works = run0 < run1;
+    if (works && warp == 0) {  // where the run begins
+        uint32_t lo = 0, hi = n_seqs;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (prefix[mid] <= run0)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        Batch b = p.batch;
+        b.status = nullptr;
+        const Seq sq = seq_of(b, lo, p.pool.page_shift);
+        const SeqInfo q{sq.row0, sq.rows, sq.len};
+        const uint64_t in = run0 - prefix[lo];
+        const uint32_t kvh = static_cast<uint32_t>(in / per_head[lo]);
+        uint64_t left = in % per_head[lo];
+        uint32_t block = 0;
+        const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
+        for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {  // the block that holds tile `left` of the KV head
+            const uint32_t mine = b0 + lane < blocks ? cell_tiles(q, b0 + lane, group, window) : 0u;
+            uint32_t incl = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= static_cast<uint32_t>(d)) incl += o;
+            }
+            const uint32_t here = __ballot_sync(0xffffffffu, incl > left);
+            if (here != 0u) {
+                const int at = __ffs(here) - 1;
+                block = b0 + at;
+                left -= __shfl_sync(0xffffffffu, incl - mine, at);
+                break;
+            }
+            left -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            plan[0] = lo;
+            plan[1] = kvh;
+            plan[2] = block;
+            plan[3] = static_cast<uint32_t>(left);
+        }
+        if (lane < kInfoSeqs && lo + lane < n_seqs) {
+            const Seq x = seq_of(b, lo + lane, p.pool.page_shift);
+            info[lane] = SeqInfo{x.row0, x.rows, x.len};
+        }
+    }
+    tc::fence_proxy_async();  // the ring was the planning's scratch, TMA writes it next
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = word[0];
+    Walk w{p, info, 0, run1, {}};
+    if (works) {
+        w.s_first = w.it.s = plan[0];
+        w.it.kvh = plan[1];
+        w.it.block = plan[2];
+        w.it.pos = run0;
+        w.open_seq();
+        w.open_cell(plan[3]);
+    }
+    const Item& it = w.it;
+    // Waits that ran out end the call: every role leaves (or, the softmax threads, walks on through their barriers without
+    // waiting), once what the role has in flight has come to rest.
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        const long long t0 = clock64();
+        while (!tc::mbar_try_wait(bar, parity)) {
+            if (*abort_flag != 0) return false;
+            if (clock64() - t0 > kWaitClocks) {
+                *abort_flag = 1;
+                raise(p.batch, kWaitRanOut);
+                return false;
+            }
+        }
+        return true;
+    };
+
+    if (warp >= kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp && works) {
+            // ---------------- loads ------------------------------------------------------------------------------------
+            const uint32_t shift = p.pool.page_shift, box_shift = min(shift, 7u);  // rows of a box: a page's, or a tile's
+            constexpr uint32_t NP = D / 64;
+            const uint32_t slot = lane / NP, panel = lane % NP;  // lane's page within the tile, and its 64 channels
+            const uint32_t row_at = slot << box_shift;           // its first row in the tile
+            uint32_t cnt = 0, landed = 0;
+            bool ok = true;
+            do {
+                const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
+                for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
+                    const uint32_t key = t * kTile + row_at;  // the box holds keys [key, key + box rows)
+                    const bool mine = row_at < kTile && key < it.hi && key + (1u << box_shift) > it.lo;
+                    uint32_t page = 0;
+                    if (mine) {
+                        page = __ldg(tab + (key >> shift));
+                        if (page >= p.pool.n_pages) {
+                            raise(p.batch, kBadPage);
+                            page = p.pool.n_pages;  // outside the map: zeros
+                        }
+                    }
+                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
+                    const uint32_t bytes = boxes << (box_shift + 7);
+                    const uint32_t a = it.lo > t * kTile ? it.lo - t * kTile : 0u, b = min(it.hi - t * kTile, kTile);
+                    const bool cut = a != 0 || b != kTile;  // rows outside [a, b) are not the block's
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const uint32_t st = cnt % NST;
+                        if (cnt >= NST && !wait(bar_empty + 8 * st, (cnt / NST - 1) & 1u)) ok = false;
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        const uint32_t dst = ring + st * Sh::kStage, bar = bar_full + 8 * st;
+                        const uint32_t signal = v == 1 && cut ? bar_land : bar;
+                        if (lane == 0) mbar_arrive_expect(signal, bytes);
+                        __syncwarp();
+                        if (mine)
+                            tma_load(dst + panel * Sh::kPanel + row_at * 128, v == 0 ? &kmap : &vmap, signal, panel * 64,
+                                     static_cast<int32_t>(key & ((1u << shift) - 1u)), static_cast<int32_t>(it.kvh), static_cast<int32_t>(page));
+                        if (v == 1 && cut) {
+                            if (!wait(bar_land, landed & 1u)) ok = false;
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            ++landed;
+                            unsigned char* const rows = smem + (dst - qbuf);
+                            const uint32_t gone = kTile - (b - a);
+                            for (uint32_t i = lane; i < gone * (D / 8); i += 32) {
+                                const uint32_t j = i / (D / 8), c = i % (D / 8);
+                                const uint32_t r = j < a ? j : b + (j - a);
+                                *reinterpret_cast<uint4*>(rows + (c / 8) * Sh::kPanel + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                            tc::fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(bar);
+                        }
+                        ++cnt;
+                    }
+                }
+            } while (ok && w.next());
+            if (!ok) {  // copies in flight land before the block's shared memory goes
+                for (uint32_t n = cnt > NST ? cnt - NST : 0u; n < cnt; ++n)
+                    tc::mbar_wait_bounded(bar_full + 8 * (n % NST), (n / NST) & 1u, kWaitClocks);
+                tc::mbar_wait_bounded(bar_land, landed & 1u, kWaitClocks);
+            }
+        } else if (warp == kMmaWarp && works && lane == 0) {
+            // ---------------- products ---------------------------------------------------------------------------------
+            constexpr uint32_t kType = std::is_same<P, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t kIdS = tc::instr_desc_f16(128, kTile, false) | kType;
+            constexpr uint32_t kIdO = tc::instr_desc_f16(128, D, true) | kType;
+            uint32_t base = 0;           // the ring's count at the item's first tile
+            uint32_t n_p[2] = {0, 0};    // weights used so far, per stream
+            uint32_t items = 0;
+            bool ok = true;
+            do {
+                uint32_t nt[2] = {it.a[0], it.a[1]};
+                bool fresh[2] = {true, true};
+                auto scores = [&](int i) -> bool {
+                    const uint32_t t = nt[i], c = base + 2 * (t - it.t0), st = c % NST;
+                    if (!wait(bar_full + 8 * st, (c / NST) & 1u)) return false;
+                    tc::fence_after_sync();
+                    const uint32_t k = ring + st * Sh::kStage, q = qbuf + (it.twin ? 0u : i * Sh::kQ), d = tmem + i * kTile;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = (ks / 4) * Sh::kPanel + (ks % 4) * 32;
+                        tc::mma_f16_ss(d, tc::smem_desc(q + off, 16, 1024), tc::smem_desc(k + off, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
+                        if constexpr (SPLIT)
+                            tc::mma_f16_ss(d, tc::smem_desc(q + Sh::kStage + off, 16, 1024), tc::smem_desc(k + off, 16, 1024), kIdS, 1u);
+                    }
+                    tc::mma_commit(bar_empty + 8 * st);
+                    if (w.users(t) == 1) tc::mma_commit(bar_empty + 8 * st);
+                    tc::mma_commit(bar_s + 8 * i);
+                    nt[i] += it.step;
+                    return true;
+                };
+                auto values = [&](int i, uint32_t t) -> bool {
+                    const uint32_t c = base + 2 * (t - it.t0) + 1, st = c % NST;
+                    if (!wait(bar_p + 8 * i, n_p[i] & 1u)) return false;
+                    ++n_p[i];
+                    if (!wait(bar_full + 8 * st, (c / NST) & 1u)) return false;
+                    tc::fence_after_sync();
+                    const uint32_t v = ring + st * Sh::kStage, a = tmem + i * kTile, d = tmem + kTmemO + i * D;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint64_t desc = tc::smem_desc(v + j * 2048, Sh::kPanel, 1024);
+                        if constexpr (SPLIT) {
+                            tc::mma_f16_ts(d, a + 16 * j, desc, kIdO, j > 0 || !fresh[i] ? 1u : 0u);
+                            tc::mma_f16_ts(d, a + 16 * j + 8, desc, kIdO, 1u);
+                        } else {
+                            tc::mma_f16_ts(d, a + 8 * j, desc, kIdO, j > 0 || !fresh[i] ? 1u : 0u);
+                        }
+                    }
+                    fresh[i] = false;
+                    tc::mma_commit(bar_empty + 8 * st);
+                    if (w.users(t) == 1) tc::mma_commit(bar_empty + 8 * st);
+                    return true;
+                };
+                for (int i = 0; ok && i < 2; ++i) {
+                    ok = wait(bar_q + 8 * i, items & 1u);
+                    if (ok && nt[i] < it.e[i]) ok = scores(i);
+                }
+                uint32_t pv[2] = {it.a[0], it.a[1]};
+                while (ok) {
+                    const bool l0 = pv[0] < it.e[0], l1 = pv[1] < it.e[1];
+                    if (!l0 && !l1) break;
+                    const int i = l0 && (!l1 || pv[0] <= pv[1]) ? 0 : 1;
+                    const uint32_t t = i == 0 ? pv[0] : pv[1];
+                    ok = i == 0 ? values(0, t) : values(1, t);
+                    if (i == 0)
+                        pv[0] += it.step;
+                    else
+                        pv[1] += it.step;
+                    const bool more = i == 0 ? nt[0] < it.e[0] : nt[1] < it.e[1];
+                    if (ok && more) ok = i == 0 ? scores(0) : scores(1);
+                    if (ok && !more) tc::mma_commit(bar_o + 8 * i);
+                }
+                base += 2 * (it.t1 - it.t0);
+                ++items;
+            } while (ok && w.next());
+            tc::mma_commit(bar_done);
+            tc::mbar_wait_bounded(bar_done, 0u, kWaitClocks);
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+        // ---------------- softmax: thread r of warpgroup i owns row r of stream i ----------------------------------------
+        const uint32_t i = warp >> 2, r = tid & 127;
+        const uint32_t lane_base = ((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lane_base + i * kTile, tO = tmem + lane_base + kTmemO + i * D;
+        const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);  // the queries carry a negative scale's sign
+        const bool flip = p.scale_log2 < 0.f;
+        const uint32_t head_dim = p.pool.head_dim;
+        uint32_t n_s = 0, n_o = 0;  // scores seen, last products seen
+        bool dead = !works;         // a wait ran out: walk on through the barriers, touch nothing
+        if (works) do {
+            // ---- the block's queries into shared memory: warp by warp, 16 bytes a lane
+            if (i == 0 || !it.twin) {
+                constexpr uint32_t CH = D / 8, RP = 32 / CH, PASSES = 32 / RP;
+                const uint32_t chunk = lane % CH;
+                unsigned char* const qs = smem + i * Sh::kQ + (chunk / 8) * Sh::kPanel;
+                auto row_of = [&](uint32_t pass) { return (warp & 3) * 32 + pass * RP + lane / CH; };
+                auto source = [&](uint32_t qr) -> const T* {
+                    const uint32_t in = i * kTile + qr;
+                    if (in >= it.pairs || chunk * 8 >= head_dim) return nullptr;
+                    const uint32_t pair = it.block * kBlockPairs + in;
+                    return static_cast<const T*>(p.q) + static_cast<uint64_t>(it.q.row0 + pair / group) * p.q_row +
+                           (it.kvh * group + pair % group) * head_dim + chunk * 8;
+                };
+                constexpr uint32_t BATCH = SPLIT ? 4 : 8;
+#pragma unroll 1
+                for (uint32_t p0 = 0; p0 < PASSES; p0 += BATCH) {
+                    Vec8<T> x[BATCH];
+#pragma unroll
+                    for (uint32_t j = 0; j < BATCH; ++j) {
+                        const T* src = source(row_of(p0 + j));
+                        x[j] = Vec8<T>{};
+                        if (src) x[j].load(src);
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < BATCH; ++j) {
+                        const uint32_t qr = row_of(p0 + j);
+                        unsigned char* dst = qs + qr * 128 + (((chunk % 8) ^ (qr & 7)) << 4);
+                        if constexpr (SPLIT) {
+                            float f[8];
+                            x[j].get(f);
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                __half h0, l0, h1, l1;
+                                split_half(flip ? -f[2 * e] : f[2 * e], h0, l0);
+                                split_half(flip ? -f[2 * e + 1] : f[2 * e + 1], h1, l1);
+                                hi[e] = pack_half2(h0, h1);
+                                lo[e] = pack_half2(l0, l1);
+                            }
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(dst + Sh::kStage) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        } else {
+                            uint4 v = x[j].w;
+                            if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                            *reinterpret_cast<uint4*>(dst) = v;
+                        }
+                    }
+                }
+                tc::fence_proxy_async();
+            }
+            mbar_arrive(bar_q + 8 * i);
+
+            const uint32_t in = it.twin ? r : i * kTile + r;  // pair within the block
+            const bool live = in < it.pairs;
+            const uint32_t pair = it.block * kBlockPairs + (live ? in : 0u);
+            const int32_t pos0 = static_cast<int32_t>(it.q.len) - static_cast<int32_t>(it.q.rows);
+            const int32_t at = live ? pos0 + static_cast<int32_t>(pair / group) : -1;
+            // keys (low, at] are seen
+            const int32_t low = window != 0 ? at - static_cast<int32_t>(min(window, 0x7fffffffu)) : -1;
+            float m = -INFINITY, l = 0.f;
+            const uint32_t a = i == 0 ? it.a[0] : it.a[1], e = i == 0 ? it.e[0] : it.e[1];
+            const bool any = a < e;
+            for (uint32_t t = a; t < e; t += it.step) {
+                dead = dead || !wait(bar_s + 8 * i, n_s & 1u);
+                dead = __any_sync(0xffffffffu, dead);
+                if (dead) break;
+                ++n_s;
+                tc::fence_after_sync();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tc::tmem_ld32(tS + 32 * j, x[j]);
+                tc::tmem_wait_ld();
+                const int32_t from = low - static_cast<int32_t>(t * kTile), to = at - static_cast<int32_t>(t * kTile);  // columns (from, to]
+                if (__any_sync(0xffffffffu, live && (from >= 0 || to < static_cast<int32_t>(kTile) - 1))) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) {
+                            const int32_t col = 32 * j + u;
+                            if (col <= from || col > to) x[j][u] = 0xff800000u;
+                        }
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int u = 0; u < 32; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[j][u]));
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+                    if (t != a) {  // the scores at hand vouch for every product before them: O is at rest
+#pragma unroll 1
+                        for (int j = 0; j < D; j += 16) {
+                            uint32_t o[16];
+                            tc::tmem_ld16(tO + j, o);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                            tc::tmem_st16(tO + j, o);
+                        }
+                    }
+                    if (grow) m = mx;
+                    l *= f;
+                }
+                const float nm = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) {
+                        const float wgt = fast_exp2(fmaf(__uint_as_float(x[j][u]), c, nm));
+                        sum[u & 3] += wgt;
+                        x[j][u] = __float_as_uint(wgt);
+                    }
+                    if constexpr (SPLIT) {
+                        uint32_t y[32];  // keys 16 s ..: high terms in columns 16 s .., low terms in 16 s + 8 ..
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            __half h0, l0, h1, l1;
+                            split_half(__uint_as_float(x[j][2 * u]), h0, l0);
+                            split_half(__uint_as_float(x[j][2 * u + 1]), h1, l1);
+                            y[(u / 8) * 16 + u % 8] = pack_half2(h0, h1);
+                            y[(u / 8) * 16 + 8 + u % 8] = pack_half2(l0, l1);
+                        }
+                        tc::tmem_st32(tS + 32 * j, y);
+                    } else {
+                        uint32_t y[16];
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) y[u] = pack2(P(), __uint_as_float(x[j][2 * u]), __uint_as_float(x[j][2 * u + 1]));
+                        tc::tmem_st16(tS + 16 * j, y);
+                    }
+                }
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                mbar_arrive(bar_p + 8 * i);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (any && !dead) {
+                dead = !wait(bar_o + 8 * i, n_o & 1u);
+                dead = __any_sync(0xffffffffu, dead);
+                ++n_o;
+                tc::fence_after_sync();
+            }
+
+            // ---- the cell's end ----------------------------------------------------------------------------------------
+            const bool whole = it.n == it.T;
+            float2* const ex = reinterpret_cast<float2*>(smem + Sh::kQ);  // [stream][row] (maximum, sum), in the unused query tile
+            float f0 = 1.f, f1 = 0.f;                                     // weights of the own and the other stream's rows
+            bool other_any = false;
+            if (it.twin) {
+                // Rows are the same in both streams and sit in the same lanes: each warpgroup takes half of the channels.
+                other_any = i == 0 ? it.a[1] < it.e[1] : it.a[0] < it.e[0];
+                ex[tid] = make_float2(m, l);
+                tc::fence_before_sync();
+                both_sync();
+                tc::fence_after_sync();
+                const float2 x = ex[tid ^ 128];
+                const float M = fmaxf(m, x.x);
+                f0 = m == -INFINITY ? 0.f : fast_exp2(m - M);
+                f1 = x.x == -INFINITY ? 0.f : fast_exp2(x.x - M);
+                l = l * f0 + x.y * f1;
+                m = M;
+            }
+            const uint32_t row = it.q.row0 + pair / group, head = it.kvh * group + pair % group;
+            const uint32_t c0 = it.twin ? i * (D / 2) : 0u, c1 = it.twin ? c0 + D / 2 : D;  // channels of this thread
+            const uint32_t tOther = tmem + lane_base + kTmemO + (1 - i) * D;
+            const uint32_t part = it.off == 0 ? 2 * cta + 1 : 2 * cta;
+            float4* const po = reinterpret_cast<float4*>(p.part_o) + static_cast<size_t>(part) * (D / 4) * kBlockPairs;
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            T* const dst = static_cast<T*>(p.out) + static_cast<uint64_t>(row) * p.out_row + head * head_dim;
+            auto put8 = [&](uint32_t ch, const float (&f)[8]) {
+                if (live && ch < head_dim) {
+                    Vec8<T> v;
+                    if constexpr (SPLIT) {
+                        v.set(f);
+                    } else {
+                        v.w = make_uint4(pack2(P(), f[0], f[1]), pack2(P(), f[2], f[3]), pack2(P(), f[4], f[5]), pack2(P(), f[6], f[7]));
+                    }
+                    v.store(dst + ch);
+                }
+            };
+            if (!dead) {
+#pragma unroll 1
+                for (uint32_t ch = c0; ch < c1; ch += 16) {
+                    uint32_t o[16], y[16];
+                    float f[16];
+                    if (any) tc::tmem_ld16(tO + ch, o);
+                    if (it.twin && other_any) tc::tmem_ld16(tOther + ch, y);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        f[u] = any ? __uint_as_float(o[u]) : 0.f;
+                        if (it.twin) f[u] = f[u] * f0 + (other_any ? __uint_as_float(y[u]) * f1 : 0.f);
+                    }
+                    if (whole) {
+#pragma unroll
+                        for (int g8 = 0; g8 < 2; ++g8) {
+                            float z[8];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) z[u] = f[8 * g8 + u] * inv;
+                            put8(ch + 8 * g8, z);
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4)
+                            po[static_cast<size_t>(ch / 4 + g4) * kBlockPairs + in] = make_float4(f[4 * g4], f[4 * g4 + 1], f[4 * g4 + 2], f[4 * g4 + 3]);
+                    }
+                }
+            }
+            auto put_lse = [&](float top, float sum) {
+                if (live && p.lse && (i == 0 || !it.twin))
+                    p.lse[static_cast<uint64_t>(row) * p.q_heads + head] =
+                        sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+            };
+            if (whole) {
+                if (!dead) put_lse(m, l);
+            } else {
+                float2* const pml = reinterpret_cast<float2*>(p.part_ml);
+                if (live && (i == 0 || !it.twin)) pml[static_cast<size_t>(part) * kBlockPairs + in] = make_float2(m, l);
+                const uint64_t cell0 = it.pos - it.off;
+                const uint32_t first = static_cast<uint32_t>(cell0 / per), last = static_cast<uint32_t>((cell0 + it.T - 1) / per);
+                both_sync();
+                if (tid == 0) {
+                    __threadfence();  // cumulative over the stores above (ordered before the barrier)
+                    const unsigned int ticket = atomicAdd(p.tickets + first, 1u);
+                    word[1] = ticket == last - first ? 1u : 0u;
+                    if (ticket == last - first) p.tickets[first] = 0u;  // as the next launch wants it
+                }
+                both_sync();
+                if (word[1] != 0u && !dead) {
+                    __threadfence();
+                    // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...
+                    if (live) {
+                        float M = -INFINITY, L = 0.f;
+                        for (uint32_t k = first; k <= last; ++k) {
+                            const float2 x = __ldcg(pml + static_cast<size_t>(k == first ? 2 * k + 1 : 2 * k) * kBlockPairs + in);
+                            const float to = fmaxf(M, x.x);
+                            const float g0 = M == -INFINITY ? 0.f : fast_exp2(M - to), g1 = x.x == -INFINITY ? 0.f : fast_exp2(x.x - to);
+                            L = L * g0 + x.y * g1;
+                            M = to;
+                        }
+                        const float il = L > 0.f || L != L ? 1.f / L : 0.f;
+                        const float4* const all = reinterpret_cast<const float4*>(p.part_o);
+#pragma unroll 1
+                        for (uint32_t ch = c0; ch < c1; ch += 8) {
+                            float z[8] = {};
+#pragma unroll 4
+                            for (uint32_t k = first; k <= last; ++k) {
+                                const size_t sl = k == first ? 2 * k + 1 : 2 * k;
+                                const float mk = __ldcg(pml + sl * kBlockPairs + in).x;
+                                const float g1 = mk == -INFINITY ? 0.f : fast_exp2(mk - M);
+                                const float4 u0 = __ldcg(all + (sl * (D / 4) + ch / 4) * kBlockPairs + in);
+                                const float4 u1 = __ldcg(all + (sl * (D / 4) + ch / 4 + 1) * kBlockPairs + in);
+                                z[0] += g1 * u0.x, z[1] += g1 * u0.y, z[2] += g1 * u0.z, z[3] += g1 * u0.w;
+                                z[4] += g1 * u1.x, z[5] += g1 * u1.y, z[6] += g1 * u1.z, z[7] += g1 * u1.w;
+                            }
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) z[u] *= il;
+                            put8(ch, z);
+                        }
+                        put_lse(M, L);
+                    }
+                }
+            }
+            // Nothing of this cell is read any more: the exchange, the other stream's accumulator, the joined flag.
+            tc::fence_before_sync();
+            both_sync();
+            tc::fence_after_sync();
+        } while (w.next());
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// [page][head][row][channel] of a pool, boxes of 64 channels and the rows that one page has in a tile.
+bool make_map(CUtensorMap* map, const Pool& pool, void* data, int32_t dtype) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const uint64_t rows = 1ull << pool.page_shift;
+    const cuuint64_t dims[4] = {pool.head_dim, rows, pool.kv_heads, pool.n_pages};
+    // (a stride of a dimension of one element is never used, and may not be zero)
+    const cuuint64_t strides[3] = {rows > 1 ? pool.row_stride * 2 : 16, pool.kv_heads > 1 ? pool.head_stride * 2 : 16,
+                                   pool.n_pages > 1 ? pool.page_stride * 2 : 16};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows < kTile ? rows : kTile), 1, 1}, one[4] = {1, 1, 1, 1};
+    return encode(map, dtype == ITK_ROW_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, data, dims, strides, box,
+                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+cudaError_t launch_as(const AttnParams& p, int32_t page_dtype, uint32_t sms, cudaStream_t s) {
+    auto kernel = paged_tc_kernel<T, D>;
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    // The warpgroups' shares are drawn from what the block was launched with: fewer, and setmaxnreg would wait for good.
+    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<T, D>::kSmem));
+    if (e != cudaSuccess) return e;
+    CUtensorMap km, vm;
+    if (!make_map(&km, p.pool, p.pool.k, page_dtype) || !make_map(&vm, p.pool, p.pool.v, page_dtype)) return cudaErrorInvalidValue;
+    kernel<<<sms, kThreads, Shape<T, D>::kSmem, s>>>(p, km, vm);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+bool tc_takes(const Pool& pool) { return pool.head_dim <= 128 && pool.page_shift >= 3; }
+
+cudaError_t launch_tc(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s) {
+    const bool narrow = p.pool.head_dim <= 64;
+    if (row_dtype == ITK_ROW_F32) return narrow ? launch_as<float, 64>(p, ITK_ROW_F16, sms, s) : launch_as<float, 128>(p, ITK_ROW_F16, sms, s);
+    if (row_dtype == ITK_ROW_F16) return narrow ? launch_as<__half, 64>(p, ITK_ROW_F16, sms, s) : launch_as<__half, 128>(p, ITK_ROW_F16, sms, s);
+    return narrow ? launch_as<__nv_bfloat16, 64>(p, ITK_ROW_BF16, sms, s) : launch_as<__nv_bfloat16, 128>(p, ITK_ROW_BF16, sms, s);
+}
+
+}  // namespace paged
+}  // namespace itk
