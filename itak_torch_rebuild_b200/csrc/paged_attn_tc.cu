@@ -56,7 +56,7 @@ constexpr uint32_t kBlockPairs = 256;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
 constexpr float kRescaleStep = 8.f;
 constexpr uint32_t kInfoSeqs = 32;  // sequences of a run kept in shared memory
-constexpr uint32_t kTailBytes = 1024;
+constexpr uint32_t kTailBytes = 1280;  // mbarriers, the run's beginning, the roles' items
 constexpr long long kWaitClocks = 2000000000ll;  // about a second
 
 template <typename T>
@@ -139,27 +139,27 @@ __device__ __forceinline__ uint32_t cell_tiles(const SeqInfo& q, uint32_t block,
     return max(r.t1 - r.t0, 1u);
 }
 
-// One cell, or the part of one that falls into this CTA's run, as every role derives it for itself.
+// One cell, or the part of one that falls into this CTA's run.  Each role (loads, products, softmax) walks the run with an
+// item of its own in shared memory: a dozen of registers less in every thread.
 struct Item {
     SeqInfo q;
     uint32_t s, kvh, block, blocks, pairs;  // pairs of the block
     uint32_t T, off, n;                     // tiles of the cell, and of those this CTA's [off, off + n)
-    uint64_t pos;                           // of tile `off` in the launch's order
-    bool twin;
-    uint32_t lo, hi;        // keys of the block
-    uint32_t t0, t1;        // tiles to load
-    uint32_t a[2], e[2];    // stream i: tiles a[i], a[i] + step, ... below e[i]
+    uint32_t twin;                          // both streams hold the same pairs
+    uint32_t lo, hi;                        // keys of the block
+    uint32_t t0, t1;                        // tiles to load
+    uint32_t a[2], e[2];                    // stream i: tiles a[i], a[i] + step, ... below e[i]
     uint32_t step;
+    uint32_t more;  // the run goes on
+    uint64_t pos;   // of tile `off` in the launch's order
 };
-
-struct Walk {
+struct Run {
     const AttnParams& p;
-    const SeqInfo* info;  // of the run's first kInfoSeqs sequences
+    const SeqInfo* info;  // of its first kInfoSeqs sequences
     uint32_t s_first;
-    uint64_t run1;
-    Item it;
+    uint64_t end;
 
-    __device__ __forceinline__ void open_seq() {
+    __device__ __forceinline__ void open_seq(Item& it) const {
         if (it.s - s_first < kInfoSeqs) {
             it.q = info[it.s - s_first];
         } else {
@@ -170,14 +170,14 @@ struct Walk {
         }
         it.blocks = (it.q.rows * p.group + kBlockPairs - 1) / kBlockPairs;
     }
-    __device__ __forceinline__ void open_cell(uint32_t off) {
+    __device__ __forceinline__ void open_cell(Item& it, uint32_t off) const {
         const uint32_t all = it.q.rows * p.group, p0 = it.block * kBlockPairs, p1 = min(all, p0 + kBlockPairs);
         it.pairs = p1 - p0;
-        it.twin = it.pairs <= kTile;
+        it.twin = it.pairs <= kTile ? 1u : 0u;
         const KeyRange r = keys_of(it.q, p0, p1, p.group, p.window);
         it.T = max(r.t1 - r.t0, 1u);
         it.off = off;
-        it.n = static_cast<uint32_t>(min(run1 - it.pos, static_cast<uint64_t>(it.T - off)));
+        it.n = static_cast<uint32_t>(min(end - it.pos, static_cast<uint64_t>(it.T - off)));
         it.lo = r.lo;
         it.hi = r.hi;
         it.t0 = min(r.t0 + off, r.t1);
@@ -196,27 +196,23 @@ struct Walk {
                 it.e[i] = min(it.t1, k.t1);
             }
         }
+        it.more = 1;
     }
-    __device__ __forceinline__ bool next() {
+    __device__ __forceinline__ void next(Item& it) const {
         it.pos += it.n;
-        if (it.pos >= run1) return false;
+        it.more = 0;
+        if (it.pos >= end) return;
         if (++it.block == it.blocks) {
             it.block = 0;
             if (++it.kvh == p.pool.kv_heads) {
                 it.kvh = 0;
                 do {  // a sequence with rows follows, since the launch has tiles left
-                    if (++it.s >= p.batch.n_seqs) return false;
-                    open_seq();
+                    if (++it.s >= p.batch.n_seqs) return;
+                    open_seq(it);
                 } while (it.blocks == 0);
             }
         }
-        open_cell(0);
-        return true;
-    }
-    // How many streams use tile t (each reports the tile's stage as read).
-    __device__ __forceinline__ uint32_t users(uint32_t t) const {
-        if (it.twin) return 1u;
-        return (t >= it.a[0] && t < it.e[0] ? 1u : 0u) + (t >= it.a[1] && t < it.e[1] ? 1u : 0u);
+        open_cell(it, 0);
     }
 };
 
@@ -246,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     volatile uint32_t* const abort_flag = word + 2;
     uint32_t* const plan = reinterpret_cast<uint32_t*>(tail_ptr + 424);  // where the run begins: sequence, KV head, block, tile
     SeqInfo* const info = reinterpret_cast<SeqInfo*>(tail_ptr + 448);
-    static_assert(448 + kInfoSeqs * sizeof(SeqInfo) <= kTailBytes, "tail");
+    Item* const items = reinterpret_cast<Item*>(tail_ptr + 448 + kInfoSeqs * sizeof(SeqInfo));  // softmax, products, loads
+    static_assert(kInfoSeqs * sizeof(SeqInfo) % 8 == 0 && 448 + kInfoSeqs * sizeof(SeqInfo) + 3 * sizeof(Item) <= kTailBytes, "tail");
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n_seqs = p.batch.n_seqs, group = p.group, window = p.window, cta = blockIdx.x;
@@ -377,16 +374,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = word[0];
-    Walk w{p, info, 0, run1, {}};
-    if (works) {
-        w.s_first = w.it.s = plan[0];
-        w.it.kvh = plan[1];
-        w.it.block = plan[2];
-        w.it.pos = run0;
-        w.open_seq();
-        w.open_cell(plan[3]);
+    const Run run{p, info, plan[0], run1};
+    if (works && tid % 128 == 0) {
+        Item& first = items[tid / 128];
+        first.s = plan[0];
+        first.kvh = plan[1];
+        first.block = plan[2];
+        first.pos = run0;
+        run.open_seq(first);
+        run.open_cell(first, plan[3]);
     }
-    const Item& it = w.it;
+    __syncthreads();
     // Waits that ran out end the call: every role leaves (or, the softmax threads, walks on through their barriers without
     // waiting), once what the role has in flight has come to rest.
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -413,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const uint32_t row_at = slot << box_shift;           // its first row in the tile
             uint32_t cnt = 0, landed = 0;
             bool ok = true;
+            Item& it = items[2];
             do {
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
                 for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
@@ -462,7 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         ++cnt;
                     }
                 }
-            } while (ok && w.next());
+                __syncwarp();
+                if (lane == 0) run.next(it);
+                __syncwarp();
+            } while (ok && it.more);
             if (!ok) {  // copies in flight land before the block's shared memory goes
                 for (uint32_t n = cnt > NST ? cnt - NST : 0u; n < cnt; ++n)
                     tc::mbar_wait_bounded(bar_full + 8 * (n % NST), (n / NST) & 1u, kWaitClocks);
@@ -473,75 +475,85 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             constexpr uint32_t kType = std::is_same<P, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t kIdS = tc::instr_desc_f16(128, kTile, false) | kType;
             constexpr uint32_t kIdO = tc::instr_desc_f16(128, D, true) | kType;
-            uint32_t base = 0;           // the ring's count at the item's first tile
-            uint32_t n_p[2] = {0, 0};    // weights used so far, per stream
-            uint32_t items = 0;
+            constexpr uint64_t kDescK = tc::smem_desc_base(16, 1024), kDescV = tc::smem_desc_base(Sh::kPanel, 1024);
+            uint32_t base = 0;              // the ring's count at the item's first tile
+            uint32_t used0 = 0, used1 = 0;  // weights used so far, per stream
+            uint32_t n_items = 0;
             bool ok = true;
+            Item& it = items[1];
             do {
-                uint32_t nt[2] = {it.a[0], it.a[1]};
-                bool fresh[2] = {true, true};
-                auto scores = [&](int i) -> bool {
-                    const uint32_t t = nt[i], c = base + 2 * (t - it.t0), st = c % NST;
-                    if (!wait(bar_full + 8 * st, (c / NST) & 1u)) return false;
-                    tc::fence_after_sync();
-                    const uint32_t k = ring + st * Sh::kStage, q = qbuf + (it.twin ? 0u : i * Sh::kQ), d = tmem + i * kTile;
+                // One copy of the code for both streams, its state in registers: this thread's own latency stands between the
+                // products (unrolled for each stream, with the item read from shared memory, it took 1600 clocks a step).
+                const uint32_t t0 = it.t0, step = it.step, twin = it.twin, a0 = it.a[0], a1 = it.a[1], e0 = it.e[0], e1 = it.e[1];
+                uint32_t nt0 = a0, nt1 = a1, pv0 = a0, pv1 = a1;  // next scores, next values
+                uint32_t i = 0, opening = 2;                      // the first two turns only issue scores
+                for (;;) {
+                    const uint32_t parity = (i != 0 ? used1 : used0) & 1u;
+                    const uint32_t end = i != 0 ? e1 : e0;
+                    if (opening == 0) {  // O_i (+)= P_i V(t)
+                        const uint32_t t = i != 0 ? pv1 : pv0;
+                        const uint32_t cn = base + 2 * (t - t0) + 1, st = cn % NST;
+                        ok = wait(bar_full + 8 * st, (cn / NST) & 1u) && wait(bar_p + 8 * i, parity);
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        const uint64_t v = kDescV + ((ring + st * Sh::kStage) >> 4);
+                        const uint32_t pa = tmem + i * kTile, d = tmem + kTmemO + i * D;
+                        const uint32_t more = t != (i != 0 ? a1 : a0) ? 1u : 0u;
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint32_t off = (ks / 4) * Sh::kPanel + (ks % 4) * 32;
-                        tc::mma_f16_ss(d, tc::smem_desc(q + off, 16, 1024), tc::smem_desc(k + off, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
-                        if constexpr (SPLIT)
-                            tc::mma_f16_ss(d, tc::smem_desc(q + Sh::kStage + off, 16, 1024), tc::smem_desc(k + off, 16, 1024), kIdS, 1u);
-                    }
-                    tc::mma_commit(bar_empty + 8 * st);
-                    if (w.users(t) == 1) tc::mma_commit(bar_empty + 8 * st);
-                    tc::mma_commit(bar_s + 8 * i);
-                    nt[i] += it.step;
-                    return true;
-                };
-                auto values = [&](int i, uint32_t t) -> bool {
-                    const uint32_t c = base + 2 * (t - it.t0) + 1, st = c % NST;
-                    if (!wait(bar_p + 8 * i, n_p[i] & 1u)) return false;
-                    ++n_p[i];
-                    if (!wait(bar_full + 8 * st, (c / NST) & 1u)) return false;
-                    tc::fence_after_sync();
-                    const uint32_t v = ring + st * Sh::kStage, a = tmem + i * kTile, d = tmem + kTmemO + i * D;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint64_t desc = tc::smem_desc(v + j * 2048, Sh::kPanel, 1024);
-                        if constexpr (SPLIT) {
-                            tc::mma_f16_ts(d, a + 16 * j, desc, kIdO, j > 0 || !fresh[i] ? 1u : 0u);
-                            tc::mma_f16_ts(d, a + 16 * j + 8, desc, kIdO, 1u);
-                        } else {
-                            tc::mma_f16_ts(d, a + 8 * j, desc, kIdO, j > 0 || !fresh[i] ? 1u : 0u);
+                        for (int j = 0; j < 8; ++j) {
+                            if constexpr (SPLIT) {  // (every tile's output is taken out: see the softmax)
+                                tc::mma_f16_ts(d, pa + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : 0u);
+                                tc::mma_f16_ts(d, pa + 16 * j + 8, v + j * 128, kIdO, 1u);
+                            } else {
+                                tc::mma_f16_ts(d, pa + 8 * j, v + j * 128, kIdO, j > 0 ? 1u : more);
+                            }
                         }
+                        tc::mma_commit(bar_empty + 8 * st);
+                        if (twin != 0 || t < a0 || t < a1 || t >= e0 || t >= e1) tc::mma_commit(bar_empty + 8 * st);  // the tile's only user
+                        used0 += i == 0 ? 1u : 0u;
+                        used1 += i != 0 ? 1u : 0u;
+                        pv0 += i == 0 ? step : 0u;
+                        pv1 += i != 0 ? step : 0u;
+                    } else {
+                        --opening;
+                        ok = wait(bar_q + 8 * i, n_items & 1u);
+                        if (!ok) break;
                     }
-                    fresh[i] = false;
-                    tc::mma_commit(bar_empty + 8 * st);
-                    if (w.users(t) == 1) tc::mma_commit(bar_empty + 8 * st);
-                    return true;
-                };
-                for (int i = 0; ok && i < 2; ++i) {
-                    ok = wait(bar_q + 8 * i, items & 1u);
-                    if (ok && nt[i] < it.e[i]) ok = scores(i);
-                }
-                uint32_t pv[2] = {it.a[0], it.a[1]};
-                while (ok) {
-                    const bool l0 = pv[0] < it.e[0], l1 = pv[1] < it.e[1];
+                    const uint32_t t = i != 0 ? nt1 : nt0;
+                    if (t < end) {  // S_i = Q_i K(t)
+                        const uint32_t cn = base + 2 * (t - t0), st = cn % NST;
+                        ok = wait(bar_full + 8 * st, (cn / NST) & 1u);
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        const uint64_t k = kDescK + ((ring + st * Sh::kStage) >> 4), q = kDescK + ((qbuf + (twin != 0 ? 0u : i * Sh::kQ)) >> 4);
+                        const uint32_t d = tmem + i * kTile;
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            constexpr uint32_t kPanel16 = Sh::kPanel / 16;
+                            const uint32_t off = (ks / 4) * kPanel16 + (ks % 4) * 2;
+                            tc::mma_f16_ss(d, q + off, k + off, kIdS, ks > 0 ? 1u : 0u);
+                            if constexpr (SPLIT) tc::mma_f16_ss(d, q + Sh::kStage / 16 + off, k + off, kIdS, 1u);
+                        }
+                        tc::mma_commit(bar_s + 8 * i);
+                        tc::mma_commit(bar_empty + 8 * st);
+                        if (twin != 0 || t < a0 || t < a1 || t >= e0 || t >= e1) tc::mma_commit(bar_empty + 8 * st);
+                        nt0 += i == 0 ? step : 0u;
+                        nt1 += i != 0 ? step : 0u;
+                    } else if (opening == 0 && (i != 0 ? a1 < e1 : a0 < e0)) {
+                        tc::mma_commit(bar_o + 8 * i);  // its last values have been issued
+                    }
+                    if (opening != 0) {
+                        i = 1;
+                        continue;
+                    }
+                    const bool l0 = pv0 < e0, l1 = pv1 < e1;
                     if (!l0 && !l1) break;
-                    const int i = l0 && (!l1 || pv[0] <= pv[1]) ? 0 : 1;
-                    const uint32_t t = i == 0 ? pv[0] : pv[1];
-                    ok = i == 0 ? values(0, t) : values(1, t);
-                    if (i == 0)
-                        pv[0] += it.step;
-                    else
-                        pv[1] += it.step;
-                    const bool more = i == 0 ? nt[0] < it.e[0] : nt[1] < it.e[1];
-                    if (ok && more) ok = i == 0 ? scores(0) : scores(1);
-                    if (ok && !more) tc::mma_commit(bar_o + 8 * i);
+                    i = l0 && (!l1 || pv0 <= pv1) ? 0u : 1u;
                 }
-                base += 2 * (it.t1 - it.t0);
-                ++items;
-            } while (ok && w.next());
+                base += 2 * (it.t1 - t0);
+                ++n_items;
+                run.next(it);
+            } while (ok && it.more);
             tc::mma_commit(bar_done);
             tc::mbar_wait_bounded(bar_done, 0u, kWaitClocks);
         }
@@ -557,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const uint32_t head_dim = p.pool.head_dim;
         uint32_t n_s = 0, n_o = 0;  // scores seen, last products seen
         bool dead = !works;         // a wait ran out: walk on through the barriers, touch nothing
+        Item& it = items[0];
         if (works) do {
             // ---- the block's queries into shared memory: warp by warp, 16 bytes a lane
             if (i == 0 || !it.twin) {
@@ -618,76 +631,126 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             // keys (low, at] are seen
             const int32_t low = window != 0 ? at - static_cast<int32_t>(min(window, 0x7fffffffu)) : -1;
             float m = -INFINITY, l = 0.f;
-            const uint32_t a = i == 0 ? it.a[0] : it.a[1], e = i == 0 ? it.e[0] : it.e[1];
+            float acc[SPLIT ? D : 1];  // f32 rows: the output so far
+#pragma unroll
+            for (int u = 0; u < (SPLIT ? D : 1); ++u) acc[u] = 0.f;
+            auto take_output = [&]() {
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        uint32_t o[16];
+                        tc::tmem_ld16(tO + 16 * j, o);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) acc[16 * j + u] += __uint_as_float(o[u]);
+                    }
+                }
+            };
+            const uint32_t a = it.a[i], e = it.e[i], step = it.step;
             const bool any = a < e;
-            for (uint32_t t = a; t < e; t += it.step) {
+            for (uint32_t t = a; t < e; t += step) {
                 dead = dead || !wait(bar_s + 8 * i, n_s & 1u);
                 dead = __any_sync(0xffffffffu, dead);
                 if (dead) break;
                 ++n_s;
                 tc::fence_after_sync();
-                uint32_t x[4][32];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) tc::tmem_ld32(tS + 32 * j, x[j]);
-                tc::tmem_wait_ld();
                 const int32_t from = low - static_cast<int32_t>(t * kTile), to = at - static_cast<int32_t>(t * kTile);  // columns (from, to]
-                if (__any_sync(0xffffffffu, live && (from >= 0 || to < static_cast<int32_t>(kTile) - 1))) {
+                const bool masked = __any_sync(0xffffffffu, live && (from >= 0 || to < static_cast<int32_t>(kTile) - 1));
+                auto hide = [&](auto& x, int col0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) {
-                            const int32_t col = 32 * j + u;
-                            if (col <= from || col > to) x[j][u] = 0xff800000u;
-                        }
-                }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int u = 0; u < 32; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[j][u]));
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-                const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-                    if (t != a) {  // the scores at hand vouch for every product before them: O is at rest
-#pragma unroll 1
-                        for (int j = 0; j < D; j += 16) {
-                            uint32_t o[16];
-                            tc::tmem_ld16(tO + j, o);
-                            tc::tmem_wait_ld();
-#pragma unroll
-                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                            tc::tmem_st16(tO + j, o);
-                        }
-                    }
-                    if (grow) m = mx;
-                    l *= f;
-                }
-                const float nm = m == -INFINITY ? 0.f : -m;
+                    for (int u = 0; u < static_cast<int>(sizeof(x) / 4); ++u)
+                        if (col0 + u <= from || col0 + u > to) x[u] = 0xff800000u;
+                };
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (SPLIT) {
+                    // The tensor core cuts its sums short of a rounding, which adds up over a long accumulation: a tile's
+                    // output is taken out of tensor memory and added here, and the scores are read twice to make room.
+                    if (t != a) take_output();
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t x[16];
+                        tc::tmem_ld16(tS + 16 * j, x);
+                        tc::tmem_wait_ld();
+                        if (masked) hide(x, 16 * j);
+                        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) {
-                        const float wgt = fast_exp2(fmaf(__uint_as_float(x[j][u]), c, nm));
-                        sum[u & 3] += wgt;
-                        x[j][u] = __float_as_uint(wgt);
+                        for (int u = 0; u < 16; ++u) top[u & 1] = fmaxf(top[u & 1], __uint_as_float(x[u]));
+                        mx = fmaxf(mx, fmaxf(top[0], top[1]));
                     }
-                    if constexpr (SPLIT) {
-                        uint32_t y[32];  // keys 16 s ..: high terms in columns 16 s .., low terms in 16 s + 8 ..
+                    mx *= c;
+                    const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) {
-                            __half h0, l0, h1, l1;
-                            split_half(__uint_as_float(x[j][2 * u]), h0, l0);
-                            split_half(__uint_as_float(x[j][2 * u + 1]), h1, l1);
-                            y[(u / 8) * 16 + u % 8] = pack_half2(h0, h1);
-                            y[(u / 8) * 16 + 8 + u % 8] = pack_half2(l0, l1);
+                        for (int u = 0; u < D; ++u) acc[u] *= f;
+                        if (grow) m = mx;
+                        l *= f;
+                    }
+                    const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {  // 16 keys: high terms in their columns 0-7, low terms in 8-15
+                        uint32_t x[16], y[16];
+                        tc::tmem_ld16(tS + 16 * j, x);
+                        tc::tmem_wait_ld();
+                        if (masked) hide(x, 16 * j);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const float w0 = fast_exp2(fmaf(__uint_as_float(x[2 * u]), c, nm));
+                            const float w1 = fast_exp2(fmaf(__uint_as_float(x[2 * u + 1]), c, nm));
+                            sum[u & 1] += w0;
+                            sum[2 + (u & 1)] += w1;
+                            const __half2 h = __floats2half2_rn(w0, w1);
+                            const float2 hf = __half22float2(h);
+                            y[u] = *reinterpret_cast<const uint32_t*>(&h);
+                            y[8 + u] = pack2(__half(), w0 - hf.x, w1 - hf.y);
                         }
-                        tc::tmem_st32(tS + 32 * j, y);
-                    } else {
+                        tc::tmem_st16(tS + 16 * j, y);
+                    }
+                } else {
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) tc::tmem_ld32(tS + 32 * j, x[j]);
+                    tc::tmem_wait_ld();
+                    if (masked) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) hide(x[j], 32 * j);
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int u = 0; u < 32; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[j][u]));
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                    const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+                        if (t != a) {  // the scores at hand vouch for every product before them: O is at rest
+#pragma unroll 1
+                            for (int j = 0; j < D; j += 16) {
+                                uint32_t o[16];
+                                tc::tmem_ld16(tO + j, o);
+                                tc::tmem_wait_ld();
+#pragma unroll
+                                for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                                tc::tmem_st16(tO + j, o);
+                            }
+                        }
+                        if (grow) m = mx;
+                        l *= f;
+                    }
+                    const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
                         uint32_t y[16];
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) y[u] = pack2(P(), __uint_as_float(x[j][2 * u]), __uint_as_float(x[j][2 * u + 1]));
+                        for (int u = 0; u < 16; ++u) {
+                            const float w0 = fast_exp2(fmaf(__uint_as_float(x[j][2 * u]), c, nm));
+                            const float w1 = fast_exp2(fmaf(__uint_as_float(x[j][2 * u + 1]), c, nm));
+                            sum[u & 1] += w0;
+                            sum[2 + (u & 1)] += w1;
+                            y[u] = pack2(P(), w0, w1);
+                        }
                         tc::tmem_st16(tS + 16 * j, y);
                     }
                 }
@@ -701,6 +764,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 dead = __any_sync(0xffffffffu, dead);
                 ++n_o;
                 tc::fence_after_sync();
+                if constexpr (SPLIT) {  // back to where the cell's end expects it
+                    if (!dead) {
+                        take_output();
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j) {
+                            uint32_t o[16];
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(acc[16 * j + u]);
+                            tc::tmem_st16(tO + 16 * j, o);
+                        }
+                        tc::tmem_wait_st();
+                    }
+                }
             }
 
             // ---- the cell's end ----------------------------------------------------------------------------------------
@@ -710,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             bool other_any = false;
             if (it.twin) {
                 // Rows are the same in both streams and sit in the same lanes: each warpgroup takes half of the channels.
-                other_any = i == 0 ? it.a[1] < it.e[1] : it.a[0] < it.e[0];
+                other_any = it.a[1 - i] < it.e[1 - i];
                 ex[tid] = make_float2(m, l);
                 tc::fence_before_sync();
                 both_sync();
@@ -729,16 +805,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             float4* const po = reinterpret_cast<float4*>(p.part_o) + static_cast<size_t>(part) * (D / 4) * kBlockPairs;
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
             T* const dst = static_cast<T*>(p.out) + static_cast<uint64_t>(row) * p.out_row + head * head_dim;
-            auto put8 = [&](uint32_t ch, const float (&f)[8]) {
-                if (live && ch < head_dim) {
-                    Vec8<T> v;
-                    if constexpr (SPLIT) {
-                        v.set(f);
-                    } else {
-                        v.w = make_uint4(pack2(P(), f[0], f[1]), pack2(P(), f[2], f[3]), pack2(P(), f[4], f[5]), pack2(P(), f[6], f[7]));
-                    }
-                    v.store(dst + ch);
+            auto put8 = [&](T* to, const float (&f)[8]) {
+                Vec8<T> v;
+                if constexpr (SPLIT) {
+                    v.set(f);
+                } else {
+                    v.w = make_uint4(pack2(P(), f[0], f[1]), pack2(P(), f[2], f[3]), pack2(P(), f[4], f[5]), pack2(P(), f[6], f[7]));
                 }
+                v.store(to);
             };
             if (!dead) {
 #pragma unroll 1
@@ -759,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             float z[8];
 #pragma unroll
                             for (int u = 0; u < 8; ++u) z[u] = f[8 * g8 + u] * inv;
-                            put8(ch + 8 * g8, z);
+                            if (live && ch + 8 * g8 < head_dim) put8(dst + ch + 8 * g8, z);
                         }
                     } else if (live) {
 #pragma unroll
@@ -768,13 +842,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
             }
-            auto put_lse = [&](float top, float sum) {
-                if (live && p.lse && (i == 0 || !it.twin))
-                    p.lse[static_cast<uint64_t>(row) * p.q_heads + head] =
+            auto put_lse = [&](uint32_t lrow, uint32_t lhead, float top, float sum) {
+                if (p.lse)
+                    p.lse[static_cast<uint64_t>(lrow) * p.q_heads + lhead] =
                         sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
             };
             if (whole) {
-                if (!dead) put_lse(m, l);
+                if (!dead && live && (i == 0 || !it.twin)) put_lse(row, head, m, l);
             } else {
                 float2* const pml = reinterpret_cast<float2*>(p.part_ml);
                 if (live && (i == 0 || !it.twin)) pml[static_cast<size_t>(part) * kBlockPairs + in] = make_float2(m, l);
@@ -790,44 +864,66 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 both_sync();
                 if (word[1] != 0u && !dead) {
                     __threadfence();
-                    // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...
-                    if (live) {
-                        float M = -INFINITY, L = 0.f;
-                        for (uint32_t k = first; k <= last; ++k) {
-                            const float2 x = __ldcg(pml + static_cast<size_t>(k == first ? 2 * k + 1 : 2 * k) * kBlockPairs + in);
-                            const float to = fmaxf(M, x.x);
-                            const float g0 = M == -INFINITY ? 0.f : fast_exp2(M - to), g1 = x.x == -INFINITY ? 0.f : fast_exp2(x.x - to);
-                            L = L * g0 + x.y * g1;
-                            M = to;
-                        }
-                        const float il = L > 0.f || L != L ? 1.f / L : 0.f;
-                        const float4* const all = reinterpret_cast<const float4*>(p.part_o);
+                    // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...  Lanes
+                    // take neighbouring rows; a thread has the loads of several parts in flight.
+                    const uint32_t across = (it.pairs + 31) / 32 * 32, n_parts = last - first + 1;
+                    const float4* const all = reinterpret_cast<const float4*>(p.part_o);
+                    auto join = [&](auto batch) {
+                        constexpr uint32_t B = decltype(batch)::value;
 #pragma unroll 1
-                        for (uint32_t ch = c0; ch < c1; ch += 8) {
-                            float z[8] = {};
-#pragma unroll 4
-                            for (uint32_t k = first; k <= last; ++k) {
-                                const size_t sl = k == first ? 2 * k + 1 : 2 * k;
-                                const float mk = __ldcg(pml + sl * kBlockPairs + in).x;
-                                const float g1 = mk == -INFINITY ? 0.f : fast_exp2(mk - M);
-                                const float4 u0 = __ldcg(all + (sl * (D / 4) + ch / 4) * kBlockPairs + in);
-                                const float4 u1 = __ldcg(all + (sl * (D / 4) + ch / 4 + 1) * kBlockPairs + in);
-                                z[0] += g1 * u0.x, z[1] += g1 * u0.y, z[2] += g1 * u0.z, z[3] += g1 * u0.w;
-                                z[4] += g1 * u1.x, z[5] += g1 * u1.y, z[6] += g1 * u1.z, z[7] += g1 * u1.w;
-                            }
+                        for (uint32_t u = tid; u < across * (head_dim / 8); u += 256) {
+                            const uint32_t jr = u % across, c8 = u / across;
+                            if (jr >= it.pairs) continue;
+                            float M = -INFINITY, L = 0.f, z[8] = {};
+#pragma unroll 1
+                            for (uint32_t k0 = 0; k0 < n_parts; k0 += B) {
+                                float2 ml[B];
+                                float4 o0[B], o1[B];
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) z[u] *= il;
-                            put8(ch, z);
+                                for (uint32_t k = 0; k < B; ++k) {
+                                    const uint32_t kk = min(k0 + k, n_parts - 1);
+                                    const size_t sl = 2 * (first + kk) + (kk == 0 ? 1 : 0);
+                                    ml[k] = __ldcg(pml + sl * kBlockPairs + jr);
+                                    o0[k] = __ldcg(all + (sl * (D / 4) + 2 * c8) * kBlockPairs + jr);
+                                    o1[k] = __ldcg(all + (sl * (D / 4) + 2 * c8 + 1) * kBlockPairs + jr);
+                                }
+                                float to = M;
+#pragma unroll
+                                for (uint32_t k = 0; k < B; ++k) to = fmaxf(to, ml[k].x);
+                                const float g0 = M == -INFINITY ? 0.f : fast_exp2(M - to);
+                                L *= g0;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) z[e] *= g0;
+                                M = to;
+#pragma unroll
+                                for (uint32_t k = 0; k < B; ++k) {
+                                    const float g1 = k0 + k < n_parts && ml[k].x != -INFINITY ? fast_exp2(ml[k].x - M) : 0.f;
+                                    L += g1 * ml[k].y;
+                                    z[0] += g1 * o0[k].x, z[1] += g1 * o0[k].y, z[2] += g1 * o0[k].z, z[3] += g1 * o0[k].w;
+                                    z[4] += g1 * o1[k].x, z[5] += g1 * o1[k].y, z[6] += g1 * o1[k].z, z[7] += g1 * o1[k].w;
+                                }
+                            }
+                            const float il = L > 0.f || L != L ? 1.f / L : 0.f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) z[e] *= il;
+                            const uint32_t jp = it.block * kBlockPairs + jr, jrow = it.q.row0 + jp / group, jhead = it.kvh * group + jp % group;
+                            put8(static_cast<T*>(p.out) + static_cast<uint64_t>(jrow) * p.out_row + jhead * head_dim + 8 * c8, z);
+                            if (c8 == 0) put_lse(jrow, jhead, M, L);
                         }
-                        put_lse(M, L);
-                    }
+                    };
+                    if (n_parts <= 2)
+                        join(std::integral_constant<uint32_t, 2>());
+                    else
+                        join(std::integral_constant<uint32_t, 6>());
                 }
             }
             // Nothing of this cell is read any more: the exchange, the other stream's accumulator, the joined flag.
             tc::fence_before_sync();
             both_sync();
+            if (tid == 0) run.next(it);
+            both_sync();
             tc::fence_after_sync();
-        } while (w.next());
+        } while (it.more);
     }
     tc::fence_before_sync();
     __syncthreads();

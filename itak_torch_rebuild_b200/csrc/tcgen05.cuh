@@ -30,6 +30,13 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes
     return d;
 }
 
+// The same without the address: add (address >> 4), and multiples of 16 bytes to move on (shared memory ends below
+// 2^18 bytes, so the 14-bit field does not run over).
+__host__ __device__ constexpr uint64_t smem_desc_base(uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    return (static_cast<uint64_t>((lbo_bytes >> 4) & 0x3fffu) << 16) | (static_cast<uint64_t>((sbo_bytes >> 4) & 0x3fffu) << 32) |
+           (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
 // 32-bit instruction descriptor of kind::f16 with f16 operands and f32 accumulation: accumulator format f32
 // (bits 4-5 = 1), A/B format f16 (0), B major-ness (bit 16: 1 = MN-major), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
 __host__ __device__ constexpr uint32_t instr_desc_f16(uint32_t m, uint32_t n, bool b_mn_major) {
