@@ -46,7 +46,7 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 384;  // two warpgroups of softmax, and one of product, load and two idle warps
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;  // stream i's products: warp kMmaWarp + 2 i
 // Registers: the softmax threads hold a whole row of scores.  setmaxnreg moves registers between the warpgroups of a
 // block launched with kLaunchRegs a thread: 256 x 216 + 128 x 72 = 384 x 168.
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
@@ -118,6 +118,32 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Two f32 values in one 64-bit register: the packed forms do two multiply-adds or sums in one issue.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN when one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // The keys that pairs [p0, p1) of a sequence see, and the 128-key tiles that hold them (none: t0 == t1).
 struct KeyRange {
     uint32_t lo, hi, t0, t1;
@@ -232,18 +258,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint32_t bar_full = tail;                // [stage] the tile has landed
     const uint32_t bar_empty = bar_full + 8 * 16;  // [stage] every product that reads it is complete
     const uint32_t bar_s = bar_empty + 8 * 16;     // [stream] scores complete
-    const uint32_t bar_p = bar_s + 16;             // [stream] weights stored
-    const uint32_t bar_o = bar_p + 16;             // [stream] the cell's last product complete
+    const uint32_t bar_p = bar_s + 16;             // [stream][half] the weights of half of the tile's keys are stored
+    const uint32_t bar_o = bar_p + 32;             // [stream] the cell's last product complete
     const uint32_t bar_q = bar_o + 16;             // [stream] the cell's queries are in shared memory
     const uint32_t bar_land = bar_q + 16;          // a V tile that needs zero rows has landed
     const uint32_t bar_done = bar_land + 8;        // everything issued to the tensor core is complete
+    const uint32_t bar_turn = bar_done + 8;        // [stream] its products of a round are issued
     static_assert(NST <= 16, "stages");
     uint32_t* const word = reinterpret_cast<uint32_t*>(tail_ptr + 400);  // [0] tensor memory, [1] joined flag, [2] abort
     volatile uint32_t* const abort_flag = word + 2;
     uint32_t* const plan = reinterpret_cast<uint32_t*>(tail_ptr + 424);  // where the run begins: sequence, KV head, block, tile
     SeqInfo* const info = reinterpret_cast<SeqInfo*>(tail_ptr + 448);
-    Item* const items = reinterpret_cast<Item*>(tail_ptr + 448 + kInfoSeqs * sizeof(SeqInfo));  // softmax, products, loads
-    static_assert(kInfoSeqs * sizeof(SeqInfo) % 8 == 0 && 448 + kInfoSeqs * sizeof(SeqInfo) + 3 * sizeof(Item) <= kTailBytes, "tail");
+    Item* const items = reinterpret_cast<Item*>(tail_ptr + 448 + kInfoSeqs * sizeof(SeqInfo));  // softmax, products of stream 0 and 1, loads
+    static_assert(kInfoSeqs * sizeof(SeqInfo) % 8 == 0 && 448 + kInfoSeqs * sizeof(SeqInfo) + 4 * sizeof(Item) <= kTailBytes, "tail");
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n_seqs = p.batch.n_seqs, group = p.group, window = p.window, cta = blockIdx.x;
@@ -256,12 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         }
         for (uint32_t i = 0; i < 2; ++i) {
             tc::mbar_init(bar_s + 8 * i, 1);
-            tc::mbar_init(bar_p + 8 * i, 128);
+            tc::mbar_init(bar_p + 16 * i, 128);
+            tc::mbar_init(bar_p + 16 * i + 8, 128);
             tc::mbar_init(bar_o + 8 * i, 1);
             tc::mbar_init(bar_q + 8 * i, 128);
+            tc::mbar_init(bar_turn + 8 * i, 1);
         }
         tc::mbar_init(bar_land, 1);
-        tc::mbar_init(bar_done, 1);
+        tc::mbar_init(bar_done, 2);
         *abort_flag = 0;
         tc::fence_mbar_init();
     }
@@ -375,8 +404,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     tc::fence_after_sync();
     const uint32_t tmem = word[0];
     const Run run{p, info, plan[0], run1};
-    if (works && tid % 128 == 0) {
-        Item& first = items[tid / 128];
+    if (works && tid % 64 == 0 && tid < 256) {
+        Item& first = items[tid / 64];
         first.s = plan[0];
         first.kvh = plan[1];
         first.block = plan[2];
@@ -411,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const uint32_t row_at = slot << box_shift;           // its first row in the tile
             uint32_t cnt = 0, landed = 0;
             bool ok = true;
-            Item& it = items[2];
+            Item& it = items[3];
             do {
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
                 for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
@@ -470,87 +499,97 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     tc::mbar_wait_bounded(bar_full + 8 * (n % NST), (n / NST) & 1u, kWaitClocks);
                 tc::mbar_wait_bounded(bar_land, landed & 1u, kWaitClocks);
             }
-        } else if (warp == kMmaWarp && works && lane == 0) {
-            // ---------------- products ---------------------------------------------------------------------------------
+        } else if ((warp == kMmaWarp || warp == kMmaWarp + 2) && works && lane == 0) {
+            // ---------------- products of one stream ---------------------------------------------------------------------
+            // A round is O += P V(t), S = Q K(t + 1).  The streams take turns round by round: left alone they fall into step,
+            // both softmaxes at a time and both products at a time, each of the two waiting for the other half of the SM
+            // (4400 clocks for two rounds).  One issuing thread each, since between two rounds a thread needs 500 clocks for
+            // waits, releases and descriptors (with one for both the tensor core idled for 1300 of every 2400 clocks): what can
+            // be waited for is waited for before the turn, and stages are released behind the round.
+            const uint32_t i = (warp - kMmaWarp) / 2;
             constexpr uint32_t kType = std::is_same<P, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t kIdS = tc::instr_desc_f16(128, kTile, false) | kType;
             constexpr uint32_t kIdO = tc::instr_desc_f16(128, D, true) | kType;
             constexpr uint64_t kDescK = tc::smem_desc_base(16, 1024), kDescV = tc::smem_desc_base(Sh::kPanel, 1024);
-            uint32_t base = 0;              // the ring's count at the item's first tile
-            uint32_t used0 = 0, used1 = 0;  // weights used so far, per stream
-            uint32_t n_items = 0;
+            const uint32_t tS = tmem + i * kTile, tO = tmem + kTmemO + i * D;
+            uint32_t base = 0;  // the ring's count at the item's first tile
+            uint32_t n_p = 0, n_items = 0, turns = 0;  // turns: the other stream's rounds of the cells before
             bool ok = true;
-            Item& it = items[1];
+            Item& it = items[1 + i];
             do {
-                // One copy of the code for both streams, its state in registers: this thread's own latency stands between the
-                // products (unrolled for each stream, with the item read from shared memory, it took 1600 clocks a step).
-                const uint32_t t0 = it.t0, step = it.step, twin = it.twin, a0 = it.a[0], a1 = it.a[1], e0 = it.e[0], e1 = it.e[1];
-                uint32_t nt0 = a0, nt1 = a1, pv0 = a0, pv1 = a1;  // next scores, next values
-                uint32_t i = 0, opening = 2;                      // the first two turns only issue scores
-                for (;;) {
-                    const uint32_t parity = (i != 0 ? used1 : used0) & 1u;
-                    const uint32_t end = i != 0 ? e1 : e0;
-                    if (opening == 0) {  // O_i (+)= P_i V(t)
-                        const uint32_t t = i != 0 ? pv1 : pv0;
-                        const uint32_t cn = base + 2 * (t - t0) + 1, st = cn % NST;
-                        ok = wait(bar_full + 8 * st, (cn / NST) & 1u) && wait(bar_p + 8 * i, parity);
-                        if (!ok) break;
+                const uint32_t t0 = it.t0, step = it.step, twin = it.twin, a = it.a[i], e = it.e[i];
+                const uint32_t oa = twin != 0 ? e : it.a[1 - i], oe = twin != 0 ? 0u : it.e[1 - i];  // tiles the other stream reads too
+                const uint64_t q = kDescK + ((qbuf + (twin != 0 ? 0u : i * Sh::kQ)) >> 4);
+                auto full = [&](uint32_t cn) { return wait(bar_full + 8 * (cn % NST), (cn / NST) & 1u); };
+                auto release = [&](uint32_t cn, uint32_t t) {  // a stage is free after two of these
+                    tc::mma_commit(bar_empty + 8 * (cn % NST));
+                    if (t < oa || t >= oe) tc::mma_commit(bar_empty + 8 * (cn % NST));
+                };
+                auto scores = [&](uint32_t cn) {  // S = Q K(t)
+                    const uint64_t k = kDescK + ((ring + cn % NST * Sh::kStage) >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        if (ks == D / 32) mbar_arrive(bar_turn + 8 * i);  // the other thread takes a while to see it
+                        constexpr uint32_t kPanel16 = Sh::kPanel / 16;
+                        const uint32_t off = (ks / 4) * kPanel16 + (ks % 4) * 2;
+                        tc::mma_f16_ss(tS, q + off, k + off, kIdS, ks > 0 ? 1u : 0u);
+                        if constexpr (SPLIT) tc::mma_f16_ss(tS, q + Sh::kStage / 16 + off, k + off, kIdS, 1u);
+                    }
+                };
+                ok = wait(bar_q + 8 * i, n_items & 1u);
+                const uint32_t xa = it.a[1 - i], xe = it.e[1 - i];
+                const uint32_t rounds = xa < xe ? (xe - xa + step - 1) / step + 1 : 0u;  // of the other stream: 0, 1, ...
+                // One copy of the code: the first round has no weights to use yet, the last no scores to make.
+                uint32_t after = i == 0 ? 0xffffffffu : 0u;  // the other stream's round that this one follows (stream 0 begins)
+                for (uint32_t nt = a; ok && a < e; nt += step, ++after) {
+                    const bool have = nt != a, more = nt < e;  // weights of tile t; scores of tile nt to come
+                    const uint32_t t = nt - step;
+                    const uint32_t cv = base + 2 * (t - t0) + 1, ck = base + 2 * (nt - t0);
+                    // (with three stages K(t + 2) takes the place of V(t), which has to be used first)
+                    constexpr bool kAhead = NST >= 5;
+                    if (have) ok = full(cv);
+                    if (ok && more && (kAhead || twin == 0 || !have)) ok = full(ck);
+                    if (ok && have) ok = wait(bar_p + 16 * i, n_p & 1u);
+                    if (ok && after < rounds) ok = wait(bar_turn + 8 * (1 - i), (turns + after) & 1u);
+                    if (ok && have) {  // O (+)= P V(t)
                         tc::fence_after_sync();
-                        const uint64_t v = kDescV + ((ring + st * Sh::kStage) >> 4);
-                        const uint32_t pa = tmem + i * kTile, d = tmem + kTmemO + i * D;
-                        const uint32_t more = t != (i != 0 ? a1 : a0) ? 1u : 0u;
+                        const uint64_t v = kDescV + ((ring + cv % NST * Sh::kStage) >> 4);
+                        const uint32_t acc = t != a ? 1u : 0u;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
+                            if (j == 4) {
+                                ok = wait(bar_p + 16 * i + 8, n_p & 1u);
+                                if (!ok) break;
+                                tc::fence_after_sync();
+                            }
                             if constexpr (SPLIT) {  // (every tile's output is taken out: see the softmax)
-                                tc::mma_f16_ts(d, pa + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : 0u);
-                                tc::mma_f16_ts(d, pa + 16 * j + 8, v + j * 128, kIdO, 1u);
+                                tc::mma_f16_ts(tO, tS + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : 0u);
+                                tc::mma_f16_ts(tO, tS + 16 * j + 8, v + j * 128, kIdO, 1u);
                             } else {
-                                tc::mma_f16_ts(d, pa + 8 * j, v + j * 128, kIdO, j > 0 ? 1u : more);
+                                tc::mma_f16_ts(tO, tS + 8 * j, v + j * 128, kIdO, j > 0 ? 1u : acc);
                             }
                         }
-                        tc::mma_commit(bar_empty + 8 * st);
-                        if (twin != 0 || t < a0 || t < a1 || t >= e0 || t >= e1) tc::mma_commit(bar_empty + 8 * st);  // the tile's only user
-                        used0 += i == 0 ? 1u : 0u;
-                        used1 += i != 0 ? 1u : 0u;
-                        pv0 += i == 0 ? step : 0u;
-                        pv1 += i != 0 ? step : 0u;
-                    } else {
-                        --opening;
-                        ok = wait(bar_q + 8 * i, n_items & 1u);
-                        if (!ok) break;
-                    }
-                    const uint32_t t = i != 0 ? nt1 : nt0;
-                    if (t < end) {  // S_i = Q_i K(t)
-                        const uint32_t cn = base + 2 * (t - t0), st = cn % NST;
-                        ok = wait(bar_full + 8 * st, (cn / NST) & 1u);
-                        if (!ok) break;
-                        tc::fence_after_sync();
-                        const uint64_t k = kDescK + ((ring + st * Sh::kStage) >> 4), q = kDescK + ((qbuf + (twin != 0 ? 0u : i * Sh::kQ)) >> 4);
-                        const uint32_t d = tmem + i * kTile;
-#pragma unroll
-                        for (int ks = 0; ks < D / 16; ++ks) {
-                            constexpr uint32_t kPanel16 = Sh::kPanel / 16;
-                            const uint32_t off = (ks / 4) * kPanel16 + (ks % 4) * 2;
-                            tc::mma_f16_ss(d, q + off, k + off, kIdS, ks > 0 ? 1u : 0u);
-                            if constexpr (SPLIT) tc::mma_f16_ss(d, q + Sh::kStage / 16 + off, k + off, kIdS, 1u);
+                        ++n_p;
+                        if (!kAhead && twin != 0) {
+                            release(cv, t);
+                            if (ok && more) ok = full(ck);
                         }
+                    }
+                    if (!ok) break;
+                    if (more) {
+                        tc::fence_after_sync();
+                        scores(ck);
                         tc::mma_commit(bar_s + 8 * i);
-                        tc::mma_commit(bar_empty + 8 * st);
-                        if (twin != 0 || t < a0 || t < a1 || t >= e0 || t >= e1) tc::mma_commit(bar_empty + 8 * st);
-                        nt0 += i == 0 ? step : 0u;
-                        nt1 += i != 0 ? step : 0u;
-                    } else if (opening == 0 && (i != 0 ? a1 < e1 : a0 < e0)) {
-                        tc::mma_commit(bar_o + 8 * i);  // its last values have been issued
+                        release(ck, nt);
+                    } else {
+                        mbar_arrive(bar_turn + 8 * i);
+                        tc::mma_commit(bar_o + 8 * i);
                     }
-                    if (opening != 0) {
-                        i = 1;
-                        continue;
-                    }
-                    const bool l0 = pv0 < e0, l1 = pv1 < e1;
-                    if (!l0 && !l1) break;
-                    i = l0 && (!l1 || pv0 <= pv1) ? 0u : 1u;
+                    if (have && (kAhead || twin == 0)) release(cv, t);
+                    if (!more) break;
                 }
                 base += 2 * (it.t1 - t0);
+                turns += rounds;
                 ++n_items;
                 run.next(it);
             } while (ok && it.more);
@@ -646,6 +685,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
             };
+            auto stored = [&](uint32_t half) {  // the weights of half of the tile's keys may be used
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                mbar_arrive(bar_p + 16 * i + 8 * half);
+            };
             const uint32_t a = it.a[i], e = it.e[i], step = it.step;
             const bool any = a < e;
             for (uint32_t t = a; t < e; t += step) {
@@ -706,6 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             y[8 + u] = pack2(__half(), w0 - hf.x, w1 - hf.y);
                         }
                         tc::tmem_st16(tS + 16 * j, y);
+                        if (j == 3) stored(0);
                     }
                 } else {
                     uint32_t x[4][32];
@@ -718,10 +763,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int u = 0; u < 32; ++u)
+                    for (int u = 0; u < 32; u += 2)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[j][u]));
-                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                        for (int j = 0; j < 4; ++j) top[j] = max3(top[j], __uint_as_float(x[j][u]), __uint_as_float(x[j][u + 1]));
+                    const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;
                     const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
@@ -739,24 +784,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         if (grow) m = mx;
                         l *= f;
                     }
-                    const float nm = m == -INFINITY ? 0.f : -m;
+                    if (!(mx < INFINITY)) m = NAN;  // a NaN or +infinity among the scores: the row is NaN from here on
+                    const uint64_t c2 = pair_of(c, c), nm2 = pair_of(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+                    uint64_t sum2[2] = {0u, 0u};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t y[16];
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
-                            const float w0 = fast_exp2(fmaf(__uint_as_float(x[j][2 * u]), c, nm));
-                            const float w1 = fast_exp2(fmaf(__uint_as_float(x[j][2 * u + 1]), c, nm));
-                            sum[u & 1] += w0;
-                            sum[2 + (u & 1)] += w1;
-                            y[u] = pack2(P(), w0, w1);
+                            const uint64_t v = fma2(pair_of(__uint_as_float(x[j][2 * u]), __uint_as_float(x[j][2 * u + 1])), c2, nm2);
+                            float2 e2 = unpair(v);
+                            e2 = make_float2(fast_exp2(e2.x), fast_exp2(e2.y));
+                            sum2[u & 1] = add2(sum2[u & 1], pair_of(e2.x, e2.y));
+                            y[u] = pack2(P(), e2.x, e2.y);
                         }
                         tc::tmem_st16(tS + 16 * j, y);
+                        if (j == 1) stored(0);
                     }
+                    const float2 s01 = unpair(add2(sum2[0], sum2[1]));
+                    sum[0] = s01.x;
+                    sum[1] = s01.y;
                 }
-                tc::tmem_wait_st();
-                tc::fence_before_sync();
-                mbar_arrive(bar_p + 8 * i);
+                stored(1);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             if (any && !dead) {
