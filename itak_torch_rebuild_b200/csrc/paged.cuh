@@ -14,6 +14,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/itak_cuda_compute.h"
 #include "kv_convert.cuh"
 
@@ -79,6 +81,7 @@ struct AttnParams {
     void* out;
     float* lse;
     uint64_t q_row, out_row;  // elements
+    int device;
     uint32_t q_heads, group, window;
     float scale_log2;  // scale * log2(e)
     unsigned int* tickets;  // zero between launches
@@ -205,6 +208,19 @@ public:
 private:
     int prev_ = 0;
     bool changed_ = false;
+};
+
+// Whether something that holds for a device from its first use on (a kernel's shared-memory limit) has been done there.
+// Two threads may both find it undone and do it twice.
+class OncePerDevice {
+public:
+    bool done(int device) const { return device >= 0 && device < 64 && ((bits_.load(std::memory_order_acquire) >> device) & 1u) != 0; }
+    void mark(int device) {
+        if (device >= 0 && device < 64) bits_.fetch_or(1ull << device, std::memory_order_release);
+    }
+
+private:
+    std::atomic<uint64_t> bits_{0};
 };
 
 constexpr uint64_t kMaxStride = 1ull << 40;

@@ -82,6 +82,7 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     const Layout l = layout_of(sms);
     if (d->workspace_bytes < l.bytes) return e.refuse(ITK_ERR_CAPACITY, "the workspace holds %llu bytes, %llu are needed", d->workspace_bytes, l.bytes);
     if (batch->total_rows == 0) return 0;
+    p.device = kv->device;
     p.q = d->q;
     p.out = d->out;
     p.lse = d->lse;

@@ -567,29 +567,32 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
     }
 }
 
-template <typename F>
-cudaError_t by_shape(uint32_t head_dim, int32_t row_dtype, F&& f) {
-    auto by_dim = [&](auto row) {
-        using T = decltype(row);
-        if (head_dim <= 64) return f(paged_stream_kernel<T, 64, 4>, smem_bytes<64, 4>);
-        if (head_dim <= 128) return f(paged_stream_kernel<T, 128, 3>, smem_bytes<128, 3>);
-        return f(paged_stream_kernel<T, 256, 3>, smem_bytes<256, 3>);
-    };
-    if (row_dtype == ITK_ROW_F32) return by_dim(float());
-    if (row_dtype == ITK_ROW_F16) return by_dim(__half());
-    return by_dim(__nv_bfloat16());
+template <typename T, int D, int STAGES>
+cudaError_t launch_as(const AttnParams& p, uint32_t sms, cudaStream_t s) {
+    auto kernel = paged_stream_kernel<T, D, STAGES>;
+    static OncePerDevice prepared;
+    if (!prepared.done(p.device)) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, STAGES>(kMaxSeqs)));
+        if (e != cudaSuccess) return e;
+        prepared.mark(p.device);
+    }
+    kernel<<<stream_ctas(sms, p.pool.head_dim), kThreads, smem_bytes<D, STAGES>(p.batch.n_seqs), s>>>(p);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_width(const AttnParams& p, uint32_t sms, cudaStream_t s) {
+    if (p.pool.head_dim <= 64) return launch_as<T, 64, 4>(p, sms, s);
+    if (p.pool.head_dim <= 128) return launch_as<T, 128, 3>(p, sms, s);
+    return launch_as<T, 256, 3>(p, sms, s);
 }
 
 }  // namespace
 
 cudaError_t launch_stream(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s) {
-    return by_shape(p.pool.head_dim, row_dtype, [&](auto kernel, auto bytes_of) {
-        const size_t bytes = bytes_of(p.batch.n_seqs);
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes_of(kMaxSeqs)));
-        if (e != cudaSuccess) return e;
-        kernel<<<stream_ctas(sms, p.pool.head_dim), kThreads, bytes, s>>>(p);
-        return cudaGetLastError();
-    });
+    if (row_dtype == ITK_ROW_F32) return launch_width<float>(p, sms, s);
+    if (row_dtype == ITK_ROW_F16) return launch_width<__half>(p, sms, s);
+    return launch_width<__nv_bfloat16>(p, sms, s);
 }
 
 }  // namespace paged

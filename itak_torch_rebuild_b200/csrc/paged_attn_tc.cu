@@ -1013,13 +1013,17 @@ bool make_map(CUtensorMap* map, const Pool& pool, void* data, int32_t dtype) {
 template <typename T, int D>
 cudaError_t launch_as(const AttnParams& p, int32_t page_dtype, uint32_t sms, cudaStream_t s) {
     auto kernel = paged_tc_kernel<T, D>;
-    cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
-    if (e != cudaSuccess) return e;
-    // The warpgroups' shares are drawn from what the block was launched with: fewer, and setmaxnreg would wait for good.
-    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<T, D>::kSmem));
-    if (e != cudaSuccess) return e;
+    static OncePerDevice prepared;
+    if (!prepared.done(p.device)) {
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+        if (e != cudaSuccess) return e;
+        // The warpgroups' shares are drawn from what the block was launched with: fewer, and setmaxnreg would wait for good.
+        if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<T, D>::kSmem));
+        if (e != cudaSuccess) return e;
+        prepared.mark(p.device);
+    }
     CUtensorMap km, vm;
     if (!make_map(&km, p.pool, p.pool.k, page_dtype) || !make_map(&vm, p.pool, p.pool.v, page_dtype)) return cudaErrorInvalidValue;
     kernel<<<sms, kThreads, Shape<T, D>::kSmem, s>>>(p, km, vm);

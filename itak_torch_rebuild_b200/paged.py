@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -27,32 +28,70 @@ _SCALINGS = {"plain": _lib.ROPE_PLAIN, "linear": _lib.ROPE_LINEAR, "base": _lib.
              "ramp": _lib.ROPE_RAMP, "pairs": _lib.ROPE_PAIRS}
 _ERROR_LEN = 256
 
+# A decode step's kernels run for a few microseconds, so the descriptors are packed in one go (filling a ctypes structure
+# takes six times as long); the layouts are those of _lib's structures.
+_PACK_ROPE = struct.Struct("8Q6I2if4x").pack
+_PACK_BATCH = struct.Struct("4Q4I").pack
+_PACK_APPEND = struct.Struct("9Q3Iif4x").pack
+_PACK_ATTENTION = struct.Struct("7Q3Iif4x").pack
+for _s, _f in ((_lib.RopeDesc, "8Q6I2if4x"), (_lib.PagedBatch, "4Q4I"), (_lib.PagedAppendDesc, "9Q3Iif4x"),
+               (_lib.PagedAttentionDesc, "7Q3Iif4x")):
+    assert C.sizeof(_s) == struct.calcsize(_f), _s
 
-def _refuse(msg: str):
-    raise CudaComputeError(_lib.ERR_INVALID_ARGUMENT, msg)
-
-
-def _raise(rc: int, err):
-    raise CudaComputeError(rc, err.value.decode("utf-8", "replace"))
-
-
-def _on(t: torch.Tensor, device: torch.device, what: str, dtype=None):
-    if t.device != device or (dtype is not None and t.dtype is not dtype):
-        _refuse(f"{what} must be {'a tensor' if dtype is None else dtype} on {device}, got {t.dtype} on {t.device}")
-
-
-def _stream(device: torch.device, stream: Optional[int]) -> int:
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+_calls: dict = {}
 
 
-def _heads(t: torch.Tensor, what: str, heads: Optional[int], head_dim: int, rows: Optional[int] = None):
-    """A ``[rows][heads][head_dim]`` tensor whose heads are contiguous; returns its row stride."""
-    if t.dim() != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads) or (rows is not None and t.shape[0] != rows):
-        _refuse(f"{what} has shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}][{heads or 'heads'}][{head_dim}]")
-    st = t.stride()
-    if st[2] != 1 or (t.shape[1] > 1 and st[1] != head_dim):
-        _refuse(f"the heads of {what} must be contiguous, got strides {st}")
-    return st[0]
+def _entry(name: str, descriptors: int):
+    """The library's entry point taking packed descriptors."""
+    fn = _calls.get(name)
+    if fn is None:
+        fn = _lib.load()[name]
+        fn.restype = C.c_int
+        fn.argtypes = [C.c_char_p] * descriptors + [C.c_void_p, C.c_char_p, C.c_size_t]
+        _calls[name] = fn
+    return fn
+
+
+def _refuse(msg: str, code: int = _lib.ERR_INVALID_ARGUMENT):
+    raise CudaComputeError(code, msg)
+
+
+def _explain(fn, *args):
+    """A refused call has done nothing: it is made again with a buffer for its reason."""
+    err = C.create_string_buffer(_ERROR_LEN)
+    rc = fn(*args, err, _ERROR_LEN)
+    if rc != _lib.OK:
+        raise CudaComputeError(rc, err.value.decode("utf-8", "replace"))
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _u32(**values):
+    for name, v in values.items():
+        if not 0 <= v <= 0xffffffff:
+            _refuse(f"{name} must be in 0..2^32 - 1, got {v}")
+
+
+def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
+    """The row stride of a ``[rows][heads][head_dim]`` tensor whose heads are contiguous."""
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse(f"{what} must be {dtype} on device {device}, got {t.dtype} on {t.device}")
+    if t.shape != (rows, heads, head_dim):
+        _refuse(f"{what} has shape {tuple(t.shape)}, expected {(rows, heads, head_dim)}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != head_dim and heads > 1):
+        _refuse(f"the heads of {what} must be contiguous, got strides {(s0, s1, s2)}")
+    return s0
+
+
+def _vector(t: torch.Tensor, what: str, dtype, n: Optional[int], device: int) -> int:
+    """The address of a contiguous vector of ``n`` elements (any number: ``None``)."""
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse(f"{what} must be {dtype} on device {device}, got {t.dtype} on {t.device}")
+    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous vector{'' if n is None else f' of {n} elements'}, got {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def rope_table(rotary_dim: int, base: float, *, scaling: str = "plain", factor: float = 1.0, original_context: float = 0.0,
@@ -75,7 +114,7 @@ def rope_table(rotary_dim: int, base: float, *, scaling: str = "plain", factor: 
     mag, err = C.c_float(), C.create_string_buffer(_ERROR_LEN)
     rc = _lib.load().itk_rope_table(C.byref(cfg), out.ctypes.data, C.byref(mag), err, _ERROR_LEN)
     if rc != _lib.OK:
-        _raise(rc, err)
+        _refuse(err.value.decode("utf-8", "replace"), rc)
     return out, mag.value
 
 
@@ -85,32 +124,28 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     ``positions[r]`` (int32).  ``pairing`` 0 joins channels (2i, 2i + 1), 1 joins (i, i + rotary_dim / 2), with
     ``rotary_dim = 2 * len(inv_freq)``; ``inverse=True`` maps the gradient of the result to the gradient of ``x``.
     ``out`` may be ``x``."""
-    dev = x.device
-    if dev.type != "cuda" or x.dtype not in _ROW_DTYPES or x.dim() != 3:
-        _refuse(f"x must be an f32, f16 or bf16 [rows][heads][head_dim] tensor on a CUDA device, got {x.dtype} {tuple(x.shape)} on {dev}")
-    rows, heads, head_dim = x.shape
+    dtype, dev = _ROW_DTYPES.get(x.dtype), x.get_device()
+    if dtype is None or dev < 0 or x.dim() != 3:
+        _refuse(f"x must be an f32, f16 or bf16 [rows][heads][head_dim] tensor on a CUDA device, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    shape = x.shape
     if out is None:
-        out = torch.empty((rows, heads, head_dim), dtype=x.dtype, device=dev)
-    else:
-        _on(out, dev, "out", x.dtype)
-        if out.shape != x.shape:
-            _refuse(f"out has shape {tuple(out.shape)}, expected {tuple(x.shape)}")
-    _on(positions, dev, "positions", torch.int32)
-    _on(inv_freq, dev, "inv_freq", torch.float64)
-    if positions.shape != (rows,) or not positions.is_contiguous():
-        _refuse(f"positions must be a contiguous [{rows}] tensor, got {tuple(positions.shape)}")
-    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        _refuse("inv_freq must be a contiguous vector")
-    xs, os = x.stride(), out.stride()
-    if (xs[2] != 1 or os[2] != 1) and head_dim > 1:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.dtype is not x.dtype or out.get_device() != dev or out.shape != shape:
+        _refuse(f"out must be {x.dtype} {tuple(shape)} on {x.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    rows, heads, head_dim = shape
+    at = _vector(positions, "positions", torch.int32, rows, dev)
+    table = _vector(inv_freq, "inv_freq", torch.float64, None, dev)
+    x0, x1, x2 = x.stride()
+    o0, o1, o2 = out.stride()
+    if x2 != 1 or o2 != 1:
         _refuse("the channels of x and out must be contiguous")
-    d = _lib.RopeDesc(x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), xs[0], xs[1], os[0], os[1],
-                      rows, heads, head_dim, 2 * inv_freq.shape[0], pairing, 1 if inverse else 0, _ROW_DTYPES[x.dtype],
-                      dev.index, magnitude)
-    err = C.create_string_buffer(_ERROR_LEN)
-    rc = _lib.load().itk_rope_apply(C.byref(d), _stream(dev, stream), err, _ERROR_LEN)
-    if rc != _lib.OK:
-        _raise(rc, err)
+    _u32(pairing=pairing)
+    d = _PACK_ROPE(x.data_ptr(), out.data_ptr(), at, table, x0, x1, o0, o1, rows, heads, head_dim, 2 * inv_freq.shape[0], pairing,
+                   1 if inverse else 0, dtype, dev, magnitude)
+    fn = _entry("itk_rope_apply", 1)
+    stream = _raw_stream(dev) if stream is None else stream
+    if fn(d, stream, None, 0) != _lib.OK:
+        _explain(fn, d, stream)
     return out
 
 
@@ -142,32 +177,33 @@ class PagedKv:
             _refuse(f"the pools must be two 4-dimensional tensors of one shape and one set of strides, got {tuple(k.shape)} and {tuple(v.shape)}")
         if k.device.type != "cuda" or k.dtype not in (torch.float16, torch.bfloat16):
             _refuse(f"the pools must be f16 or bf16 tensors on a CUDA device, got {k.dtype} on {k.device}")
-        _on(v, k.device, "v", k.dtype)
+        if v.device != k.device or v.dtype is not k.dtype:
+            _refuse(f"the pools must be of one type on one device, got {k.dtype} on {k.device} and {v.dtype} on {v.device}")
         st = k.stride()
         if st[3] != 1:
             _refuse("the channels of a page must be contiguous")
         self.k, self.v, self.layout, self.device, self.dtype = k, v, layout, k.device, k.dtype
         heads_at, rows_at = (1, 2) if layout == "head" else (2, 1)
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = k.shape[0], k.shape[heads_at], k.shape[rows_at], k.shape[3]
-        self._lib = _lib.load()
-        self._kv = _lib.PagedKv(k.data_ptr(), v.data_ptr(), st[0], st[heads_at], st[rows_at], self.n_pages, self.page_size,
-                                self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], k.device.index)
+        self._index = k.get_device()
+        self._scale = 1.0 / math.sqrt(max(self.head_dim, 1))
+        self._kv = bytes(_lib.PagedKv(k.data_ptr(), v.data_ptr(), st[0], st[heads_at], st[rows_at], self.n_pages, self.page_size,
+                                      self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], self._index))
 
-    def _batch(self, table, row_start, kv_len, total_rows, status):
-        dev = self.device
-        n = kv_len.shape[0]
-        for t, what in ((table, "table"), (row_start, "row_start"), (kv_len, "kv_len")):
-            _on(t, dev, what, torch.int32)
+    def _batch(self, table, row_start, kv_len, total_rows, status) -> bytes:
+        dev, n = self._index, kv_len.shape[0]
+        lens = _vector(kv_len, "kv_len", torch.int32, None, dev)
+        starts = _vector(row_start, "row_start", torch.int32, n + 1, dev)
+        if table.dtype is not torch.int32 or table.get_device() != dev:
+            _refuse(f"table must be {torch.int32} on device {dev}, got {table.dtype} on {table.device}")
         if table.dim() != 2 or table.shape[0] != n or (table.stride(1) != 1 and table.shape[1] > 1):
             _refuse(f"table must be [{n}][pages of a sequence] with contiguous rows, got {tuple(table.shape)}")
-        if row_start.shape != (n + 1,) or kv_len.dim() != 1 or not row_start.is_contiguous() or not kv_len.is_contiguous():
-            _refuse(f"row_start must be a contiguous [{n + 1}] and kv_len a contiguous [{n}] tensor, got {tuple(row_start.shape)} and {tuple(kv_len.shape)}")
+        word = 0
         if status is not None:
-            _on(status, dev, "status", torch.int32)
+            word = _vector(status, "status", torch.int32, None, dev)
             if status.numel() < 1:
                 _refuse("status must hold one element")
-        return _lib.PagedBatch(table.data_ptr(), row_start.data_ptr(), kv_len.data_ptr(),
-                               None if status is None else status.data_ptr(), n, table.shape[1], table.stride(0), total_rows)
+        return _PACK_BATCH(table.data_ptr(), starts, lens, word, n, table.shape[1], table.stride(0), total_rows)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *,
                q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
@@ -175,38 +211,38 @@ class PagedKv:
         """Stores the new rows ``k``, ``v`` ``[rows][kv_heads][head_dim]`` into their pages, K rotated by ``inv_freq``
         (``None``: stored as it is), and returns ``q`` rotated alike (in ``q_out``, which may be ``q``) when ``q`` is
         given.  f32 rows go into f16 pages, 16-bit rows into pages of their type (``itk_paged_append``)."""
-        dev, d = self.device, self.head_dim
+        dev, d, dtype = self._index, self.head_dim, k.dtype
+        row_dtype = _ROW_DTYPES.get(dtype)
+        if row_dtype is None:
+            _refuse(f"rows must be f32, f16 or bf16, got {dtype}")
         rows = k.shape[0]
-        k_row = _heads(k, "k", self.kv_heads, d)
-        v_row = _heads(v, "v", self.kv_heads, d, rows)
-        _on(k, dev, "k")
-        if k.dtype not in _ROW_DTYPES:
-            _refuse(f"rows must be f32, f16 or bf16, got {k.dtype}")
-        _on(v, dev, "v", k.dtype)
-        q_row = q_out_row = q_heads = 0
+        k_row = _rows(k, "k", rows, self.kv_heads, d, dtype, dev)
+        v_row = _rows(v, "v", rows, self.kv_heads, d, dtype, dev)
+        q_row = q_out_row = q_heads = q_at = q_out_at = 0
         if q is not None:
-            _on(q, dev, "q", k.dtype)
-            q_row, q_heads = _heads(q, "q", None, d, rows), q.shape[1]
+            if q.dim() != 3:
+                _refuse(f"q has shape {tuple(q.shape)}, expected [{rows}][heads][{d}]")
+            q_heads = q.shape[1]
+            q_row = _rows(q, "q", rows, q_heads, d, dtype, dev)
             if q_out is None:
-                q_out = torch.empty((rows, q_heads, d), dtype=q.dtype, device=dev)
-            _on(q_out, dev, "q_out", k.dtype)
-            q_out_row = _heads(q_out, "q_out", q_heads, d, rows)
+                q_out = torch.empty((rows, q_heads, d), dtype=dtype, device=self.device)
+            q_out_row = _rows(q_out, "q_out", rows, q_heads, d, dtype, dev)
+            q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             _refuse("q, q_out and q_heads go together")
+        freq = rotary = 0
         if inv_freq is not None:
-            _on(inv_freq, dev, "inv_freq", torch.float64)
-            if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-                _refuse("inv_freq must be a contiguous vector")
+            freq, rotary = _vector(inv_freq, "inv_freq", torch.float64, None, dev), 2 * inv_freq.shape[0]
+        _u32(pairing=pairing)
         batch = self._batch(table, row_start, kv_len, rows, status)
-        a = _lib.PagedAppendDesc(None if q is None else q.data_ptr(), None if q is None else q_out.data_ptr(), k.data_ptr(),
-                                 v.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), q_row, q_out_row, k_row, v_row,
-                                 q_heads, 0 if inv_freq is None else 2 * inv_freq.shape[0], pairing, _ROW_DTYPES[k.dtype], magnitude)
         if rows == 0:  # torch gives empty tensors no address
             return q_out
-        err = C.create_string_buffer(_ERROR_LEN)
-        rc = self._lib.itk_paged_append(C.byref(self._kv), C.byref(batch), C.byref(a), _stream(dev, stream), err, _ERROR_LEN)
-        if rc != _lib.OK:
-            _raise(rc, err)
+        a = _PACK_APPEND(q_at, q_out_at, k.data_ptr(), v.data_ptr(), freq, q_row, q_out_row, k_row, v_row, q_heads, rotary, pairing,
+                         row_dtype, magnitude)
+        fn = _entry("itk_paged_append", 3)
+        stream = _raw_stream(dev) if stream is None else stream
+        if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
+            _explain(fn, self._kv, batch, a, stream)
         return q_out
 
     def attention(self, q: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *, max_rows: int,
@@ -218,42 +254,36 @@ class PagedKv:
         and only chooses between kernels; ``scale`` is ``1 / sqrt(head_dim)`` unless given; ``lse`` ``[rows][q_heads]``
         f32 receives the log-sum-exp.  Without ``workspace`` calls of one stream share one of this module's; a call
         that is being captured must be given its own (``attention_workspace``)."""
-        dev, d = self.device, self.head_dim
-        rows, q_heads = q.shape[0], q.shape[1]
-        q_row = _heads(q, "q", None, d)
-        _on(q, dev, "q")
-        if q.dtype not in _ROW_DTYPES:
-            _refuse(f"rows must be f32, f16 or bf16, got {q.dtype}")
+        dev, d, dtype = self._index, self.head_dim, q.dtype
+        row_dtype = _ROW_DTYPES.get(dtype)
+        if row_dtype is None or q.dim() != 3:
+            _refuse(f"rows must be f32, f16 or bf16 [rows][heads][{d}], got {dtype} {tuple(q.shape)}")
+        rows, q_heads, _ = q.shape
+        q_row = _rows(q, "q", rows, q_heads, d, dtype, dev)
         if out is None:
-            out = torch.empty((rows, q_heads, d), dtype=q.dtype, device=dev)
-        else:
-            _on(out, dev, "out", q.dtype)
-        out_row = _heads(out, "out", q_heads, d, rows)
+            out = torch.empty((rows, q_heads, d), dtype=dtype, device=self.device)
+        out_row = _rows(out, "out", rows, q_heads, d, dtype, dev)
+        lse_at = 0
         if lse is not None:
-            _on(lse, dev, "lse", torch.float32)
-            if lse.shape != (rows, q_heads) or not lse.is_contiguous():
-                _refuse(f"lse must be a contiguous [{rows}][{q_heads}] tensor, got {tuple(lse.shape)}")
-        if not 0 <= window <= 0xffffffff or not 0 <= max_rows <= 0xffffffff:
-            _refuse(f"window {window} and max_rows {max_rows} must not be negative")
-        raw = _stream(dev, stream)
+            if lse.dtype is not torch.float32 or lse.get_device() != dev or lse.shape != (rows, q_heads) or not lse.is_contiguous():
+                _refuse(f"lse must be a contiguous {torch.float32} [{rows}][{q_heads}] tensor on device {dev}, got {lse.dtype} {tuple(lse.shape)} on {lse.device}")
+            lse_at = lse.data_ptr()
+        _u32(window=window, max_rows=max_rows)
+        stream = _raw_stream(dev) if stream is None else stream
         if workspace is None:
-            workspace = _workspaces.get((dev.index, raw))
             if torch.cuda.is_current_stream_capturing():
                 _refuse("a call that is being captured needs a workspace of its own (attention_workspace)")
+            workspace = _workspaces.get((dev, stream))
             if workspace is None:
-                workspace = _workspaces[(dev.index, raw)] = attention_workspace(dev)
-        else:
-            _on(workspace, dev, "workspace", torch.uint8)
-            if not workspace.is_contiguous():
-                _refuse("the workspace must be contiguous")
+                workspace = _workspaces[(dev, stream)] = attention_workspace(self.device)
+        elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+            _refuse(f"the workspace must be a contiguous {torch.uint8} tensor on device {dev}, got {workspace.dtype} on {workspace.device}")
         batch = self._batch(table, row_start, kv_len, rows, status)
         if rows == 0:  # torch gives empty tensors no address
             return out
-        a = _lib.PagedAttentionDesc(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                                    workspace.numel(), q_row, out_row, q_heads, max_rows, window, _ROW_DTYPES[q.dtype],
-                                    1.0 / math.sqrt(d) if scale is None else scale)
-        err = C.create_string_buffer(_ERROR_LEN)
-        rc = self._lib.itk_paged_attention(C.byref(self._kv), C.byref(batch), C.byref(a), raw, err, _ERROR_LEN)
-        if rc != _lib.OK:
-            _raise(rc, err)
+        a = _PACK_ATTENTION(q.data_ptr(), out.data_ptr(), lse_at, workspace.data_ptr(), workspace.numel(), q_row, out_row, q_heads,
+                            max_rows, window, row_dtype, self._scale if scale is None else scale)
+        fn = _entry("itk_paged_attention", 3)
+        if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
+            _explain(fn, self._kv, batch, a, stream)
         return out
