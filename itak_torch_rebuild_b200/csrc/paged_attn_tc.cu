@@ -55,8 +55,9 @@ constexpr uint32_t kTile = 128;       // keys of a tile, and rows of a stream
 constexpr uint32_t kBlockPairs = 256;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
 constexpr float kRescaleStep = 8.f;
-constexpr uint32_t kInfoSeqs = 32;  // sequences of a run kept in shared memory
-constexpr uint32_t kTailBytes = 1280;  // mbarriers, the run's beginning, the roles' items
+constexpr uint32_t kFlush = 2;            // f32 rows: tiles that add up in tensor memory
+constexpr uint32_t kSmemBytes = 232448;   // all that a block can have
+constexpr uint32_t kTailBytes = 3072;     // mbarriers, the roles' items, the streams' exchange
 constexpr long long kWaitClocks = 2000000000ll;  // about a second
 
 template <typename T>
@@ -83,11 +84,10 @@ struct Shape {
     static constexpr uint32_t kPanel = kTile * 128;              // bytes of [128 rows][64 channels]
     static constexpr uint32_t kStage = (D / 64) * kPanel;        // a K or V tile
     static constexpr uint32_t kQ = (kSplit ? 2 : 1) * kStage;    // a stream's queries: (high) panels, then low ones
-    static constexpr uint32_t kStages = (232448u - 1024u - kTailBytes - 2 * kQ) / kStage;
-    static constexpr uint32_t kSmem = 2 * kQ + kStages * kStage + kTailBytes + 1024;
+    static constexpr uint32_t kStages = (kSmemBytes - kTailBytes - 2 * kQ) / kStage;
+    static constexpr uint32_t kSmem = 2 * kQ + kStages * kStage + kTailBytes;
     static_assert(kStages >= 3, "K(t), V(t) and K(t + 1)");
-    static_assert(kStages * kStage >= (2 * kMaxSeqs + 1) * 8, "the ring is the planning's scratch");
-    static_assert(kQ >= 2 * kTile * 8, "stream 1's query tile is the streams' exchange");
+    static_assert(kStages * kStage >= (2 * kMaxSeqs + 1) * 8 + kMaxSeqs * 12, "the ring is the planning's scratch");
 };
 
 struct SeqInfo {
@@ -181,19 +181,13 @@ struct Item {
 };
 struct Run {
     const AttnParams& p;
-    const SeqInfo* info;  // of its first kInfoSeqs sequences
-    uint32_t s_first;
     uint64_t end;
 
     __device__ __forceinline__ void open_seq(Item& it) const {
-        if (it.s - s_first < kInfoSeqs) {
-            it.q = info[it.s - s_first];
-        } else {
-            Batch b = p.batch;
-            b.status = nullptr;
-            const Seq q = seq_of(b, it.s, p.pool.page_shift);
-            it.q = SeqInfo{q.row0, q.rows, q.len};
-        }
+        Batch b = p.batch;
+        b.status = nullptr;
+        const Seq q = seq_of(b, it.s, p.pool.page_shift);
+        it.q = SeqInfo{q.row0, q.rows, q.len};
         it.blocks = (it.q.rows * p.group + kBlockPairs - 1) / kBlockPairs;
     }
     __device__ __forceinline__ void open_cell(Item& it, uint32_t off) const {
@@ -250,27 +244,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     constexpr bool SPLIT = Sh::kSplit;
     constexpr uint32_t NST = Sh::kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* const smem =
-        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* const smem = smem_raw;
+    if ((smem_u32(smem) & 1023u) != 0) {  // (the tiles' swizzle goes by address bits; never so far)
+        if (threadIdx.x == 0) raise(p.batch, kWaitRanOut);
+        return;
+    }
     const uint32_t qbuf = smem_u32(smem), ring = qbuf + 2 * Sh::kQ, tail = ring + NST * Sh::kStage;
     unsigned char* const tail_ptr = smem + 2 * Sh::kQ + NST * Sh::kStage;
     // mbarriers
     const uint32_t bar_full = tail;                // [stage] the tile has landed
-    const uint32_t bar_empty = bar_full + 8 * 16;  // [stage] every product that reads it is complete
-    const uint32_t bar_s = bar_empty + 8 * 16;     // [stream] scores complete
-    const uint32_t bar_p = bar_s + 16;             // [stream][half] the weights of half of the tile's keys are stored
-    const uint32_t bar_o = bar_p + 32;             // [stream] the cell's last product complete
-    const uint32_t bar_q = bar_o + 16;             // [stream] the cell's queries are in shared memory
-    const uint32_t bar_land = bar_q + 16;          // a V tile that needs zero rows has landed
-    const uint32_t bar_done = bar_land + 8;        // everything issued to the tensor core is complete
-    const uint32_t bar_turn = bar_done + 8;        // [stream] its products of a round are issued
-    static_assert(NST <= 16, "stages");
-    uint32_t* const word = reinterpret_cast<uint32_t*>(tail_ptr + 400);  // [0] tensor memory, [1] joined flag, [2] abort
+    const uint32_t bar_empty = bar_full + 8 * NST;  // [stage] every product that reads it is complete
+    const uint32_t bar_s = bar_empty + 8 * NST;     // [stream] scores complete
+    const uint32_t bar_p = bar_s + 16;              // [stream][half] the weights of half of the tile's keys are stored
+    const uint32_t bar_o = bar_p + 32;              // [stream] the cell's last product complete
+    const uint32_t bar_q = bar_o + 16;              // [stream] the cell's queries are in shared memory
+    const uint32_t bar_land = bar_q + 16;           // a V tile that needs zero rows has landed
+    const uint32_t bar_done = bar_land + 8;         // everything issued to the tensor core is complete
+    constexpr uint32_t kWordAt = 16 * NST + 96, kItemsAt = kWordAt + 24, kItems = 7;
+    static_assert(kItemsAt + kItems * sizeof(Item) + 256 * sizeof(float2) <= kTailBytes, "tail");
+    uint32_t* const word = reinterpret_cast<uint32_t*>(tail_ptr + kWordAt);  // [0] tensor memory, [1] joined flag
     volatile uint32_t* const abort_flag = word + 2;
-    uint32_t* const plan = reinterpret_cast<uint32_t*>(tail_ptr + 424);  // where the run begins: sequence, KV head, block, tile
-    SeqInfo* const info = reinterpret_cast<SeqInfo*>(tail_ptr + 448);
-    Item* const items = reinterpret_cast<Item*>(tail_ptr + 448 + kInfoSeqs * sizeof(SeqInfo));  // softmax, products of stream 0 and 1, loads
-    static_assert(kInfoSeqs * sizeof(SeqInfo) % 8 == 0 && 448 + kInfoSeqs * sizeof(SeqInfo) + 4 * sizeof(Item) <= kTailBytes, "tail");
+    volatile uint32_t* const issued = word + 4;  // [stream] rounds of products issued so far
+    // softmax's cells (streams 0 and 1), the cells after them, the products' (streams 0 and 1), the loads'
+    Item* const items = reinterpret_cast<Item*>(tail_ptr + kItemsAt);
+    float2* const exchange = reinterpret_cast<float2*>(items + kItems);  // [stream][row] (maximum, sum)
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n_seqs = p.batch.n_seqs, group = p.group, window = p.window, cta = blockIdx.x;
@@ -287,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             tc::mbar_init(bar_p + 16 * i + 8, 128);
             tc::mbar_init(bar_o + 8 * i, 1);
             tc::mbar_init(bar_q + 8 * i, 128);
-            tc::mbar_init(bar_turn + 8 * i, 1);
+            issued[i] = 0;
         }
         tc::mbar_init(bar_land, 1);
         tc::mbar_init(bar_done, 2);
@@ -300,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     }
     uint64_t* const prefix = reinterpret_cast<uint64_t*>(smem + 2 * Sh::kQ);  // [n_seqs + 1], scratch in the ring
     uint64_t* const per_head = prefix + n_seqs + 1;  // [n_seqs] tiles of one KV head
+    SeqInfo* const info = reinterpret_cast<SeqInfo*>(per_head + n_seqs);
     constexpr uint64_t kLater = ~0ull;
     constexpr uint32_t kOwnBlocks = 8;  // a sequence of more blocks is summed by a whole warp
     for (uint32_t s = tid; s < n_seqs; s += kThreads) {
@@ -307,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         if (cta != 0) b.status = nullptr;  // one CTA reports
         const Seq sq = seq_of(b, s, p.pool.page_shift);
         const SeqInfo q{sq.row0, sq.rows, sq.len};
+        info[s] = q;
         const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
         uint64_t sum = kLater;
         if (blocks <= kOwnBlocks) {
@@ -318,10 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     __syncthreads();
     for (uint32_t s = warp; s < n_seqs; s += kThreads / 32) {
         if (per_head[s] != kLater) continue;
-        Batch b = p.batch;
-        b.status = nullptr;
-        const Seq sq = seq_of(b, s, p.pool.page_shift);
-        const SeqInfo q{sq.row0, sq.rows, sq.len};
+        const SeqInfo q = info[s];
         const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
         uint64_t sum = 0;
         for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window);
@@ -352,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint64_t per = max((W + gridDim.x - 1) / gridDim.x, static_cast<uint64_t>(1));
     const uint64_t run0 = cta * per, run1 = min(W, run0 + per);
     const bool works = run0 < run1;
+    const Run run{p, run1};
     if (works && warp == 0) {  // where the run begins
         uint32_t lo = 0, hi = n_seqs;
         while (hi - lo > 1) {
@@ -361,10 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             else
                 hi = mid;
         }
-        Batch b = p.batch;
-        b.status = nullptr;
-        const Seq sq = seq_of(b, lo, p.pool.page_shift);
-        const SeqInfo q{sq.row0, sq.rows, sq.len};
+        const SeqInfo q = info[lo];
         const uint64_t in = run0 - prefix[lo];
         const uint32_t kvh = static_cast<uint32_t>(in / per_head[lo]);
         uint64_t left = in % per_head[lo];
@@ -387,33 +381,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             }
             left -= __shfl_sync(0xffffffffu, incl, 31);
         }
+        Item& first = items[0];
         if (lane == 0) {
-            plan[0] = lo;
-            plan[1] = kvh;
-            plan[2] = block;
-            plan[3] = static_cast<uint32_t>(left);
+            first.s = lo;
+            first.kvh = kvh;
+            first.block = block;
+            first.blocks = blocks;
+            first.pos = run0;
+            first.q = q;
+            run.open_cell(first, static_cast<uint32_t>(left));
         }
-        if (lane < kInfoSeqs && lo + lane < n_seqs) {
-            const Seq x = seq_of(b, lo + lane, p.pool.page_shift);
-            info[lane] = SeqInfo{x.row0, x.rows, x.len};
-        }
+        __syncwarp();
+        if (lane > 0 && lane < kItems) items[lane] = first;
     }
     tc::fence_proxy_async();  // the ring was the planning's scratch, TMA writes it next
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = word[0];
-    const Run run{p, info, plan[0], run1};
-    if (works && tid % 64 == 0 && tid < 256) {
-        Item& first = items[tid / 64];
-        first.s = plan[0];
-        first.kvh = plan[1];
-        first.block = plan[2];
-        first.pos = run0;
-        run.open_seq(first);
-        run.open_cell(first, plan[3]);
-    }
-    __syncthreads();
     // Waits that ran out end the call: every role leaves (or, the softmax threads, walks on through their barriers without
     // waiting), once what the role has in flight has come to rest.
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -440,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const uint32_t row_at = slot << box_shift;           // its first row in the tile
             uint32_t cnt = 0, landed = 0;
             bool ok = true;
-            Item& it = items[3];
+            Item& it = items[6];
             do {
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
                 for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
@@ -513,9 +498,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             constexpr uint64_t kDescK = tc::smem_desc_base(16, 1024), kDescV = tc::smem_desc_base(Sh::kPanel, 1024);
             const uint32_t tS = tmem + i * kTile, tO = tmem + kTmemO + i * D;
             uint32_t base = 0;  // the ring's count at the item's first tile
-            uint32_t n_p = 0, n_items = 0, turns = 0;  // turns: the other stream's rounds of the cells before
+            uint32_t n_p = 0, n_items = 0, mine = 0, turns = 0;  // turns: the other stream's rounds of the cells before
+            auto wait_round = [&](uint32_t n) -> bool {  // until the other stream has issued its round n
+                if (static_cast<int32_t>(issued[1 - i] - n) > 0) return true;
+                const long long t0 = clock64();
+                while (static_cast<int32_t>(issued[1 - i] - n) <= 0) {
+                    if (*abort_flag != 0) return false;
+                    if (clock64() - t0 > kWaitClocks) {
+                        *abort_flag = 1;
+                        raise(p.batch, kWaitRanOut);
+                        return false;
+                    }
+                }
+                return true;
+            };
             bool ok = true;
-            Item& it = items[1 + i];
+            Item& it = items[4 + i];
             do {
                 const uint32_t t0 = it.t0, step = it.step, twin = it.twin, a = it.a[i], e = it.e[i];
                 const uint32_t oa = twin != 0 ? e : it.a[1 - i], oe = twin != 0 ? 0u : it.e[1 - i];  // tiles the other stream reads too
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const uint64_t k = kDescK + ((ring + cn % NST * Sh::kStage) >> 4);
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks) {
-                        if (ks == D / 32) mbar_arrive(bar_turn + 8 * i);  // the other thread takes a while to see it
+                        if (ks == D / 32) issued[i] = ++mine;  // the other thread takes a while to see it
                         constexpr uint32_t kPanel16 = Sh::kPanel / 16;
                         const uint32_t off = (ks / 4) * kPanel16 + (ks % 4) * 2;
                         tc::mma_f16_ss(tS, q + off, k + off, kIdS, ks > 0 ? 1u : 0u);
@@ -540,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const uint32_t xa = it.a[1 - i], xe = it.e[1 - i];
                 const uint32_t rounds = xa < xe ? (xe - xa + step - 1) / step + 1 : 0u;  // of the other stream: 0, 1, ...
                 // One copy of the code: the first round has no weights to use yet, the last no scores to make.
+                uint32_t n_in = 0;  // tiles of the cell used
                 uint32_t after = i == 0 ? 0xffffffffu : 0u;  // the other stream's round that this one follows (stream 0 begins)
                 for (uint32_t nt = a; ok && a < e; nt += step, ++after) {
                     const bool have = nt != a, more = nt < e;  // weights of tile t; scores of tile nt to come
@@ -550,11 +549,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (have) ok = full(cv);
                     if (ok && more && (kAhead || twin == 0 || !have)) ok = full(ck);
                     if (ok && have) ok = wait(bar_p + 16 * i, n_p & 1u);
-                    if (ok && after < rounds) ok = wait(bar_turn + 8 * (1 - i), (turns + after) & 1u);
+                    if (ok && after < rounds) ok = wait_round(turns + after);
                     if (ok && have) {  // O (+)= P V(t)
                         tc::fence_after_sync();
                         const uint64_t v = kDescV + ((ring + cv % NST * Sh::kStage) >> 4);
-                        const uint32_t acc = t != a ? 1u : 0u;
+                        // (f32 rows: the softmax takes the output out after every kFlush tiles)
+                        const uint32_t acc = SPLIT ? (n_in++ % kFlush != 0 ? 1u : 0u) : (t != a ? 1u : 0u);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             if (j == 4) {
@@ -562,8 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                                 if (!ok) break;
                                 tc::fence_after_sync();
                             }
-                            if constexpr (SPLIT) {  // (every tile's output is taken out: see the softmax)
-                                tc::mma_f16_ts(tO, tS + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : 0u);
+                            if constexpr (SPLIT) {
+                                tc::mma_f16_ts(tO, tS + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : acc);
                                 tc::mma_f16_ts(tO, tS + 16 * j + 8, v + j * 128, kIdO, 1u);
                             } else {
                                 tc::mma_f16_ts(tO, tS + 8 * j, v + j * 128, kIdO, j > 0 ? 1u : acc);
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         tc::mma_commit(bar_s + 8 * i);
                         release(ck, nt);
                     } else {
-                        mbar_arrive(bar_turn + 8 * i);
+                        issued[i] = ++mine;
                         tc::mma_commit(bar_o + 8 * i);
                     }
                     if (have && (kAhead || twin == 0)) release(cv, t);
@@ -603,65 +603,88 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const uint32_t i = warp >> 2, r = tid & 127;
         const uint32_t lane_base = ((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + i * kTile, tO = tmem + lane_base + kTmemO + i * D;
+        const uint32_t tOther = tmem + lane_base + kTmemO + (1 - i) * D;
         const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);  // the queries carry a negative scale's sign
         const bool flip = p.scale_log2 < 0.f;
         const uint32_t head_dim = p.pool.head_dim;
         uint32_t n_s = 0, n_o = 0;  // scores seen, last products seen
         bool dead = !works;         // a wait ran out: walk on through the barriers, touch nothing
-        Item& it = items[0];
-        if (works) do {
-            // ---- the block's queries into shared memory: warp by warp, 16 bytes a lane
-            if (i == 0 || !it.twin) {
-                constexpr uint32_t CH = D / 8, RP = 32 / CH, PASSES = 32 / RP;
-                const uint32_t chunk = lane % CH;
-                unsigned char* const qs = smem + i * Sh::kQ + (chunk / 8) * Sh::kPanel;
-                auto row_of = [&](uint32_t pass) { return (warp & 3) * 32 + pass * RP + lane / CH; };
-                auto source = [&](uint32_t qr) -> const T* {
-                    const uint32_t in = i * kTile + qr;
-                    if (in >= it.pairs || chunk * 8 >= head_dim) return nullptr;
-                    const uint32_t pair = it.block * kBlockPairs + in;
-                    return static_cast<const T*>(p.q) + static_cast<uint64_t>(it.q.row0 + pair / group) * p.q_row +
-                           (it.kvh * group + pair % group) * head_dim + chunk * 8;
-                };
-                constexpr uint32_t BATCH = SPLIT ? 4 : 8;
-#pragma unroll 1
-                for (uint32_t p0 = 0; p0 < PASSES; p0 += BATCH) {
-                    Vec8<T> x[BATCH];
+        Item &it = items[i], &nx = items[2 + i];  // the warpgroup's cell and the one after it
+        auto group_sync = [&]() {
+            if (i == 0)
+                asm volatile("bar.sync 2, 128;\n" ::: "memory");
+            else
+                asm volatile("bar.sync 3, 128;\n" ::: "memory");
+        };
+        // A row of Q, and of the output on its way out, lies in the stream's query tile: 16-byte chunk k of row x here.
+        unsigned char* const qs = smem + i * Sh::kQ;
+        auto chunk_at = [&](uint32_t x, uint32_t k) { return qs + (k / 8) * Sh::kPanel + x * 128 + (((k % 8) ^ (x & 7)) << 4); };
+        // A block's queries, a batch of passes at a time.  16-bit rows are requested before the cell ahead of them ends, all
+        // passes at once, and stored behind it; f32 rows would take 128 registers and go batch by batch at its end.
+        constexpr uint32_t CH = D / 8, RP = 32 / CH;  // lanes of a row, rows of a pass; CH passes for a warp's 32 rows
+        constexpr uint32_t QB = SPLIT ? CH / 4 : CH;
+        struct Queries {
+            Vec8<T> v[QB];
+        };
+        auto query_row = [&](const Item& n) -> int64_t {  // where row r's query lies, or -1
+            const uint32_t in = i * kTile + r, pair = n.block * kBlockPairs + in;
+            if (in >= n.pairs || (i == 1 && n.twin)) return -1;  // (a twin cell's streams both read stream 0's)
+            return static_cast<int64_t>((n.q.row0 + pair / group) * p.q_row + (n.kvh * group + pair % group) * head_dim);
+        };
+        auto request_queries = [&](int64_t mine, uint32_t j0, Queries& xq) {
+            const uint32_t ch = (lane % CH) * 8;
 #pragma unroll
-                    for (uint32_t j = 0; j < BATCH; ++j) {
-                        const T* src = source(row_of(p0 + j));
-                        x[j] = Vec8<T>{};
-                        if (src) x[j].load(src);
-                    }
-#pragma unroll
-                    for (uint32_t j = 0; j < BATCH; ++j) {
-                        const uint32_t qr = row_of(p0 + j);
-                        unsigned char* dst = qs + qr * 128 + (((chunk % 8) ^ (qr & 7)) << 4);
-                        if constexpr (SPLIT) {
-                            float f[8];
-                            x[j].get(f);
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                __half h0, l0, h1, l1;
-                                split_half(flip ? -f[2 * e] : f[2 * e], h0, l0);
-                                split_half(flip ? -f[2 * e + 1] : f[2 * e + 1], h1, l1);
-                                hi[e] = pack_half2(h0, h1);
-                                lo[e] = pack_half2(l0, l1);
-                            }
-                            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4*>(dst + Sh::kStage) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        } else {
-                            uint4 v = x[j].w;
-                            if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-                            *reinterpret_cast<uint4*>(dst) = v;
-                        }
-                    }
-                }
-                tc::fence_proxy_async();
+            for (uint32_t j = 0; j < QB; ++j) {
+                const int64_t off = __shfl_sync(0xffffffffu, mine, (j0 + j) * RP + lane / CH);
+                xq.v[j] = Vec8<T>{};
+                if (off >= 0 && ch < head_dim) xq.v[j].load(static_cast<const T*>(p.q) + off + ch);
             }
+        };
+        auto store_queries = [&](uint32_t j0, const Queries& xq) {
+#pragma unroll
+            for (uint32_t j = 0; j < QB; ++j) {
+                unsigned char* const dst = chunk_at((warp & 3) * 32 + (j0 + j) * RP + lane / CH, lane % CH);
+                if constexpr (SPLIT) {
+                    float f[8];
+                    xq.v[j].get(f);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        __half h0, l0, h1, l1;
+                        split_half(flip ? -f[2 * e] : f[2 * e], h0, l0);
+                        split_half(flip ? -f[2 * e + 1] : f[2 * e + 1], h1, l1);
+                        hi[e] = pack_half2(h0, h1);
+                        lo[e] = pack_half2(l0, l1);
+                    }
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(dst + Sh::kStage) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else {
+                    uint4 v = xq.v[j].w;
+                    if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                    *reinterpret_cast<uint4*>(dst) = v;
+                }
+            }
+        };
+        auto fetch_queries = [&](const Item& n) {
+            const int64_t mine = query_row(n);
+#pragma unroll 1
+            for (uint32_t j0 = 0; j0 < CH; j0 += QB) {
+                Queries xq;
+                request_queries(mine, j0, xq);
+                if (i == 0 || !n.twin) store_queries(j0, xq);
+            }
+        };
+        auto hand_over_queries = [&]() {
+            tc::fence_proxy_async();
             mbar_arrive(bar_q + 8 * i);
-
+        };
+        if (works) {
+            if (r == 0) run.next(nx);
+            fetch_queries(it);
+            hand_over_queries();
+            group_sync();
+        }
+        while (works && it.more) {
             const uint32_t in = it.twin ? r : i * kTile + r;  // pair within the block
             const bool live = in < it.pairs;
             const uint32_t pair = it.block * kBlockPairs + (live ? in : 0u);
@@ -685,6 +708,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
             };
+            auto rescale_output = [&](float f) {  // the scores at hand vouch for every product before them: O is at rest
+#pragma unroll 1
+                for (int j = 0; j < D; j += 16) {
+                    uint32_t o[16];
+                    tc::tmem_ld16(tO + j, o);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                    tc::tmem_st16(tO + j, o);
+                }
+            };
             auto stored = [&](uint32_t half) {  // the weights of half of the tile's keys may be used
                 tc::tmem_wait_st();
                 tc::fence_before_sync();
@@ -692,7 +726,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             };
             const uint32_t a = it.a[i], e = it.e[i], step = it.step;
             const bool any = a < e;
-            for (uint32_t t = a; t < e; t += step) {
+            uint32_t turn = 0;  // tiles of this cell done
+            for (uint32_t t = a; t < e; t += step, ++turn) {
                 dead = dead || !wait(bar_s + 8 * i, n_s & 1u);
                 dead = __any_sync(0xffffffffu, dead);
                 if (dead) break;
@@ -705,22 +740,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     for (int u = 0; u < static_cast<int>(sizeof(x) / 4); ++u)
                         if (col0 + u <= from || col0 + u > to) x[u] = 0xff800000u;
                 };
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (SPLIT) {
-                    // The tensor core cuts its sums short of a rounding, which adds up over a long accumulation: a tile's
-                    // output is taken out of tensor memory and added here, and the scores are read twice to make room.
-                    if (t != a) take_output();
+                    // The tensor core cuts its sums short of a rounding, which adds up over a long accumulation: after every
+                    // kFlush tiles the output is taken out of tensor memory and added here, and the scores are read twice to
+                    // make room for it.
+                    const bool fresh = turn % kFlush == 0;
+                    if (fresh && turn != 0) take_output();
                     float mx = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t x[16];
-                        tc::tmem_ld16(tS + 16 * j, x);
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[32];
+                        tc::tmem_ld32(tS + 32 * j, x);
                         tc::tmem_wait_ld();
-                        if (masked) hide(x, 16 * j);
+                        if (masked) hide(x, 32 * j);
                         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) top[u & 1] = fmaxf(top[u & 1], __uint_as_float(x[u]));
-                        mx = fmaxf(mx, fmaxf(top[0], top[1]));
+                        for (int u = 0; u < 32; u += 4) {
+                            top[0] = max3(top[0], __uint_as_float(x[u]), __uint_as_float(x[u + 1]));
+                            top[1] = max3(top[1], __uint_as_float(x[u + 2]), __uint_as_float(x[u + 3]));
+                        }
+                        mx = max3(mx, top[0], top[1]);
                     }
                     mx *= c;
                     const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
@@ -728,30 +767,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
 #pragma unroll
                         for (int u = 0; u < D; ++u) acc[u] *= f;
+                        if (!fresh) rescale_output(f);
                         if (grow) m = mx;
                         l *= f;
                     }
+                    if (!(mx < INFINITY)) m = NAN;  // a NaN or +infinity among the scores: the row is NaN from here on
                     const float nm = m == -INFINITY ? 0.f : -m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {  // 16 keys: high terms in their columns 0-7, low terms in 8-15
-                        uint32_t x[16], y[16];
-                        tc::tmem_ld16(tS + 16 * j, x);
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[32];
+                        tc::tmem_ld32(tS + 32 * j, x);
                         tc::tmem_wait_ld();
-                        if (masked) hide(x, 16 * j);
+                        if (masked) hide(x, 32 * j);
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const float w0 = fast_exp2(fmaf(__uint_as_float(x[2 * u]), c, nm));
-                            const float w1 = fast_exp2(fmaf(__uint_as_float(x[2 * u + 1]), c, nm));
-                            sum[u & 1] += w0;
-                            sum[2 + (u & 1)] += w1;
-                            const __half2 h = __floats2half2_rn(w0, w1);
-                            const float2 hf = __half22float2(h);
-                            y[u] = *reinterpret_cast<const uint32_t*>(&h);
-                            y[8 + u] = pack2(__half(), w0 - hf.x, w1 - hf.y);
+                        for (int g = 0; g < 2; ++g) {  // 16 keys: high terms in their columns 0-7, low terms in 8-15
+                            uint32_t y[16];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) {
+                                const float w0 = fast_exp2(fmaf(__uint_as_float(x[16 * g + 2 * u]), c, nm));
+                                const float w1 = fast_exp2(fmaf(__uint_as_float(x[16 * g + 2 * u + 1]), c, nm));
+                                sum[u & 1] += w0;
+                                sum[2 + (u & 1)] += w1;
+                                const __half2 h = __floats2half2_rn(w0, w1);
+                                const float2 hf = __half22float2(h);
+                                y[u] = *reinterpret_cast<const uint32_t*>(&h);
+                                y[8 + u] = pack2(__half(), w0 - hf.x, w1 - hf.y);
+                            }
+                            tc::tmem_st16(tS + 32 * j + 16 * g, y);
                         }
-                        tc::tmem_st16(tS + 16 * j, y);
-                        if (j == 3) stored(0);
+                        if (j == 1) stored(0);
                     }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 } else {
                     uint32_t x[4][32];
 #pragma unroll
@@ -770,21 +817,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const bool grow = mx > m + kRescaleStep || (m == -INFINITY && mx > m);
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-                        if (t != a) {  // the scores at hand vouch for every product before them: O is at rest
-#pragma unroll 1
-                            for (int j = 0; j < D; j += 16) {
-                                uint32_t o[16];
-                                tc::tmem_ld16(tO + j, o);
-                                tc::tmem_wait_ld();
-#pragma unroll
-                                for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                                tc::tmem_st16(tO + j, o);
-                            }
-                        }
+                        if (turn != 0) rescale_output(f);
                         if (grow) m = mx;
                         l *= f;
                     }
-                    if (!(mx < INFINITY)) m = NAN;  // a NaN or +infinity among the scores: the row is NaN from here on
+                    if (!(mx < INFINITY)) m = NAN;
                     const uint64_t c2 = pair_of(c, c), nm2 = pair_of(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
                     uint64_t sum2[2] = {0u, 0u};
 #pragma unroll
@@ -792,8 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         uint32_t y[16];
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
-                            const uint64_t v = fma2(pair_of(__uint_as_float(x[j][2 * u]), __uint_as_float(x[j][2 * u + 1])), c2, nm2);
-                            float2 e2 = unpair(v);
+                            float2 e2 = unpair(fma2(pair_of(__uint_as_float(x[j][2 * u]), __uint_as_float(x[j][2 * u + 1])), c2, nm2));
                             e2 = make_float2(fast_exp2(e2.x), fast_exp2(e2.y));
                             sum2[u & 1] = add2(sum2[u & 1], pair_of(e2.x, e2.y));
                             y[u] = pack2(P(), e2.x, e2.y);
@@ -802,11 +838,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         if (j == 1) stored(0);
                     }
                     const float2 s01 = unpair(add2(sum2[0], sum2[1]));
-                    sum[0] = s01.x;
-                    sum[1] = s01.y;
+                    l += s01.x + s01.y;
                 }
                 stored(1);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            Queries xq = {};
+            const bool more = nx.more != 0;
+            if constexpr (!SPLIT) {
+                if (more) request_queries(query_row(nx), 0, xq);
             }
             if (any && !dead) {
                 dead = !wait(bar_o + 8 * i, n_o & 1u);
@@ -829,78 +868,101 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             }
 
             // ---- the cell's end ----------------------------------------------------------------------------------------
-            const bool whole = it.n == it.T;
-            float2* const ex = reinterpret_cast<float2*>(smem + Sh::kQ);  // [stream][row] (maximum, sum), in the unused query tile
-            float f0 = 1.f, f1 = 0.f;                                     // weights of the own and the other stream's rows
+            const bool whole = it.n == it.T, twin = it.twin != 0;
+            float f0 = 1.f, f1 = 0.f;  // weights of the own and the other stream's rows
             bool other_any = false;
-            if (it.twin) {
+            if (twin) {
                 // Rows are the same in both streams and sit in the same lanes: each warpgroup takes half of the channels.
                 other_any = it.a[1 - i] < it.e[1 - i];
-                ex[tid] = make_float2(m, l);
+                exchange[tid] = make_float2(m, l);
                 tc::fence_before_sync();
                 both_sync();
                 tc::fence_after_sync();
-                const float2 x = ex[tid ^ 128];
-                const float M = fmaxf(m, x.x);
+                const float2 x = exchange[tid ^ 128];
+                const float M = m != m || x.x != x.x ? NAN : fmaxf(m, x.x);
                 f0 = m == -INFINITY ? 0.f : fast_exp2(m - M);
                 f1 = x.x == -INFINITY ? 0.f : fast_exp2(x.x - M);
                 l = l * f0 + x.y * f1;
                 m = M;
             }
             const uint32_t row = it.q.row0 + pair / group, head = it.kvh * group + pair % group;
-            const uint32_t c0 = it.twin ? i * (D / 2) : 0u, c1 = it.twin ? c0 + D / 2 : D;  // channels of this thread
-            const uint32_t tOther = tmem + lane_base + kTmemO + (1 - i) * D;
-            const uint32_t part = it.off == 0 ? 2 * cta + 1 : 2 * cta;
-            float4* const po = reinterpret_cast<float4*>(p.part_o) + static_cast<size_t>(part) * (D / 4) * kBlockPairs;
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            T* const dst = static_cast<T*>(p.out) + static_cast<uint64_t>(row) * p.out_row + head * head_dim;
-            auto put8 = [&](T* to, const float (&f)[8]) {
-                Vec8<T> v;
-                if constexpr (SPLIT) {
-                    v.set(f);
-                } else {
-                    v.w = make_uint4(pack2(P(), f[0], f[1]), pack2(P(), f[2], f[3]), pack2(P(), f[4], f[5]), pack2(P(), f[6], f[7]));
+            const uint32_t c0 = twin ? i * (D / 2) : 0u, c1 = twin ? c0 + D / 2 : D;  // channels of this thread
+            const int64_t dst = live ? static_cast<int64_t>(row * p.out_row + head * head_dim) : -1;
+            auto output16 = [&](uint32_t ch, float (&f)[16]) {
+                uint32_t o[16], y[16] = {};
+                tc::tmem_ld16(tO + ch, o);
+                if (twin) tc::tmem_ld16(tOther + ch, y);
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    f[u] = any ? __uint_as_float(o[u]) : 0.f;
+                    if (twin) f[u] = f[u] * f0 + (other_any ? __uint_as_float(y[u]) * f1 : 0.f);
                 }
-                v.store(to);
             };
-            if (!dead) {
-#pragma unroll 1
-                for (uint32_t ch = c0; ch < c1; ch += 16) {
-                    uint32_t o[16], y[16];
-                    float f[16];
-                    if (any) tc::tmem_ld16(tO + ch, o);
-                    if (it.twin && other_any) tc::tmem_ld16(tOther + ch, y);
-                    tc::tmem_wait_ld();
+            // A finished row goes out by way of shared memory, so that a warp stores whole rows: thread by thread, 32 rows at
+            // a time, every store would touch 32 lines (7000 clocks a cell).
+            auto stage16 = [&](uint32_t ch, const float (&f)[16], float by) {
+                if constexpr (SPLIT) {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        f[u] = any ? __uint_as_float(o[u]) : 0.f;
-                        if (it.twin) f[u] = f[u] * f0 + (other_any ? __uint_as_float(y[u]) * f1 : 0.f);
-                    }
-                    if (whole) {
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4*>(chunk_at(r, ch / 4 + g)) = make_float4(f[4 * g] * by, f[4 * g + 1] * by, f[4 * g + 2] * by, f[4 * g + 3] * by);
+                } else {
 #pragma unroll
-                        for (int g8 = 0; g8 < 2; ++g8) {
-                            float z[8];
-#pragma unroll
-                            for (int u = 0; u < 8; ++u) z[u] = f[8 * g8 + u] * inv;
-                            if (live && ch + 8 * g8 < head_dim) put8(dst + ch + 8 * g8, z);
-                        }
-                    } else if (live) {
-#pragma unroll
-                        for (int g4 = 0; g4 < 4; ++g4)
-                            po[static_cast<size_t>(ch / 4 + g4) * kBlockPairs + in] = make_float4(f[4 * g4], f[4 * g4 + 1], f[4 * g4 + 2], f[4 * g4 + 3]);
-                    }
+                    for (int g = 0; g < 2; ++g)
+                        *reinterpret_cast<uint4*>(chunk_at(r, ch / 8 + g)) =
+                            make_uint4(pack2(P(), f[8 * g] * by, f[8 * g + 1] * by), pack2(P(), f[8 * g + 2] * by, f[8 * g + 3] * by),
+                                       pack2(P(), f[8 * g + 4] * by, f[8 * g + 5] * by), pack2(P(), f[8 * g + 6] * by, f[8 * g + 7] * by));
                 }
-            }
+            };
+            auto send_rows = [&]() {
+                __syncwarp();
+                constexpr uint32_t E = 16 / sizeof(T);  // channels of a chunk
+                const uint32_t wide = (c1 - c0) / E, first = c0 / E;  // chunks of a row: a power of two up to 32
+                const uint32_t k = first + lane % wide, sub = lane / wide, rows = 32 / wide;
+#pragma unroll 4
+                for (uint32_t x = 0; x < 32; x += rows) {
+                    const int64_t off = __shfl_sync(0xffffffffu, dst, x + sub);
+                    if (off >= 0 && k * E < head_dim)
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + off + k * E) = *reinterpret_cast<const uint4*>(chunk_at((warp & 3) * 32 + x + sub, k));
+                }
+                __syncwarp();
+            };
             auto put_lse = [&](uint32_t lrow, uint32_t lhead, float top, float sum) {
                 if (p.lse)
                     p.lse[static_cast<uint64_t>(lrow) * p.q_heads + lhead] =
                         sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
             };
+            auto inverse = [](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };
             if (whole) {
-                if (!dead && live && (i == 0 || !it.twin)) put_lse(row, head, m, l);
+                if (!dead) {
+                    const float inv = inverse(l);
+#pragma unroll 1
+                    for (uint32_t ch = c0; ch < c1; ch += 16) {
+                        float f[16];
+                        output16(ch, f);
+                        stage16(ch, f, inv);
+                    }
+                    send_rows();
+                    if (live && (i == 0 || !twin)) put_lse(row, head, m, l);
+                }
             } else {
+                // The part goes out channels by rows: a warp's store is 512 contiguous bytes.
+                const uint32_t part = it.off == 0 ? 2 * cta + 1 : 2 * cta;
+                float4* const all = reinterpret_cast<float4*>(p.part_o);
                 float2* const pml = reinterpret_cast<float2*>(p.part_ml);
-                if (live && (i == 0 || !it.twin)) pml[static_cast<size_t>(part) * kBlockPairs + in] = make_float2(m, l);
+                if (!dead) {
+#pragma unroll 1
+                    for (uint32_t ch = c0; ch < c1; ch += 16) {
+                        float f[16];
+                        output16(ch, f);
+                        if (live) {
+#pragma unroll
+                            for (int g = 0; g < 4; ++g)
+                                all[(static_cast<size_t>(part) * (D / 4) + ch / 4 + g) * kBlockPairs + in] = make_float4(f[4 * g], f[4 * g + 1], f[4 * g + 2], f[4 * g + 3]);
+                        }
+                    }
+                }
+                if (live && (i == 0 || !twin)) pml[static_cast<size_t>(part) * kBlockPairs + in] = make_float2(m, l);
                 const uint64_t cell0 = it.pos - it.off;
                 const uint32_t first = static_cast<uint32_t>(cell0 / per), last = static_cast<uint32_t>((cell0 + it.T - 1) / per);
                 both_sync();
@@ -911,14 +973,53 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (ticket == last - first) p.tickets[first] = 0u;  // as the next launch wants it
                 }
                 both_sync();
+                // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...
+                const uint32_t n_parts = last - first + 1;
+                auto slot_of = [&](uint32_t k) { return static_cast<size_t>(2 * (first + k) + (k == 0 ? 1 : 0)); };
                 if (word[1] != 0u && !dead) {
                     __threadfence();
-                    // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...  Lanes
-                    // take neighbouring rows; a thread has the loads of several parts in flight.
-                    const uint32_t across = (it.pairs + 31) / 32 * 32, n_parts = last - first + 1;
-                    const float4* const all = reinterpret_cast<const float4*>(p.part_o);
-                    auto join = [&](auto batch) {
-                        constexpr uint32_t B = decltype(batch)::value;
+                    if (n_parts <= 3) {
+                        // One or two other parts: every thread joins its own row, its own part still in tensor memory.
+                        const uint32_t self = cta - first, k1 = self == 0 ? 1 : 0, k2 = n_parts == 3 ? (self == 2 ? 1 : 2) : k1;
+                        const float w2 = n_parts == 3 ? 1.f : 0.f;
+                        float2 x1 = make_float2(-INFINITY, 0.f), x2 = x1;
+                        if (live) {
+                            x1 = __ldcg(pml + slot_of(k1) * kBlockPairs + in);
+                            if (n_parts == 3) x2 = __ldcg(pml + slot_of(k2) * kBlockPairs + in);
+                        }
+                        float M = fmaxf(m, fmaxf(x1.x, x2.x));
+                        if (m != m || x1.x != x1.x || x2.x != x2.x) M = NAN;
+                        const float g0 = m == -INFINITY ? 0.f : fast_exp2(m - M), g1 = x1.x == -INFINITY ? 0.f : fast_exp2(x1.x - M),
+                                    g2 = x2.x == -INFINITY ? 0.f : w2 * fast_exp2(x2.x - M);
+                        const float L = l * g0 + x1.y * g1 + x2.y * g2, inv = inverse(L);
+                        const float4* const o1 = all + slot_of(k1) * (D / 4) * kBlockPairs + in;
+                        const float4* const o2 = all + slot_of(k2) * (D / 4) * kBlockPairs + in;
+#pragma unroll 1
+                        for (uint32_t ch = c0; ch < c1; ch += 16) {
+                            float f[16];
+                            float4 y1[4], y2[4];
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                y1[g] = y2[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (live) y1[g] = __ldcg(o1 + static_cast<size_t>(ch / 4 + g) * kBlockPairs);
+                                if (live && n_parts == 3) y2[g] = __ldcg(o2 + static_cast<size_t>(ch / 4 + g) * kBlockPairs);
+                            }
+                            output16(ch, f);
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                f[4 * g] = f[4 * g] * g0 + y1[g].x * g1 + y2[g].x * g2;
+                                f[4 * g + 1] = f[4 * g + 1] * g0 + y1[g].y * g1 + y2[g].y * g2;
+                                f[4 * g + 2] = f[4 * g + 2] * g0 + y1[g].z * g1 + y2[g].z * g2;
+                                f[4 * g + 3] = f[4 * g + 3] * g0 + y1[g].w * g1 + y2[g].w * g2;
+                            }
+                            stage16(ch, f, inv);
+                        }
+                        send_rows();
+                        if (live && (i == 0 || !twin)) put_lse(row, head, M, L);
+                    } else {
+                        // Many parts, of few rows as a rule: threads take (row, eight channels) and several parts at a time.
+                        constexpr uint32_t B = 6;
+                        const uint32_t across = (it.pairs + 31) / 32 * 32;
 #pragma unroll 1
                         for (uint32_t u = tid; u < across * (head_dim / 8); u += 256) {
                             const uint32_t jr = u % across, c8 = u / across;
@@ -930,19 +1031,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                                 float4 o0[B], o1[B];
 #pragma unroll
                                 for (uint32_t k = 0; k < B; ++k) {
-                                    const uint32_t kk = min(k0 + k, n_parts - 1);
-                                    const size_t sl = 2 * (first + kk) + (kk == 0 ? 1 : 0);
+                                    const size_t sl = slot_of(min(k0 + k, n_parts - 1));
                                     ml[k] = __ldcg(pml + sl * kBlockPairs + jr);
                                     o0[k] = __ldcg(all + (sl * (D / 4) + 2 * c8) * kBlockPairs + jr);
                                     o1[k] = __ldcg(all + (sl * (D / 4) + 2 * c8 + 1) * kBlockPairs + jr);
                                 }
                                 float to = M;
 #pragma unroll
-                                for (uint32_t k = 0; k < B; ++k) to = fmaxf(to, ml[k].x);
+                                for (uint32_t k = 0; k < B; ++k) to = max3(to, ml[k].x, ml[k].x);
                                 const float g0 = M == -INFINITY ? 0.f : fast_exp2(M - to);
                                 L *= g0;
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) z[e] *= g0;
+                                for (int q = 0; q < 8; ++q) z[q] *= g0;
                                 M = to;
 #pragma unroll
                                 for (uint32_t k = 0; k < B; ++k) {
@@ -952,27 +1052,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                                     z[4] += g1 * o1[k].x, z[5] += g1 * o1[k].y, z[6] += g1 * o1[k].z, z[7] += g1 * o1[k].w;
                                 }
                             }
-                            const float il = L > 0.f || L != L ? 1.f / L : 0.f;
+                            const float inv = inverse(L);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) z[e] *= il;
+                            for (int q = 0; q < 8; ++q) z[q] *= inv;
                             const uint32_t jp = it.block * kBlockPairs + jr, jrow = it.q.row0 + jp / group, jhead = it.kvh * group + jp % group;
-                            put8(static_cast<T*>(p.out) + static_cast<uint64_t>(jrow) * p.out_row + jhead * head_dim + 8 * c8, z);
+                            Vec8<T> v;
+                            if constexpr (SPLIT) {
+                                v.set(z);
+                            } else {
+                                v.w = make_uint4(pack2(P(), z[0], z[1]), pack2(P(), z[2], z[3]), pack2(P(), z[4], z[5]), pack2(P(), z[6], z[7]));
+                            }
+                            v.store(static_cast<T*>(p.out) + static_cast<uint64_t>(jrow) * p.out_row + jhead * head_dim + 8 * c8);
                             if (c8 == 0) put_lse(jrow, jhead, M, L);
                         }
-                    };
-                    if (n_parts <= 2)
-                        join(std::integral_constant<uint32_t, 2>());
-                    else
-                        join(std::integral_constant<uint32_t, 6>());
+                    }
                 }
             }
-            // Nothing of this cell is read any more: the exchange, the other stream's accumulator, the joined flag.
-            tc::fence_before_sync();
-            both_sync();
-            if (tid == 0) run.next(it);
-            both_sync();
-            tc::fence_after_sync();
-        } while (it.more);
+            if (twin) {  // the other stream's accumulator and the exchange are done with
+                tc::fence_before_sync();
+                both_sync();
+                tc::fence_after_sync();
+            }
+            if (more) {
+                // A twin cell's stream 1 reads the queries of stream 0: neither is handed over before both are free.
+                if (nx.twin) both_sync();
+                if constexpr (SPLIT) {
+                    fetch_queries(nx);
+                } else {
+                    if (i == 0 || !nx.twin) store_queries(0, xq);
+                }
+                hand_over_queries();
+            }
+            group_sync();
+            if (r == 0) {
+                it = nx;
+                if (nx.more) run.next(nx);
+            }
+            group_sync();
+        }
     }
     tc::fence_before_sync();
     __syncthreads();
