@@ -854,12 +854,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 tc::fence_after_sync();
                 if constexpr (SPLIT) {  // back to where the cell's end expects it
                     if (!dead) {
-                        take_output();
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) {
                             uint32_t o[16];
+                            tc::tmem_ld16(tO + 16 * j, o);
+                            tc::tmem_wait_ld();
 #pragma unroll
-                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(acc[16 * j + u]);
+                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(acc[16 * j + u] + __uint_as_float(o[u]));
                             tc::tmem_st16(tO + 16 * j, o);
                         }
                         tc::tmem_wait_st();
