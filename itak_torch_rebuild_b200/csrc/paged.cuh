@@ -233,9 +233,10 @@ int check_batch(const itk_paged_batch* b, const ErrorText& e, Batch* out);
 int check_row_dtype(int32_t rows, int32_t pages, const ErrorText& e);
 
 // The streaming kernel (any shape) on a device of `sms` multiprocessors.
-constexpr uint32_t kStreamRows = 16;  // rows of one of its parts
+constexpr uint32_t kStreamRows = 32;  // rows of one of its parts
 inline uint32_t stream_ctas(uint32_t sms, uint32_t head_dim) { return head_dim <= 128 ? 2 * sms : sms; }
-cudaError_t launch_stream(const AttnParams& p, int32_t row_dtype, uint32_t sms, cudaStream_t s);
+uint32_t stream_pairs(int32_t row_dtype);  // (row, head) pairs of its narrow block; the wide one has twice as many
+cudaError_t launch_stream(const AttnParams& p, int32_t row_dtype, bool wide, uint32_t sms, cudaStream_t s);
 // The tensor-memory kernel, for pools that it takes: head_dim up to 128, pages of at least 8 rows.
 constexpr uint32_t kTcRows = 256, kTcWidth = 128;  // rows and channels of one of its parts
 bool tc_takes(const Pool& pool);

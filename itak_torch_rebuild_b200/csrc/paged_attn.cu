@@ -32,7 +32,7 @@ struct Layout {
 Layout layout_of(uint32_t sms) {
     Layout l;
     // Two parts of 256 rows for each of the tensor-memory kernel's CTAs, one per multiprocessor; the streaming kernel's
-    // twice as many CTAs (above 128 channels: as many, of twice the width) have parts of 16 rows.
+    // twice as many CTAs (above 128 channels: as many, of twice the width) have parts of 32 rows.
     const uint64_t rows = 2ull * sms * kTcRows;
     static_assert(2 * kStreamRows <= kTcRows, "the larger of the two");
     l.ml = round_up(sizeof(unsigned int) * 2ull * sms);
@@ -96,11 +96,11 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     p.tickets = reinterpret_cast<unsigned int*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + l.ml);
     p.part_o = reinterpret_cast<float*>(ws + l.o);
-    // Few pairs per KV head stream, many go to tensor memory: up to the streaming kernel's block the score product has no
-    // room left for a second use of a key.
+    // Few pairs per KV head stream, many go to tensor memory.
     const uint64_t pairs = static_cast<uint64_t>(d->max_rows < batch->total_rows ? d->max_rows : batch->total_rows) * p.group;
     const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    const bool many = pairs > (d->dtype == ITK_ROW_F32 ? 8u : 16u);
-    const cudaError_t err = many && tc_takes(p.pool) ? launch_tc(p, d->dtype, sms, s) : launch_stream(p, d->dtype, sms, s);
+    const uint32_t narrow = stream_pairs(d->dtype);
+    const cudaError_t err = pairs > 2 * narrow && tc_takes(p.pool) ? launch_tc(p, d->dtype, sms, s)
+                                                                   : launch_stream(p, d->dtype, pairs > narrow, sms, s);
     return err == cudaSuccess ? 0 : e.cuda("paged attention launch failed", err);
 }
