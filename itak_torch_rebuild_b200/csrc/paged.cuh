@@ -166,6 +166,13 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __ushort_as
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// The kernels are launched as programmatic dependents: their blocks take their places while the kernel before them in the
+// stream still runs, and wait here before they touch memory (2 us of a call that follows another).
+__device__ __forceinline__ void after_predecessor() {
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
 
 // Writes the reason of a refusal into the caller's buffer.
@@ -222,6 +229,23 @@ public:
 private:
     std::atomic<uint64_t> bits_{0};
 };
+
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), uint32_t grid, uint32_t threads, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    const cudaError_t last = cudaGetLastError();
+    return e != cudaSuccess ? e : last;
+}
 
 constexpr uint64_t kMaxStride = 1ull << 40;
 

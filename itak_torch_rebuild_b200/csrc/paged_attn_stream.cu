@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
     const uint32_t n_seqs = p.batch.n_seqs, G = gridDim.x, cta = blockIdx.x;
     const uint32_t group = p.group, head_dim = p.pool.head_dim, shift = p.pool.page_shift;
 
+    after_predecessor();
+
     // ---- the batch summed up: prefix[s] = tiles reserved before sequence s -----------------------------------------
     // A cell's block of pairs reserves the tiles of its whole sequence (of its first row's window to its last key);
     // tiles that the block does not see are passed over in the walk.
@@ -675,8 +677,7 @@ cudaError_t launch_as(const AttnParams& p, uint32_t sms, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         prepared.mark(p.device);
     }
-    kernel<<<stream_ctas(sms, p.pool.head_dim), kThreads, smem_bytes<D, STAGES>(MT, p.batch.n_seqs), s>>>(p);
-    return cudaGetLastError();
+    return launch_dependent(kernel, stream_ctas(sms, p.pool.head_dim), kThreads, smem_bytes<D, STAGES>(MT, p.batch.n_seqs), s, p);
 }
 template <typename T>
 cudaError_t launch_width(const AttnParams& p, bool wide, uint32_t sms, cudaStream_t s) {

@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         tc::tmem_alloc(smem_u32(word), kTmemCols);
         tc::tmem_relinquish();
     }
+    after_predecessor();
     uint64_t* const prefix = reinterpret_cast<uint64_t*>(smem + 2 * Sh::kQ);  // [n_seqs + 1], scratch in the ring
     uint64_t* const per_head = prefix + n_seqs + 1;  // [n_seqs] tiles of one KV head
     SeqInfo* const info = reinterpret_cast<SeqInfo*>(per_head + n_seqs);
@@ -980,9 +981,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (word[1] != 0u && !dead) {
                     __threadfence();
                     if (n_parts <= 3) {
-                        // One or two other parts: every thread joins its own row, its own part still in tensor memory.
+                        // One or two other parts: every thread joins its own row, its own part still in tensor memory - in the
+                        // order of the parts, whichever of them came last, so that the same call gives the same bits.
                         const uint32_t self = cta - first, k1 = self == 0 ? 1 : 0, k2 = n_parts == 3 ? (self == 2 ? 1 : 2) : k1;
-                        const float w2 = n_parts == 3 ? 1.f : 0.f;
                         float2 x1 = make_float2(-INFINITY, 0.f), x2 = x1;
                         if (live) {
                             x1 = __ldcg(pml + slot_of(k1) * kBlockPairs + in);
@@ -990,9 +991,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         }
                         float M = fmaxf(m, fmaxf(x1.x, x2.x));
                         if (m != m || x1.x != x1.x || x2.x != x2.x) M = NAN;
-                        const float g0 = m == -INFINITY ? 0.f : fast_exp2(m - M), g1 = x1.x == -INFINITY ? 0.f : fast_exp2(x1.x - M),
-                                    g2 = x2.x == -INFINITY ? 0.f : w2 * fast_exp2(x2.x - M);
-                        const float L = l * g0 + x1.y * g1 + x2.y * g2, inv = inverse(L);
+                        auto weight = [&](float top) { return top == -INFINITY ? 0.f : fast_exp2(top - M); };
+                        // of (own, first other, second other), the one whose part is number 0, 1, 2
+                        auto in_order = [&](float own, float y1, float y2, float (&v)[3]) {
+                            v[0] = self == 0 ? own : y1;
+                            v[1] = self == 1 ? own : self == 0 ? y1 : y2;
+                            v[2] = self == 2 ? own : y2;
+                        };
+                        float wt[3], sums[3];
+                        in_order(weight(m), weight(x1.x), weight(x2.x), wt);
+                        in_order(l, x1.y, x2.y, sums);
+                        const float L = fmaf(sums[2], wt[2], fmaf(sums[1], wt[1], sums[0] * wt[0])), inv = inverse(L);
                         const float4* const o1 = all + slot_of(k1) * (D / 4) * kBlockPairs + in;
                         const float4* const o2 = all + slot_of(k2) * (D / 4) * kBlockPairs + in;
 #pragma unroll 1
@@ -1008,10 +1017,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             output16(ch, f);
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {
-                                f[4 * g] = f[4 * g] * g0 + y1[g].x * g1 + y2[g].x * g2;
-                                f[4 * g + 1] = f[4 * g + 1] * g0 + y1[g].y * g1 + y2[g].y * g2;
-                                f[4 * g + 2] = f[4 * g + 2] * g0 + y1[g].z * g1 + y2[g].z * g2;
-                                f[4 * g + 3] = f[4 * g + 3] * g0 + y1[g].w * g1 + y2[g].w * g2;
+                                const float u1[4] = {y1[g].x, y1[g].y, y1[g].z, y1[g].w}, u2[4] = {y2[g].x, y2[g].y, y2[g].z, y2[g].w};
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    float v[3];
+                                    in_order(f[4 * g + q], u1[q], u2[q], v);
+                                    f[4 * g + q] = fmaf(v[2], wt[2], fmaf(v[1], wt[1], v[0] * wt[0]));
+                                }
                             }
                             stage16(ch, f, inv);
                         }
@@ -1144,8 +1156,7 @@ cudaError_t launch_as(const AttnParams& p, int32_t page_dtype, uint32_t sms, cud
     }
     CUtensorMap km, vm;
     if (!make_map(&km, p.pool, p.pool.k, page_dtype) || !make_map(&vm, p.pool, p.pool.v, page_dtype)) return cudaErrorInvalidValue;
-    kernel<<<sms, kThreads, Shape<T, D>::kSmem, s>>>(p, km, vm);
-    return cudaGetLastError();
+    return launch_dependent(kernel, sms, kThreads, Shape<T, D>::kSmem, s, p, km, vm);
 }
 
 }  // namespace

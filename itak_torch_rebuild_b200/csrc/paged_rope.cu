@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) rope_apply_kernel(const __grid_const
     const T* src = static_cast<const T*>(p.x) + row * p.x_row;
     T* dst = static_cast<T*>(p.out) + row * p.o_row;
     Wide<T> ahead[kAhead];
+    after_predecessor();
     if constexpr (WIDE) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -186,6 +187,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
     const T* v = static_cast<const T*>(p.v) + row * p.v_row;
     auto source = [&](uint32_t h) { return h < hq ? q + h * D : h < hq + hkv ? k + (h - hq) * D : v + (h - hq - hkv) * D; };
     Wide<T> ahead[kAhead];
+    after_predecessor();
     if constexpr (WIDE) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -427,14 +429,14 @@ extern "C" int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* e
     const DeviceScope scope(d->device);
     if (scope.err != cudaSuccess) return e.cuda("rotate: the device cannot be used", scope.err);
     const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    auto launch = [&](auto kernel) { kernel<<<d->rows, kThreads, 0, s>>>(p); };
+    cudaError_t err = cudaSuccess;
+    auto launch = [&](auto kernel) { err = launch_dependent(kernel, d->rows, kThreads, 0, s, p); };
     if (d->dtype == ITK_ROW_F32)
         wide ? launch(rope_apply_kernel<float, true>) : launch(rope_apply_kernel<float, false>);
     else if (d->dtype == ITK_ROW_F16)
         wide ? launch(rope_apply_kernel<__half, true>) : launch(rope_apply_kernel<__half, false>);
     else
         wide ? launch(rope_apply_kernel<__nv_bfloat16, true>) : launch(rope_apply_kernel<__nv_bfloat16, false>);
-    const cudaError_t err = cudaGetLastError();
     return err == cudaSuccess ? 0 : e.cuda("rotate launch failed", err);
 }
 
@@ -488,7 +490,8 @@ extern "C" int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* b
     const DeviceScope scope(kv->device);
     if (scope.err != cudaSuccess) return e.cuda("paged append: the device cannot be used", scope.err);
     const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    auto launch = [&](auto kernel) { kernel<<<batch->total_rows, kThreads, 0, s>>>(p); };
+    cudaError_t err = cudaSuccess;
+    auto launch = [&](auto kernel) { err = launch_dependent(kernel, batch->total_rows, kThreads, 0, s, p); };
     if (d->dtype == ITK_ROW_F32)
         wide ? launch(paged_append_kernel<float, __half, true>) : launch(paged_append_kernel<float, __half, false>);
     else if (d->dtype == ITK_ROW_F16)
@@ -496,6 +499,5 @@ extern "C" int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* b
     else
         wide ? launch(paged_append_kernel<__nv_bfloat16, __nv_bfloat16, true>)
              : launch(paged_append_kernel<__nv_bfloat16, __nv_bfloat16, false>);
-    const cudaError_t err = cudaGetLastError();
     return err == cudaSuccess ? 0 : e.cuda("paged append launch failed", err);
 }
