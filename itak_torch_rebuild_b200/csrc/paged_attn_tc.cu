@@ -620,62 +620,62 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         // A row of Q, and of the output on its way out, lies in the stream's query tile: 16-byte chunk k of row x here.
         unsigned char* const qs = smem + i * Sh::kQ;
         auto chunk_at = [&](uint32_t x, uint32_t k) { return qs + (k / 8) * Sh::kPanel + x * 128 + (((k % 8) ^ (x & 7)) << 4); };
-        // A block's queries, a batch of passes at a time.  16-bit rows are requested before the cell ahead of them ends, all
-        // passes at once, and stored behind it; f32 rows would take 128 registers and go batch by batch at its end.
+        // A block's queries into shared memory, a warp its own 32 rows, 16 bytes of channels a lane.  This, like all that runs
+        // once a cell, is a rolled loop: its code is never in the instruction cache when its turn comes, and straight-line
+        // code is fetched at about a byte a clock (16 unrolled loads took 5000 clocks to issue).
         constexpr uint32_t CH = D / 8, RP = 32 / CH;  // lanes of a row, rows of a pass; CH passes for a warp's 32 rows
-        constexpr uint32_t QB = SPLIT ? CH / 4 : CH;
-        struct Queries {
-            Vec8<T> v[QB];
-        };
-        auto query_row = [&](const Item& n) -> int64_t {  // where row r's query lies, or -1
+        auto fetch_queries = [&](const Item& n) {
             const uint32_t in = i * kTile + r, pair = n.block * kBlockPairs + in;
-            if (in >= n.pairs || (i == 1 && n.twin)) return -1;  // (a twin cell's streams both read stream 0's)
-            return static_cast<int64_t>((n.q.row0 + pair / group) * p.q_row + (n.kvh * group + pair % group) * head_dim);
-        };
-        auto request_queries = [&](int64_t mine, uint32_t j0, Queries& xq) {
+            const bool has = in < n.pairs;
+            const int64_t mine = has ? static_cast<int64_t>((n.q.row0 + pair / group) * p.q_row + (n.kvh * group + pair % group) * head_dim) : -1;
+            if (i == 1 && n.twin) return;  // both streams read stream 0's
             const uint32_t ch = (lane % CH) * 8;
+            const T* const q = static_cast<const T*>(p.q);
+            if (SPLIT || flip) {
+                constexpr uint32_t QB = 4;
+#pragma unroll 1
+                for (uint32_t j0 = 0; j0 < CH; j0 += QB) {
+                    Vec8<T> x[QB];
 #pragma unroll
-            for (uint32_t j = 0; j < QB; ++j) {
-                const int64_t off = __shfl_sync(0xffffffffu, mine, (j0 + j) * RP + lane / CH);
-                xq.v[j] = Vec8<T>{};
-                if (off >= 0 && ch < head_dim) xq.v[j].load(static_cast<const T*>(p.q) + off + ch);
-            }
-        };
-        auto store_queries = [&](uint32_t j0, const Queries& xq) {
-#pragma unroll
-            for (uint32_t j = 0; j < QB; ++j) {
-                unsigned char* const dst = chunk_at((warp & 3) * 32 + (j0 + j) * RP + lane / CH, lane % CH);
-                if constexpr (SPLIT) {
-                    float f[8];
-                    xq.v[j].get(f);
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        __half h0, l0, h1, l1;
-                        split_half(flip ? -f[2 * e] : f[2 * e], h0, l0);
-                        split_half(flip ? -f[2 * e + 1] : f[2 * e + 1], h1, l1);
-                        hi[e] = pack_half2(h0, h1);
-                        lo[e] = pack_half2(l0, l1);
+                    for (uint32_t j = 0; j < QB; ++j) {
+                        const int64_t off = __shfl_sync(0xffffffffu, mine, (j0 + j) * RP + lane / CH);
+                        x[j] = Vec8<T>{};
+                        if (off >= 0 && ch < head_dim) x[j].load(q + off + ch);
                     }
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(dst + Sh::kStage) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                } else {
-                    uint4 v = xq.v[j].w;
-                    if (flip) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-                    *reinterpret_cast<uint4*>(dst) = v;
+#pragma unroll
+                    for (uint32_t j = 0; j < QB; ++j) {
+                        unsigned char* const dst = chunk_at((warp & 3) * 32 + (j0 + j) * RP + lane / CH, lane % CH);
+                        if constexpr (SPLIT) {
+                            float f[8];
+                            x[j].get(f);
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                __half h0, l0, h1, l1;
+                                split_half(flip ? -f[2 * e] : f[2 * e], h0, l0);
+                                split_half(flip ? -f[2 * e + 1] : f[2 * e + 1], h1, l1);
+                                hi[e] = pack_half2(h0, h1);
+                                lo[e] = pack_half2(l0, l1);
+                            }
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(dst + Sh::kStage) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        } else {
+                            const uint4 v = x[j].w;
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll 2
+                for (uint32_t j = 0; j < CH; ++j) {
+                    const int64_t off = __shfl_sync(0xffffffffu, mine, j * RP + lane / CH);
+                    const bool live = off >= 0 && ch < head_dim;
+                    cp_async16(smem_u32(chunk_at((warp & 3) * 32 + j * RP + lane / CH, lane % CH)), q + (live ? off + ch : 0), live ? 16u : 0u);
                 }
             }
         };
-        auto fetch_queries = [&](const Item& n) {
-            const int64_t mine = query_row(n);
-#pragma unroll 1
-            for (uint32_t j0 = 0; j0 < CH; j0 += QB) {
-                Queries xq;
-                request_queries(mine, j0, xq);
-                if (i == 0 || !n.twin) store_queries(j0, xq);
-            }
-        };
         auto hand_over_queries = [&]() {
+            asm volatile("cp.async.wait_all;\n" ::: "memory");
             tc::fence_proxy_async();
             mbar_arrive(bar_q + 8 * i);
         };
@@ -843,11 +843,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
                 stored(1);
             }
-            Queries xq = {};
-            const bool more = nx.more != 0;
-            if constexpr (!SPLIT) {
-                if (more) request_queries(query_row(nx), 0, xq);
-            }
             if (any && !dead) {
                 dead = !wait(bar_o + 8 * i, n_o & 1u);
                 dead = __any_sync(0xffffffffu, dead);
@@ -980,50 +975,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 auto slot_of = [&](uint32_t k) { return static_cast<size_t>(2 * (first + k) + (k == 0 ? 1 : 0)); };
                 if (word[1] != 0u && !dead) {
                     __threadfence();
-                    if (n_parts <= 3) {
-                        // One or two other parts: every thread joins its own row, its own part still in tensor memory - in the
-                        // order of the parts, whichever of them came last, so that the same call gives the same bits.
-                        const uint32_t self = cta - first, k1 = self == 0 ? 1 : 0, k2 = n_parts == 3 ? (self == 2 ? 1 : 2) : k1;
-                        float2 x1 = make_float2(-INFINITY, 0.f), x2 = x1;
-                        if (live) {
-                            x1 = __ldcg(pml + slot_of(k1) * kBlockPairs + in);
-                            if (n_parts == 3) x2 = __ldcg(pml + slot_of(k2) * kBlockPairs + in);
-                        }
-                        float M = fmaxf(m, fmaxf(x1.x, x2.x));
-                        if (m != m || x1.x != x1.x || x2.x != x2.x) M = NAN;
-                        auto weight = [&](float top) { return top == -INFINITY ? 0.f : fast_exp2(top - M); };
-                        // of (own, first other, second other), the one whose part is number 0, 1, 2
-                        auto in_order = [&](float own, float y1, float y2, float (&v)[3]) {
-                            v[0] = self == 0 ? own : y1;
-                            v[1] = self == 1 ? own : self == 0 ? y1 : y2;
-                            v[2] = self == 2 ? own : y2;
+                    if (n_parts == 2) {
+                        // Every thread joins its own row, its own part still in tensor memory - in the order of the parts,
+                        // whichever of the two came last, so that the same call gives the same bits.
+                        const bool own_first = cta == first;
+                        const size_t slot = slot_of(own_first ? 1 : 0);
+                        float2 x1 = make_float2(-INFINITY, 0.f);
+                        if (live) x1 = __ldcg(pml + slot * kBlockPairs + in);
+                        const float M = m != m || x1.x != x1.x ? NAN : fmaxf(m, x1.x);
+                        const float g0 = m == -INFINITY ? 0.f : fast_exp2(m - M), g1 = x1.x == -INFINITY ? 0.f : fast_exp2(x1.x - M);
+                        const float wa = own_first ? g0 : g1, wb = own_first ? g1 : g0;
+                        auto joined = [&](float own, float other) {
+                            return fmaf(own_first ? other : own, wb, (own_first ? own : other) * wa);
                         };
-                        float wt[3], sums[3];
-                        in_order(weight(m), weight(x1.x), weight(x2.x), wt);
-                        in_order(l, x1.y, x2.y, sums);
-                        const float L = fmaf(sums[2], wt[2], fmaf(sums[1], wt[1], sums[0] * wt[0])), inv = inverse(L);
-                        const float4* const o1 = all + slot_of(k1) * (D / 4) * kBlockPairs + in;
-                        const float4* const o2 = all + slot_of(k2) * (D / 4) * kBlockPairs + in;
-#pragma unroll 1
+                        const float L = joined(l, x1.y), inv = inverse(L);
+                        const float4* const o1 = all + slot * (D / 4) * kBlockPairs + in;
+#pragma unroll 2
                         for (uint32_t ch = c0; ch < c1; ch += 16) {
                             float f[16];
-                            float4 y1[4], y2[4];
+                            float4 y1[4];
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {
-                                y1[g] = y2[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                y1[g] = make_float4(0.f, 0.f, 0.f, 0.f);
                                 if (live) y1[g] = __ldcg(o1 + static_cast<size_t>(ch / 4 + g) * kBlockPairs);
-                                if (live && n_parts == 3) y2[g] = __ldcg(o2 + static_cast<size_t>(ch / 4 + g) * kBlockPairs);
                             }
                             output16(ch, f);
 #pragma unroll
                             for (int g = 0; g < 4; ++g) {
-                                const float u1[4] = {y1[g].x, y1[g].y, y1[g].z, y1[g].w}, u2[4] = {y2[g].x, y2[g].y, y2[g].z, y2[g].w};
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    float v[3];
-                                    in_order(f[4 * g + q], u1[q], u2[q], v);
-                                    f[4 * g + q] = fmaf(v[2], wt[2], fmaf(v[1], wt[1], v[0] * wt[0]));
-                                }
+                                f[4 * g] = joined(f[4 * g], y1[g].x);
+                                f[4 * g + 1] = joined(f[4 * g + 1], y1[g].y);
+                                f[4 * g + 2] = joined(f[4 * g + 2], y1[g].z);
+                                f[4 * g + 3] = joined(f[4 * g + 3], y1[g].w);
                             }
                             stage16(ch, f, inv);
                         }
@@ -1086,21 +1068,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 both_sync();
                 tc::fence_after_sync();
             }
+            const bool more = nx.more != 0;
             if (more) {
                 // A twin cell's stream 1 reads the queries of stream 0: neither is handed over before both are free.
                 if (nx.twin) both_sync();
-                if constexpr (SPLIT) {
-                    fetch_queries(nx);
-                } else {
-                    if (i == 0 || !nx.twin) store_queries(0, xq);
-                }
-                hand_over_queries();
+                fetch_queries(nx);
             }
             group_sync();
             if (r == 0) {
                 it = nx;
-                if (nx.more) run.next(nx);
+                if (more) run.next(nx);
             }
+            if (more) hand_over_queries();
             group_sync();
         }
     }
