@@ -55,6 +55,10 @@ constexpr uint32_t kTile = 128;       // keys of a tile, and rows of a stream
 constexpr uint32_t kBlockPairs = 256;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;
 constexpr float kRescaleStep = 8.f;
+// How the tiles of all cells are cut into runs.  A cell's end costs its CTA about 3 tiles (the last products, the rows' way
+// out, the next queries), so each cell reserves as many beyond its own; a cut inside a cell costs two CTAs a partial each and
+// one of them the join; a cut that would leave kSnap tiles at a cell's beginning or end moves there.
+constexpr uint32_t kCellCost = 3, kSnap = 1;
 constexpr uint32_t kFlush = 2;            // f32 rows: tiles that add up in tensor memory
 constexpr uint32_t kSmemBytes = 232448;   // all that a block can have
 constexpr uint32_t kTailBytes = 3072;     // mbarriers, the roles' items, the streams' exchange
@@ -219,7 +223,7 @@ struct Run {
         it.more = 1;
     }
     __device__ __forceinline__ void next(Item& it) const {
-        it.pos += it.n;
+        it.pos += it.T + kCellCost - it.off;
         it.more = 0;
         if (it.pos >= end) return;
         if (++it.block == it.blocks) {
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         uint64_t sum = kLater;
         if (blocks <= kOwnBlocks) {
             sum = 0;
-            for (uint32_t i = 0; i < blocks; ++i) sum += cell_tiles(q, i, group, window);
+            for (uint32_t i = 0; i < blocks; ++i) sum += cell_tiles(q, i, group, window) + kCellCost;
         }
         per_head[s] = sum;
     }
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const SeqInfo q = info[s];
         const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
         uint64_t sum = 0;
-        for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window);
+        for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window) + kCellCost;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         __syncwarp();
@@ -347,53 +351,85 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     __syncthreads();
     const uint64_t W = prefix[n_seqs];
     const uint64_t per = max((W + gridDim.x - 1) / gridDim.x, static_cast<uint64_t>(1));
-    const uint64_t run0 = cta * per, run1 = min(W, run0 + per);
+    const uint64_t snap = min(static_cast<uint64_t>(kSnap), per / 2);
+    // CTA c's run is [cut(c), cut(c + 1)): warps 0 and 1 work the two out.
+    if (warp < 2) {
+        uint64_t pos = (cta + warp) * per;
+        uint32_t s = 0, kvh = 0, block = 0, blocks = 0;
+        uint64_t left = 0;
+        SeqInfo q{0, 0, 0};
+        if (pos < W) {
+            uint32_t lo = 0, hi = n_seqs;  // the last sequence that begins at or before pos and is not empty
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (prefix[mid] <= pos)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            s = lo;
+            q = info[s];
+            const uint64_t in = pos - prefix[s];
+            kvh = static_cast<uint32_t>(in / per_head[s]);
+            left = in % per_head[s];
+            blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
+            uint32_t tiles = 0;  // of that block
+            for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {  // the block that holds position `left` of the KV head
+                const uint32_t mine = b0 + lane < blocks ? cell_tiles(q, b0 + lane, group, window) + kCellCost : 0u;
+                uint32_t incl = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= static_cast<uint32_t>(d)) incl += o;
+                }
+                const uint32_t here = __ballot_sync(0xffffffffu, incl > left);
+                if (here != 0u) {
+                    const int at = __ffs(here) - 1;
+                    block = b0 + at;
+                    left -= __shfl_sync(0xffffffffu, incl - mine, at);
+                    tiles = __shfl_sync(0xffffffffu, mine, at) - kCellCost;
+                    break;
+                }
+                left -= __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (left <= snap) {
+                pos -= left;
+                left = 0;
+            } else if (left + snap >= tiles) {  // to the next cell
+                pos += tiles + kCellCost - left;
+                left = 0;
+                if (++block == blocks) {
+                    block = 0;
+                    if (++kvh == p.pool.kv_heads) {
+                        kvh = 0;
+                        do ++s;
+                        while (s < n_seqs && info[s].rows == 0);
+                        if (s < n_seqs) q = info[s];
+                        blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            Item& x = items[warp];
+            x.pos = min(pos, W);
+            x.s = s;
+            x.kvh = kvh;
+            x.block = block;
+            x.blocks = blocks;
+            x.off = static_cast<uint32_t>(left);
+            x.q = q;
+        }
+    }
+    __syncthreads();
+    const uint64_t run0 = items[0].pos, run1 = items[1].pos;
     const bool works = run0 < run1;
     const Run run{p, run1};
-    if (works && warp == 0) {  // where the run begins
-        uint32_t lo = 0, hi = n_seqs;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (prefix[mid] <= run0)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        const SeqInfo q = info[lo];
-        const uint64_t in = run0 - prefix[lo];
-        const uint32_t kvh = static_cast<uint32_t>(in / per_head[lo]);
-        uint64_t left = in % per_head[lo];
-        uint32_t block = 0;
-        const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
-        for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {  // the block that holds tile `left` of the KV head
-            const uint32_t mine = b0 + lane < blocks ? cell_tiles(q, b0 + lane, group, window) : 0u;
-            uint32_t incl = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= static_cast<uint32_t>(d)) incl += o;
-            }
-            const uint32_t here = __ballot_sync(0xffffffffu, incl > left);
-            if (here != 0u) {
-                const int at = __ffs(here) - 1;
-                block = b0 + at;
-                left -= __shfl_sync(0xffffffffu, incl - mine, at);
-                break;
-            }
-            left -= __shfl_sync(0xffffffffu, incl, 31);
-        }
-        Item& first = items[0];
-        if (lane == 0) {
-            first.s = lo;
-            first.kvh = kvh;
-            first.block = block;
-            first.blocks = blocks;
-            first.pos = run0;
-            first.q = q;
-            run.open_cell(first, static_cast<uint32_t>(left));
-        }
+    __syncthreads();
+    if (works && warp == 0) {
+        if (lane == 0) run.open_cell(items[0], items[0].off);
         __syncwarp();
-        if (lane > 0 && lane < kItems) items[lane] = first;
+        if (lane > 0 && lane < kItems) items[lane] = items[0];
     }
     tc::fence_proxy_async();  // the ring was the planning's scratch, TMA writes it next
     tc::fence_before_sync();
@@ -429,16 +465,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             Item& it = items[6];
             do {
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
+                const uint32_t lo = it.lo, hi = it.hi;
+                auto holds = [&](uint32_t key) { return row_at < kTile && key < hi && key + (1u << box_shift) > lo; };
+                auto page_of = [&](uint32_t key) { return holds(key) ? __ldg(tab + (key >> shift)) : 0u; };
+                uint32_t ahead = it.t0 < it.t1 ? page_of(it.t0 * kTile + row_at) : 0u;  // page numbers come a tile ahead
                 for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
                     const uint32_t key = t * kTile + row_at;  // the box holds keys [key, key + box rows)
-                    const bool mine = row_at < kTile && key < it.hi && key + (1u << box_shift) > it.lo;
-                    uint32_t page = 0;
-                    if (mine) {
-                        page = __ldg(tab + (key >> shift));
-                        if (page >= p.pool.n_pages) {
-                            raise(p.batch, kBadPage);
-                            page = p.pool.n_pages;  // outside the map: zeros
-                        }
+                    const bool mine = holds(key);
+                    uint32_t page = ahead;
+                    if (t + 1 < it.t1) ahead = page_of(key + kTile);
+                    if (mine && page >= p.pool.n_pages) {
+                        raise(p.batch, kBadPage);
+                        page = p.pool.n_pages;  // outside the map: zeros
                     }
                     const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
                     const uint32_t bytes = boxes << (box_shift + 7);
@@ -960,8 +998,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
                 if (live && (i == 0 || !twin)) pml[static_cast<size_t>(part) * kBlockPairs + in] = make_float2(m, l);
+                // The CTAs that share it: those whose runs begin inside it, and the one in whose run it begins.
                 const uint64_t cell0 = it.pos - it.off;
-                const uint32_t first = static_cast<uint32_t>(cell0 / per), last = static_cast<uint32_t>((cell0 + it.T - 1) / per);
+                uint32_t first = static_cast<uint32_t>(cell0 / per), last = static_cast<uint32_t>((cell0 + it.T - 1) / per);
+                if ((first + 1) * per - cell0 <= snap) ++first;  // that cut has moved to the cell's beginning
+                if (last > first && last * per - cell0 + snap >= it.T) --last;  // ... and that one behind its end
                 both_sync();
                 if (tid == 0) {
                     __threadfence();  // cumulative over the stores above (ordered before the barrier)
@@ -1012,53 +1053,77 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         send_rows();
                         if (live && (i == 0 || !twin)) put_lse(row, head, M, L);
                     } else {
-                        // Many parts, of few rows as a rule: threads take (row, eight channels) and several parts at a time.
-                        constexpr uint32_t B = 6;
-                        const uint32_t across = (it.pairs + 31) / 32 * 32;
+                        // Threads take (row, eight channels), two such at a time and several parts of each: what a join costs
+                        // is the latency of its loads.
+                        constexpr uint32_t B = 5;
+                        const uint32_t across = (it.pairs + 31) / 32 * 32, units = across * (head_dim / 8);
 #pragma unroll 1
-                        for (uint32_t u = tid; u < across * (head_dim / 8); u += 256) {
-                            const uint32_t jr = u % across, c8 = u / across;
-                            if (jr >= it.pairs) continue;
-                            float M = -INFINITY, L = 0.f, z[8] = {};
+                        for (uint32_t u0 = tid; u0 < units; u0 += 512) {
+                            float M[2] = {-INFINITY, -INFINITY}, L[2] = {}, z[2][8] = {};
+                            uint32_t jr[2], c8[2];
+                            bool has[2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t u = u0 + 256 * h;
+                                jr[h] = u % across;
+                                c8[h] = u / across;
+                                has[h] = u < units && jr[h] < it.pairs;
+                            }
 #pragma unroll 1
                             for (uint32_t k0 = 0; k0 < n_parts; k0 += B) {
-                                float2 ml[B];
-                                float4 o0[B], o1[B];
+                                float2 ml[2][B];
+                                float4 o0[2][B], o1[2][B];
 #pragma unroll
-                                for (uint32_t k = 0; k < B; ++k) {
-                                    const size_t sl = slot_of(min(k0 + k, n_parts - 1));
-                                    ml[k] = __ldcg(pml + sl * kBlockPairs + jr);
-                                    o0[k] = __ldcg(all + (sl * (D / 4) + 2 * c8) * kBlockPairs + jr);
-                                    o1[k] = __ldcg(all + (sl * (D / 4) + 2 * c8 + 1) * kBlockPairs + jr);
-                                }
-                                float to = M;
+                                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                                for (uint32_t k = 0; k < B; ++k) to = max3(to, ml[k].x, ml[k].x);
-                                const float g0 = M == -INFINITY ? 0.f : fast_exp2(M - to);
-                                L *= g0;
+                                    for (uint32_t k = 0; k < B; ++k) {
+                                        const size_t sl = slot_of(min(k0 + k, n_parts - 1));
+                                        ml[h][k] = make_float2(-INFINITY, 0.f);
+                                        o0[h][k] = o1[h][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                        if (has[h]) {
+                                            ml[h][k] = __ldcg(pml + sl * kBlockPairs + jr[h]);
+                                            o0[h][k] = __ldcg(all + (sl * (D / 4) + 2 * c8[h]) * kBlockPairs + jr[h]);
+                                            o1[h][k] = __ldcg(all + (sl * (D / 4) + 2 * c8[h] + 1) * kBlockPairs + jr[h]);
+                                        }
+                                    }
 #pragma unroll
-                                for (int q = 0; q < 8; ++q) z[q] *= g0;
-                                M = to;
+                                for (int h = 0; h < 2; ++h) {
+                                    float to = M[h];
 #pragma unroll
-                                for (uint32_t k = 0; k < B; ++k) {
-                                    const float g1 = k0 + k < n_parts && ml[k].x != -INFINITY ? fast_exp2(ml[k].x - M) : 0.f;
-                                    L += g1 * ml[k].y;
-                                    z[0] += g1 * o0[k].x, z[1] += g1 * o0[k].y, z[2] += g1 * o0[k].z, z[3] += g1 * o0[k].w;
-                                    z[4] += g1 * o1[k].x, z[5] += g1 * o1[k].y, z[6] += g1 * o1[k].z, z[7] += g1 * o1[k].w;
+                                    for (uint32_t k = 0; k < B; ++k) to = max3(to, ml[h][k].x, ml[h][k].x);
+                                    const float g0 = M[h] == -INFINITY ? 0.f : fast_exp2(M[h] - to);
+                                    L[h] *= g0;
+#pragma unroll
+                                    for (int q = 0; q < 8; ++q) z[h][q] *= g0;
+                                    M[h] = to;
+#pragma unroll
+                                    for (uint32_t k = 0; k < B; ++k) {
+                                        const float g1 = k0 + k < n_parts && ml[h][k].x != -INFINITY ? fast_exp2(ml[h][k].x - to) : 0.f;
+                                        L[h] += g1 * ml[h][k].y;
+                                        const float4 x0 = o0[h][k], x1 = o1[h][k];
+                                        z[h][0] += g1 * x0.x, z[h][1] += g1 * x0.y, z[h][2] += g1 * x0.z, z[h][3] += g1 * x0.w;
+                                        z[h][4] += g1 * x1.x, z[h][5] += g1 * x1.y, z[h][6] += g1 * x1.z, z[h][7] += g1 * x1.w;
+                                    }
                                 }
                             }
-                            const float inv = inverse(L);
+#pragma unroll 1
+                            for (int h = 0; h < 2; ++h) {
+                                if (!(h == 0 ? has[0] : has[1])) continue;
+                                const uint32_t row_in = h == 0 ? jr[0] : jr[1], ch = 8 * (h == 0 ? c8[0] : c8[1]);
+                                const float top = h == 0 ? M[0] : M[1], sum = h == 0 ? L[0] : L[1], inv = inverse(sum);
+                                float f[8];
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) z[q] *= inv;
-                            const uint32_t jp = it.block * kBlockPairs + jr, jrow = it.q.row0 + jp / group, jhead = it.kvh * group + jp % group;
-                            Vec8<T> v;
-                            if constexpr (SPLIT) {
-                                v.set(z);
-                            } else {
-                                v.w = make_uint4(pack2(P(), z[0], z[1]), pack2(P(), z[2], z[3]), pack2(P(), z[4], z[5]), pack2(P(), z[6], z[7]));
+                                for (int q = 0; q < 8; ++q) f[q] = (h == 0 ? z[0][q] : z[1][q]) * inv;
+                                const uint32_t jp = it.block * kBlockPairs + row_in, jrow = it.q.row0 + jp / group, jhead = it.kvh * group + jp % group;
+                                Vec8<T> v;
+                                if constexpr (SPLIT) {
+                                    v.set(f);
+                                } else {
+                                    v.w = make_uint4(pack2(P(), f[0], f[1]), pack2(P(), f[2], f[3]), pack2(P(), f[4], f[5]), pack2(P(), f[6], f[7]));
+                                }
+                                v.store(static_cast<T*>(p.out) + static_cast<uint64_t>(jrow) * p.out_row + jhead * head_dim + ch);
+                                if (ch == 0) put_lse(jrow, jhead, top, sum);
                             }
-                            v.store(static_cast<T*>(p.out) + static_cast<uint64_t>(jrow) * p.out_row + jhead * head_dim + 8 * c8);
-                            if (c8 == 0) put_lse(jrow, jhead, M, L);
                         }
                     }
                 }
