@@ -59,7 +59,6 @@ constexpr float kRescaleStep = 8.f;
 // out, the next queries), so each cell reserves as many beyond its own; a cut inside a cell costs two CTAs a partial each and
 // one of them the join; a cut that would leave kSnap tiles at a cell's beginning or end moves there.
 constexpr uint32_t kCellCost = 3, kSnap = 1;
-constexpr uint32_t kFlush = 2;            // f32 rows: tiles that add up in tensor memory
 constexpr uint32_t kSmemBytes = 232448;   // all that a block can have
 constexpr uint32_t kTailBytes = 3072;     // mbarriers, the roles' items, the streams' exchange
 constexpr long long kWaitClocks = 2000000000ll;  // about a second
@@ -577,7 +576,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const uint32_t xa = it.a[1 - i], xe = it.e[1 - i];
                 const uint32_t rounds = xa < xe ? (xe - xa + step - 1) / step + 1 : 0u;  // of the other stream: 0, 1, ...
                 // One copy of the code: the first round has no weights to use yet, the last no scores to make.
-                uint32_t n_in = 0;  // tiles of the cell used
                 uint32_t after = i == 0 ? 0xffffffffu : 0u;  // the other stream's round that this one follows (stream 0 begins)
                 for (uint32_t nt = a; ok && a < e; nt += step, ++after) {
                     const bool have = nt != a, more = nt < e;  // weights of tile t; scores of tile nt to come
@@ -592,8 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (ok && have) {  // O (+)= P V(t)
                         tc::fence_after_sync();
                         const uint64_t v = kDescV + ((ring + cv % NST * Sh::kStage) >> 4);
-                        // (f32 rows: the softmax takes the output out after every kFlush tiles)
-                        const uint32_t acc = SPLIT ? (n_in++ % kFlush != 0 ? 1u : 0u) : (t != a ? 1u : 0u);
+                        [[maybe_unused]] const uint32_t acc = t != a ? 1u : 0u;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             if (j == 4) {
@@ -601,8 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                                 if (!ok) break;
                                 tc::fence_after_sync();
                             }
-                            if constexpr (SPLIT) {
-                                tc::mma_f16_ts(tO, tS + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : acc);
+                            if constexpr (SPLIT) {  // (the softmax takes every tile's output out)
+                                tc::mma_f16_ts(tO, tS + 16 * j, v + j * 128, kIdO, j > 0 ? 1u : 0u);
                                 tc::mma_f16_ts(tO, tS + 16 * j + 8, v + j * 128, kIdO, 1u);
                             } else {
                                 tc::mma_f16_ts(tO, tS + 8 * j, v + j * 128, kIdO, j > 0 ? 1u : acc);
@@ -773,25 +770,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 ++n_s;
                 tc::fence_after_sync();
                 const int32_t from = low - static_cast<int32_t>(t * kTile), to = at - static_cast<int32_t>(t * kTile);  // columns (from, to]
-                const bool masked = __any_sync(0xffffffffu, live && (from >= 0 || to < static_cast<int32_t>(kTile) - 1));
-                auto hide = [&](auto& x, int col0) {
+                if (__any_sync(0xffffffffu, live && (from >= 0 || to < static_cast<int32_t>(kTile) - 1))) {
+                    // Scores of keys that a row does not see become -infinity where they lie, in a rolled loop over the blocks
+                    // that need it: few tiles do, and the loop that every tile runs through stays short.
+#pragma unroll 1
+                    for (int32_t col = 0; col < static_cast<int32_t>(kTile); col += 16) {
+                        if (!__any_sync(0xffffffffu, live && (col <= from || col + 15 > to))) continue;
+                        uint32_t x[16];
+                        tc::tmem_ld16(tS + col, x);
+                        tc::tmem_wait_ld();
 #pragma unroll
-                    for (int u = 0; u < static_cast<int>(sizeof(x) / 4); ++u)
-                        if (col0 + u <= from || col0 + u > to) x[u] = 0xff800000u;
-                };
+                        for (int u = 0; u < 16; ++u)
+                            if (col + u <= from || col + u > to) x[u] = 0xff800000u;
+                        tc::tmem_st16(tS + col, x);
+                    }
+                    tc::tmem_wait_st();
+                }
                 if constexpr (SPLIT) {
-                    // The tensor core cuts its sums short of a rounding, which adds up over a long accumulation: after every
-                    // kFlush tiles the output is taken out of tensor memory and added here, and the scores are read twice to
-                    // make room for it.
-                    const bool fresh = turn % kFlush == 0;
-                    if (fresh && turn != 0) take_output();
+                    // The tensor core cuts its sums short of a rounding, which adds up over a long accumulation (2.8e-6 of the
+                    // norm at 2048 keys, against 0.8e-6): every tile's output is taken out of tensor memory and added here,
+                    // and the scores are read twice to make room for it.
+                    if (turn != 0) take_output();
                     float mx = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t x[32];
                         tc::tmem_ld32(tS + 32 * j, x);
                         tc::tmem_wait_ld();
-                        if (masked) hide(x, 32 * j);
                         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int u = 0; u < 32; u += 4) {
@@ -806,7 +811,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         const float f = grow ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
 #pragma unroll
                         for (int u = 0; u < D; ++u) acc[u] *= f;
-                        if (!fresh) rescale_output(f);
                         if (grow) m = mx;
                         l *= f;
                     }
@@ -818,7 +822,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         uint32_t x[32];
                         tc::tmem_ld32(tS + 32 * j, x);
                         tc::tmem_wait_ld();
-                        if (masked) hide(x, 32 * j);
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {  // 16 keys: high terms in their columns 0-7, low terms in 8-15
                             uint32_t y[16];
@@ -843,10 +846,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
 #pragma unroll
                     for (int j = 0; j < 4; ++j) tc::tmem_ld32(tS + 32 * j, x[j]);
                     tc::tmem_wait_ld();
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) hide(x[j], 32 * j);
-                    }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int u = 0; u < 32; u += 2)
