@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (uint32_t i = 0; i < NST; ++i) {
             tc::mbar_init(bar_full + 8 * i, 1);
-            tc::mbar_init(bar_empty + 8 * i, 2);
+            tc::mbar_init(bar_empty + 8 * i, 2);  // both streams
         }
         for (uint32_t i = 0; i < 2; ++i) {
             tc::mbar_init(bar_s + 8 * i, 1);
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             constexpr uint32_t kIdO = tc::instr_desc_f16(128, D, true) | kType;
             constexpr uint64_t kDescK = tc::smem_desc_base(16, 1024), kDescV = tc::smem_desc_base(Sh::kPanel, 1024);
             const uint32_t tS = tmem + i * kTile, tO = tmem + kTmemO + i * D;
-            uint32_t base = 0;  // the ring's count at the item's first tile
+            uint32_t base = 0, next = 0;  // the ring's count at the item's first tile; the next place to pass
             uint32_t n_p = 0, n_items = 0, mine = 0, turns = 0;  // turns: the other stream's rounds of the cells before
             auto wait_round = [&](uint32_t n) -> bool {  // until the other stream has issued its round n
                 if (static_cast<int32_t>(issued[1 - i] - n) > 0) return true;
@@ -554,13 +554,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             Item& it = items[4 + i];
             do {
                 const uint32_t t0 = it.t0, step = it.step, twin = it.twin, a = it.a[i], e = it.e[i];
-                const uint32_t oa = twin != 0 ? e : it.a[1 - i], oe = twin != 0 ? 0u : it.e[1 - i];  // tiles the other stream reads too
                 const uint64_t q = kDescK + ((qbuf + (twin != 0 ? 0u : i * Sh::kQ)) >> 4);
-                auto full = [&](uint32_t cn) { return wait(bar_full + 8 * (cn % NST), (cn / NST) & 1u); };
-                auto release = [&](uint32_t cn, uint32_t t) {  // a stage is free after two of these
-                    tc::mma_commit(bar_empty + 8 * (cn % NST));
-                    if (t < oa || t >= oe) tc::mma_commit(bar_empty + 8 * (cn % NST));
+                // Every place of the ring goes through both threads' hands, in order: a tile that this stream does not take is
+                // waited for and released too, so that no stage's barrier can run two phases ahead of a thread that tells
+                // phases by their parity.
+                auto reach = [&](uint32_t cn) -> bool {
+                    for (; next != cn; ++next) {
+                        if (!wait(bar_full + 8 * (next % NST), (next / NST) & 1u)) return false;
+                        mbar_arrive(bar_empty + 8 * (next % NST));
+                    }
+                    return true;
                 };
+                auto full = [&](uint32_t cn) -> bool {
+                    if (!reach(cn) || !wait(bar_full + 8 * (cn % NST), (cn / NST) & 1u)) return false;
+                    ++next;
+                    return true;
+                };
+                auto release = [&](uint32_t cn) { tc::mma_commit(bar_empty + 8 * (cn % NST)); };  // once its products are complete
                 auto scores = [&](uint32_t cn) {  // S = Q K(t)
                     const uint64_t k = kDescK + ((ring + cn % NST * Sh::kStage) >> 4);
 #pragma unroll
@@ -607,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         }
                         ++n_p;
                         if (!kAhead && twin != 0) {
-                            release(cv, t);
+                            release(cv);
                             if (ok && more) ok = full(ck);
                         }
                     }
@@ -616,15 +626,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         tc::fence_after_sync();
                         scores(ck);
                         tc::mma_commit(bar_s + 8 * i);
-                        release(ck, nt);
+                        release(ck);
                     } else {
                         issued[i] = ++mine;
                         tc::mma_commit(bar_o + 8 * i);
                     }
-                    if (have && (kAhead || twin == 0)) release(cv, t);
+                    if (have && (kAhead || twin == 0)) release(cv);
                     if (!more) break;
                 }
                 base += 2 * (it.t1 - t0);
+                ok = ok && reach(base);
                 turns += rounds;
                 ++n_items;
                 run.next(it);
