@@ -16,7 +16,7 @@ namespace itk {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // (8192 rows x 64 heads of 128 bf16 channels: 46.5 us, with 256 threads 51.5)
 constexpr int kAhead = 2;  // heads of a thread requested before the angles are there
 
 struct RopeLaunch {
@@ -108,8 +108,51 @@ __device__ __forceinline__ void wide_turn(const Wide<T>& w, O* row, uint32_t ite
     o.set(g);
     o.store(row + c + half);
 }
-// One pair, or one copied channel, at a time: for half-split pairs whose halves are not multiples of eight channels,
-// and rows that 16-byte words cannot address.
+// How a kernel goes through a head row: kWide as above; kWhole for half-split pairs whose halves are not multiples of eight
+// channels - a warp takes whole rows (as many as its lanes cover, eight channels a lane) by way of shared memory, where
+// partners lie at any distance (8192 x 64 rows of 62 rotated channels: 178 us pair by pair); kNarrow, one pair or one copied channel at
+// a time, for rows that 16-byte words cannot address.
+enum Mode { kWide, kWhole, kNarrow };
+constexpr int kWarps = kThreads / 32;
+
+// Lanes of kWhole read eight elements apart: one place more for every eight spreads them over the banks.
+__device__ __forceinline__ uint32_t skew(uint32_t i) { return i + i / 8; }
+constexpr uint32_t kSkewedDim = kMaxHeadDim + kMaxHeadDim / 8;
+
+// Lane `item` of a row's head_dim / 8; `row` holds the head row in f32.  The whole warp calls it, `active` lanes work.
+template <typename T, typename O>
+__device__ __forceinline__ void whole_turn(const T* src, O* dst, bool active, uint32_t item, uint32_t half, const float2* cs, float* row) {
+    Vec8<T> v = {};
+    float f[8];
+    if (active) {
+        v.load(src + 8 * item);
+        v.get(f);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) row[skew(8 * item) + j] = f[j];
+    }
+    __syncwarp();
+    if (active) {
+        if (8 * item >= 2 * half) {
+            copy8(v, dst + 8 * item);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                const uint32_t c = 8 * item + j;
+                const bool first = c < half;
+                if (c < 2 * half) {
+                    const float2 t = cs[skew(first ? c : c - half)];
+                    const float other = row[skew(first ? c + half : c - half)];
+                    f[j] = f[j] * t.x + (first ? -other : other) * t.y;
+                }
+            }
+            Vec8<O> o;
+            o.set(f);
+            o.store(dst + 8 * item);
+        }
+    }
+    __syncwarp();
+}
+
 template <typename T, typename O>
 __device__ __forceinline__ void narrow_turn(const T* src, O* dst, uint32_t item, uint32_t half, uint32_t pairing,
                                             const float2* cs) {
@@ -127,26 +170,35 @@ __device__ __forceinline__ void narrow_turn(const T* src, O* dst, uint32_t item,
     }
 }
 
-template <typename T, bool WIDE>
+template <typename T, Mode M>
 __global__ void __launch_bounds__(kThreads) rope_apply_kernel(const __grid_constant__ RopeLaunch p) {
-    __shared__ float2 cs[kMaxHeadDim / 2];
+    __shared__ float2 cs[kSkewedDim / 2];
+    __shared__ float whole[M == kWhole ? kWarps : 1][M == kWhole ? kSkewedDim : 1];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    const uint32_t step = kThreads / p.items;  // heads the CTA works on at a time
+    const uint32_t step = max(kThreads / p.items, 1u);  // heads the CTA works on at a time (one, when it has more items than threads)
     const uint32_t item = tid % p.items, h0 = tid / p.items;
     const T* src = static_cast<const T*>(p.x) + row * p.x_row;
     T* dst = static_cast<T*>(p.out) + row * p.o_row;
     Wide<T> ahead[kAhead];
     after_predecessor();
-    if constexpr (WIDE) {
+    if constexpr (M == kWide) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (h0 < step && h0 + j * step < p.heads) wide_load(ahead[j], src + (h0 + j * step) * p.x_head, item, p.half, p.pairing);
     }
     const double pos = static_cast<double>(p.positions[row]);
-    for (uint32_t i = tid; i < p.half; i += kThreads) cs[i] = turn_of(pos, p.inv_freq[i], p.magnitude, p.sign);
+    for (uint32_t i = tid; i < p.half; i += kThreads) cs[M == kWhole ? skew(i) : i] = turn_of(pos, p.inv_freq[i], p.magnitude, p.sign);
     __syncthreads();
+    if constexpr (M == kWhole) {
+        const uint32_t lane = tid & 31, at_once = 32 / p.items, sub = lane / p.items, u = lane % p.items;
+        for (uint32_t first = (tid >> 5) * at_once; first < p.heads; first += kWarps * at_once) {
+            const uint32_t h = first + sub;
+            whole_turn(src + h * p.x_head, dst + h * p.o_head, sub < at_once && h < p.heads, u, p.half, cs, whole[tid >> 5] + (sub < at_once ? sub : 0u) * skew(p.head_dim));
+        }
+        return;
+    }
     if (h0 >= step) return;
-    if constexpr (WIDE) {
+    if constexpr (M == kWide) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (h0 + j * step < p.heads) wide_turn(ahead[j], dst + (h0 + j * step) * p.o_head, item, p.half, p.pairing, cs);
@@ -156,7 +208,8 @@ __global__ void __launch_bounds__(kThreads) rope_apply_kernel(const __grid_const
             wide_turn(w, dst + h * p.o_head, item, p.half, p.pairing, cs);
         }
     } else {
-        for (uint32_t h = h0; h < p.heads; h += step) narrow_turn(src + h * p.x_head, dst + h * p.o_head, item, p.half, p.pairing, cs);
+        for (uint32_t h = h0; h < p.heads; h += step)
+            for (uint32_t u = item; u < p.items; u += kThreads) narrow_turn(src + h * p.x_head, dst + h * p.o_head, u, p.half, p.pairing, cs);
     }
 }
 
@@ -174,13 +227,14 @@ struct AppendRows {
 };
 
 // T: rows, P: pages.  Heads are counted through: the q_heads of q first (none without q), then K's, then V's.
-template <typename T, typename P, bool WIDE>
+template <typename T, typename P, Mode M>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_constant__ AppendRows p) {
-    __shared__ float2 cs[kMaxHeadDim / 2];
+    __shared__ float2 cs[kSkewedDim / 2];
+    __shared__ float whole[M == kWhole ? kWarps : 1][M == kWhole ? kSkewedDim : 1];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const uint32_t D = p.pool.head_dim, hq = p.q_heads, hkv = p.pool.kv_heads;
     const uint32_t heads = hq + 2 * hkv;
-    const uint32_t step = kThreads / p.items;
+    const uint32_t step = max(kThreads / p.items, 1u);
     const uint32_t item = tid % p.items, h0 = tid / p.items;
     const T* q = static_cast<const T*>(p.q) + row * p.q_row;
     const T* k = static_cast<const T*>(p.k) + row * p.k_row;
@@ -188,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
     auto source = [&](uint32_t h) { return h < hq ? q + h * D : h < hq + hkv ? k + (h - hq) * D : v + (h - hq - hkv) * D; };
     Wide<T> ahead[kAhead];
     after_predecessor();
-    if constexpr (WIDE) {
+    if constexpr (M == kWide) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (h0 < step && h0 + j * step < heads) wide_load(ahead[j], source(h0 + j * step), item, p.half, p.pairing);
@@ -216,8 +270,30 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
     P* const kp = static_cast<P*>(p.pool.k) + at;
     P* const vp = static_cast<P*>(p.pool.v) + at;
     T* const qo = static_cast<T*>(p.q_out) + row * p.q_out_row;
-    for (uint32_t i = tid; i < p.half; i += kThreads) cs[i] = turn_of(static_cast<double>(pos), p.inv_freq[i], p.magnitude, 1.f);
+    for (uint32_t i = tid; i < p.half; i += kThreads) cs[M == kWhole ? skew(i) : i] = turn_of(static_cast<double>(pos), p.inv_freq[i], p.magnitude, 1.f);
     __syncthreads();
+    if constexpr (M == kWhole) {
+        const uint32_t lane = tid & 31, at_once = 32 / p.items, sub = lane / p.items, u = lane % p.items;
+        float* const mine = whole[tid >> 5] + (sub < at_once ? sub : 0u) * skew(D);
+        const uint32_t turned = hq + hkv;
+        for (uint32_t first = (tid >> 5) * at_once; first < turned; first += kWarps * at_once) {  // (Q and K rows in one go: a
+            const uint32_t h = first + sub;                                                      // warp's rows may be of both)
+            const bool active = sub < at_once && h < turned && (h < hq || stored);
+            if constexpr (sizeof(T) == sizeof(P)) {
+                whole_turn(source(h < turned ? h : 0u), h < hq ? reinterpret_cast<P*>(qo + h * D) : kp + (h - hq) * p.pool.head_stride, active, u, p.half, cs, mine);
+            } else {
+                whole_turn(source(h < turned ? h : 0u), qo + h * D, active && h < hq, u, p.half, cs, mine);
+                whole_turn(source(h < turned ? h : 0u), kp + (h - hq) * p.pool.head_stride, active && h >= hq, u, p.half, cs, mine);
+            }
+        }
+        if (stored)
+            for (uint32_t i = tid; i < hkv * p.items; i += kThreads) {
+                Vec8<T> x;
+                x.load(v + 8 * i);  // (a token's heads are contiguous)
+                copy8(x, vp + (i / p.items) * p.pool.head_stride + 8 * (i % p.items));
+            }
+        return;
+    }
     if (h0 >= step) return;
     auto put = [&](uint32_t h, const Wide<T>& w) {
         if (h < hq) {
@@ -233,7 +309,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
             }
         }
     };
-    if constexpr (WIDE) {
+    if constexpr (M == kWide) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (h0 + j * step < heads) put(h0 + j * step, ahead[j]);
@@ -244,27 +320,37 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
         }
     } else {
         for (uint32_t h = h0; h < heads; h += step) {
-            if (h < hq) {
-                narrow_turn(source(h), qo + h * D, item, p.half, p.pairing, cs);
+            const T* src = source(h);
+            if (h < hq + hkv) {
+                if (h >= hq && !stored) continue;
+                for (uint32_t u = item; u < p.items; u += kThreads) {
+                    if (h < hq)
+                        narrow_turn(src, qo + h * D, u, p.half, p.pairing, cs);
+                    else
+                        narrow_turn(src, kp + (h - hq) * p.pool.head_stride, u, p.half, p.pairing, cs);
+                }
             } else if (stored) {
-                if (h < hq + hkv) {
-                    narrow_turn(source(h), kp + (h - hq) * p.pool.head_stride, item, p.half, p.pairing, cs);
-                } else {
-                    const T* src = source(h);
-                    P* dst = vp + (h - hq - hkv) * p.pool.head_stride;
-                    for (uint32_t c = item; c < D; c += p.items) dst[c] = from_f32<P>(to_f32(src[c]));
+                P* dst = vp + (h - hq - hkv) * p.pool.head_stride;
+                const uint32_t across = min(p.items, static_cast<uint32_t>(kThreads));
+                for (uint32_t c = item; c < D; c += across) {
+                    if constexpr (sizeof(T) == sizeof(P))
+                        dst[c] = src[c];
+                    else
+                        dst[c] = from_f32<P>(to_f32(src[c]));
                 }
             }
         }
     }
 }
 
-// Items of a head row, and whether they may be eight channels wide.
-uint32_t wide_items(uint32_t head_dim, uint32_t half, uint32_t pairing) {
-    return pairing == 0 ? head_dim / 8 : half / 8 + (head_dim - 2 * half) / 8;
+// The way through rows that sixteen-byte words can address or not, and its items per head row.
+Mode mode_of(bool words, uint32_t head_dim, uint32_t half, uint32_t pairing) {
+    if (!words || head_dim % 8 != 0) return kNarrow;
+    return pairing == 0 || half % 8 == 0 ? kWide : kWhole;
 }
-bool wide_fits(uint32_t head_dim, uint32_t half, uint32_t pairing) {
-    return head_dim % 8 == 0 && (pairing == 0 || half % 8 == 0);
+uint32_t items_of(Mode m, uint32_t head_dim, uint32_t half, uint32_t pairing) {
+    if (m == kNarrow) return half + (head_dim - 2 * half);
+    return m == kWide && pairing != 0 ? half / 8 + (head_dim - 2 * half) / 8 : head_dim / 8;
 }
 
 }  // namespace
@@ -407,9 +493,9 @@ extern "C" int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* e
     if (d->x == d->out && ((R > 1 && d->x_row_stride != d->out_row_stride) || (H > 1 && d->x_head_stride != d->out_head_stride)))
         return e.invalid("a rotation in place needs the strides of x and out to be the same");
     const uint32_t half = d->rotary_dim / 2;
-    // Sixteen-byte words: the halves, the head row and every stride are whole words of eight channels.
-    const bool wide = wide_fits(d->head_dim, half, d->pairing) && aligned16(d->x) && aligned16(d->out) &&
-                      ((R == 1 ? 0 : st[0] | st[2]) | (H == 1 ? 0 : st[1] | st[3])) % 8 == 0;
+    // Sixteen-byte words: every row starts on one.
+    const bool words = aligned16(d->x) && aligned16(d->out) && ((R == 1 ? 0 : st[0] | st[2]) | (H == 1 ? 0 : st[1] | st[3])) % 8 == 0;
+    const Mode mode = mode_of(words, d->head_dim, half, d->pairing);
     RopeLaunch p{};
     p.x = d->x;
     p.out = d->out;
@@ -423,7 +509,7 @@ extern "C" int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* e
     p.head_dim = d->head_dim;
     p.half = half;
     p.pairing = d->pairing;
-    p.items = wide ? wide_items(d->head_dim, half, d->pairing) : half + (d->head_dim - 2 * half);
+    p.items = items_of(mode, d->head_dim, half, d->pairing);
     p.magnitude = d->magnitude;
     p.sign = d->inverse ? -1.f : 1.f;
     const DeviceScope scope(d->device);
@@ -431,12 +517,11 @@ extern "C" int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* e
     const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
     auto launch = [&](auto kernel) { err = launch_dependent(kernel, d->rows, kThreads, 0, s, p); };
-    if (d->dtype == ITK_ROW_F32)
-        wide ? launch(rope_apply_kernel<float, true>) : launch(rope_apply_kernel<float, false>);
-    else if (d->dtype == ITK_ROW_F16)
-        wide ? launch(rope_apply_kernel<__half, true>) : launch(rope_apply_kernel<__half, false>);
-    else
-        wide ? launch(rope_apply_kernel<__nv_bfloat16, true>) : launch(rope_apply_kernel<__nv_bfloat16, false>);
+    auto by_mode = [&](auto row) {
+        using T = decltype(row);
+        mode == kWide ? launch(rope_apply_kernel<T, kWide>) : mode == kWhole ? launch(rope_apply_kernel<T, kWhole>) : launch(rope_apply_kernel<T, kNarrow>);
+    };
+    d->dtype == ITK_ROW_F32 ? by_mode(float()) : d->dtype == ITK_ROW_F16 ? by_mode(__half()) : by_mode(__nv_bfloat16());
     return err == cudaSuccess ? 0 : e.cuda("rotate launch failed", err);
 }
 
@@ -461,7 +546,7 @@ extern "C" int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* b
     const uintptr_t starts = reinterpret_cast<uintptr_t>(d->k_new) | reinterpret_cast<uintptr_t>(d->v_new) |
                              reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->q_out);
     if (starts % size != 0) return e.invalid("rows must be aligned to their element type");
-    const uint64_t kv_width = static_cast<uint64_t>(kv->kv_heads) * kv->head_dim, q_width = static_cast<uint64_t>(d->q_heads) * kv->head_dim;
+    const uint64_t q_width = static_cast<uint64_t>(d->q_heads) * kv->head_dim;
     const uint64_t st[4] = {d->k_row_stride, d->v_row_stride, with_q ? d->q_row_stride : 0, with_q ? d->q_out_row_stride : 0};
     for (uint64_t s : st)
         if (s >= kMaxStride) return e.invalid("row stride %llu is too large", s);
@@ -469,7 +554,6 @@ extern "C" int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* b
         return e.invalid("rows of q_out overlap (row stride %llu, %llu elements)", d->q_out_row_stride, q_width);
     if (with_q && d->q == d->q_out && batch->total_rows > 1 && d->q_row_stride != d->q_out_row_stride)
         return e.invalid("a rotation in place needs the strides of q and q_out to be the same");
-    (void)kv_width;
     if (batch->total_rows == 0) return 0;
     p.q = d->q;
     p.q_out = d->q_out;
@@ -484,20 +568,19 @@ extern "C" int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* b
     p.half = rot / 2;
     p.pairing = d->pairing;
     p.magnitude = d->magnitude;
-    const bool wide = wide_fits(kv->head_dim, p.half, p.pairing) && starts % 16 == 0 &&
-                      (batch->total_rows == 1 || (st[0] | st[1] | st[2] | st[3]) % 8 == 0);
-    p.items = wide ? wide_items(kv->head_dim, p.half, p.pairing) : p.half + (kv->head_dim - 2 * p.half);
+    const bool words = starts % 16 == 0 && (batch->total_rows == 1 || (st[0] | st[1] | st[2] | st[3]) % 8 == 0);
+    const Mode mode = mode_of(words, kv->head_dim, p.half, p.pairing);
+    p.items = items_of(mode, kv->head_dim, p.half, p.pairing);
     const DeviceScope scope(kv->device);
     if (scope.err != cudaSuccess) return e.cuda("paged append: the device cannot be used", scope.err);
     const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     cudaError_t err = cudaSuccess;
     auto launch = [&](auto kernel) { err = launch_dependent(kernel, batch->total_rows, kThreads, 0, s, p); };
-    if (d->dtype == ITK_ROW_F32)
-        wide ? launch(paged_append_kernel<float, __half, true>) : launch(paged_append_kernel<float, __half, false>);
-    else if (d->dtype == ITK_ROW_F16)
-        wide ? launch(paged_append_kernel<__half, __half, true>) : launch(paged_append_kernel<__half, __half, false>);
-    else
-        wide ? launch(paged_append_kernel<__nv_bfloat16, __nv_bfloat16, true>)
-             : launch(paged_append_kernel<__nv_bfloat16, __nv_bfloat16, false>);
+    auto by_mode = [&](auto row, auto page) {
+        using T = decltype(row);
+        using P = decltype(page);
+        mode == kWide ? launch(paged_append_kernel<T, P, kWide>) : mode == kWhole ? launch(paged_append_kernel<T, P, kWhole>) : launch(paged_append_kernel<T, P, kNarrow>);
+    };
+    d->dtype == ITK_ROW_F32 ? by_mode(float(), __half()) : d->dtype == ITK_ROW_F16 ? by_mode(__half(), __half()) : by_mode(__nv_bfloat16(), __nv_bfloat16());
     return err == cudaSuccess ? 0 : e.cuda("paged append launch failed", err);
 }
