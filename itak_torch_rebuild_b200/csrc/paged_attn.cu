@@ -96,11 +96,22 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     p.tickets = reinterpret_cast<unsigned int*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + l.ml);
     p.part_o = reinterpret_cast<float*>(ws + l.o);
-    // Few pairs per KV head stream, many go to tensor memory.
+    // Few (row, head) pairs per KV head stream, many go to tensor memory.  Measured at 2055-2487 keys, 32 / 8 heads of 128
+    // channels (streaming : tensor memory, us):
+    //   16-bit rows, 16 pairs   16 sequences 37 : 53     2 sequences 17 : 19
+    //                28 pairs   16 sequences 49 : 54     8 sequences 40 : 37     2 sequences 28 : 19
+    //                48 pairs   16 sequences 75 : 54     2 sequences 32 : 21
+    //   f32 rows,    28 pairs   16 sequences 69 : 94     2 sequences 23 : 29
+    //                48 pairs   16 sequences 98 : 96     2 sequences 27 : 31
+    //                64 pairs   16 sequences 125 : 96    2 sequences 30 : 32
+    // Between 17 and 32 pairs of 16-bit rows what counts is how many CTAs share a cell, since the streaming kernel's joins
+    // are the slower ones: it takes them when there is a cell (sequence and KV head) for two of three multiprocessors.
     const uint64_t pairs = static_cast<uint64_t>(d->max_rows < batch->total_rows ? d->max_rows : batch->total_rows) * p.group;
-    const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     const uint32_t narrow = stream_pairs(d->dtype);
-    const cudaError_t err = pairs > 2 * narrow && tc_takes(p.pool) ? launch_tc(p, d->dtype, sms, s)
-                                                                   : launch_stream(p, d->dtype, pairs > narrow, sms, s);
+    const bool many_cells = static_cast<uint64_t>(batch->n_seqs) * kv->kv_heads * 3 >= sms * 2ull;
+    const uint64_t streams = d->dtype == ITK_ROW_F32 ? 48 : many_cells ? 32 : 16;
+    const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    const cudaError_t err = pairs > streams && tc_takes(p.pool) ? launch_tc(p, d->dtype, sms, s)
+                                                                : launch_stream(p, d->dtype, pairs > narrow, sms, s);
     return err == cudaSuccess ? 0 : e.cuda("paged attention launch failed", err);
 }
