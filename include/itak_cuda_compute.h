@@ -480,8 +480,9 @@ int itk_decode_attention_noalloc(const void* k_layer, const void* v_layer, uint3
  * into a graph follows them from replay to replay.  No counterpart in the reference, whose cache is one slot per
  * session (crates/wgpu-compute/src/session.rs:235-249).  Like itk_draft_attention these calls take no backend handle:
  * they queue work on `cuda_stream` (NULL = the default stream of `device`), allocate nothing, keep nothing between
- * calls, may be captured, and report a refusal through error_text.  They run on the device the structure names,
- * whichever is current.  Head rows are head_dim contiguous elements; strides count elements.
+ * calls, may be captured (the first call of a kind on a device loads its kernel: make that one outside a capture), and
+ * report a refusal through error_text.  They run on the device the structure names, whichever is current, and are launched
+ * as programmatic dependents of what precedes them in the stream.  Head rows are head_dim contiguous elements; strides count elements.
  *
  * Element types of rows: f32 rows go with f16 pages (rounded to nearest even on append, NaN -> sign|0x7e00), f16 rows
  * with f16 pages, bf16 rows with bf16 pages. */
@@ -536,7 +537,7 @@ int itk_rope_apply(const itk_rope_desc* d, void* cuda_stream, char* error_text, 
 
 /* The pools: element (page, head, row, channel) of K at page * page_stride + head * head_stride + row * row_stride +
  * channel, V alike.  Both [page][kv_head][row][D] and [page][row][kv_head][D] are such layouts.  Pools start on a
- * 16-byte boundary and strides are multiples of 8. */
+ * 16-byte boundary and strides are multiples of 8; up to 2^31 - 1 pages. */
 typedef struct itk_paged_kv {
     void* k;
     void* v;
@@ -597,7 +598,10 @@ int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* batch, const
  * what lies outside a sequence's keys never reaches a result.
  *
  * `workspace`: device memory of itk_paged_attention_workspace() bytes, 256-byte aligned, that must be zero before its
- * first use; every call leaves what it needs of it zero again.  Calls that may run at the same time need one each. */
+ * first use; every call leaves what it needs of it zero again (after a call that raised bit 4 of *status the caller clears
+ * it).  Calls that may run at the same time need one each.
+ *
+ * The same call gives the same bits: partial results of a key range that several CTAs shared are joined in one order. */
 typedef struct itk_paged_attention_desc {
     const void* q; /* [total_rows][q_heads][head_dim] */
     void* out;     /* as q, same type */

@@ -89,6 +89,14 @@ struct AttnParams {
     float* part_o;          // [part][row][D]: unnormalised outputs
 };
 
+// Takes a ticket: orders the block's stores before it (all of them precede a barrier that the caller has passed) and what
+// the block reads behind a further barrier after it, with one instruction of one thread.
+__device__ __forceinline__ uint32_t take_ticket(unsigned int* counter) {
+    uint32_t ticket;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(ticket) : "l"(counter) : "memory");
+    return ticket;
+}
+
 // ---- element types ------------------------------------------------------------------------------------------------
 
 // Eight consecutive channels of a row as they travel: two 16-byte words of f32, one of a 16-bit type.
@@ -247,8 +255,9 @@ cudaError_t launch_dependent(void (*kernel)(Params...), uint32_t grid, uint32_t 
     return e != cudaSuccess ? e : last;
 }
 
-constexpr uint64_t kMaxStride = 1ull << 40;
+constexpr uint64_t kMaxStride = 1ull << 38;
 
+inline bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Refusals that append and attention share; 0 when the pools and the batch can be used.

@@ -67,6 +67,7 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
         return e.invalid("total_rows x q_heads = %llu is too large", static_cast<uint64_t>(batch->total_rows) * d->q_heads);
     if (!isfinite(d->scale)) return e.invalid("the scale must be finite");
     if (!d->q || !d->out || !d->workspace) return e.invalid("null pointer argument");
+    if (!aligned_to(d->lse, 4)) return e.invalid("lse must be aligned to 4 bytes");
     if (!aligned16(d->q) || !aligned16(d->out)) return e.invalid("q and out must start on a 16-byte boundary");
     const uint64_t width = static_cast<uint64_t>(d->q_heads) * kv->head_dim;
     if (d->q_row_stride % 8 != 0 || d->out_row_stride % 8 != 0 || d->q_row_stride >= kMaxStride || d->out_row_stride >= kMaxStride)

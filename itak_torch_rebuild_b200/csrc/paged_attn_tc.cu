@@ -13,15 +13,15 @@
 //   columns   0-127  S0, then in place its weights P0       columns 256-...  O0
 //   columns 128-255  S1, then P1                            columns 256 + D  O1
 //   more than 128 pairs: stream i holds pairs [128 i, 128 i + 128) of the block and takes every tile it sees;
-//   128 pairs or fewer:  both hold the same pairs, stream i takes every second tile, and the two are joined at the end -
-//                        otherwise the tensor core and the loads would wait for one softmax after every tile.
-// One thread issues all products, in the order O_i += P_i V(t), S_i = Q_i K(t + 1), the other stream's, ...: products
+//   128 pairs or fewer ("twin"): both hold the same pairs, stream i takes every second tile, and the two are joined at the
+//                        end - otherwise tensor core and loads would wait for one softmax after every tile.
+// One thread per stream issues its products, O += P V(t) and then S = Q K(t + 1), and the two take turns; a thread's products
 // complete in order, so S may overwrite the weights of the tile before without a barrier of its own, and scores that are
 // complete vouch for every product issued before them.
 //
-// Warps 0-3 and 4-7: softmax of stream 0 and 1.  Warp 8: the products (one lane), tensor-memory allocation.  Warp 9: TMA
-// loads of K and V through one ring, K(t), V(t), K(t + 1), ...; a tile is fetched page by page, lane j taking one box
-// (64 channels of the rows that a page has in the tile), pages outside the keys of the block left out.  Score columns of
+// Warps 0-3 and 4-7: softmax of stream 0 and 1.  Warps 8 and 10: their products (one lane each); 8 allocates tensor memory.
+// Warp 9: TMA loads of K and V through one ring, K(t), V(t), K(t + 1), ...; a tile is fetched page by page, lane j taking one
+// box (64 channels of the rows that a page has in the tile), pages outside the keys of the block left out.  Score columns of
 // keys that a row does not see become -infinity whatever the tile holds there; V rows outside the block's keys are
 // overwritten with zeros in shared memory, since a weight of zero does not hide a NaN.
 //
@@ -32,7 +32,11 @@
 // maximum is used for weights and sum alike, so nothing is lost.
 //
 // Bound: a 128 x 128 tile of both products takes 1024 clocks on the tensor core (D = 128) and its 16384 exponentials 1024
-// clocks on the special-function units.
+// clocks on the special-function units.  A round (both products of a tile of one stream) takes about 1600: softmax and
+// products of one stream follow one another, and two streams do not quite cover that chain.  (2^x by a polynomial on the
+// multiply-add pipe for part of the weights made it longer.)  Measured: 4096 bf16 rows at 16384 keys, 32 / 8 heads of 128:
+// 797-900 us by the board's power state, 1.07-1.21 PFLOP/s of 1.66; 4 x 512 rows at 1024-2048 keys: f16 73 us, f32 157 us,
+// where a cell's end (3 tiles' time), the joins and 14000 clocks before the first tile count as much as the tiles.
 #include <cuda.h>
 
 #include <type_traits>
@@ -1015,8 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (last > first && last * per - cell0 + snap >= it.T) --last;  // ... and that one behind its end
                 both_sync();
                 if (tid == 0) {
-                    __threadfence();  // cumulative over the stores above (ordered before the barrier)
-                    const unsigned int ticket = atomicAdd(p.tickets + first, 1u);
+                    const uint32_t ticket = take_ticket(p.tickets + first);
                     word[1] = ticket == last - first ? 1u : 0u;
                     if (ticket == last - first) p.tickets[first] = 0u;  // as the next launch wants it
                 }
@@ -1025,7 +1028,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const uint32_t n_parts = last - first + 1;
                 auto slot_of = [&](uint32_t k) { return static_cast<size_t>(2 * (first + k) + (k == 0 ? 1 : 0)); };
                 if (word[1] != 0u && !dead) {
-                    __threadfence();
                     if (n_parts == 2) {
                         // Every thread joins its own row, its own part still in tensor memory - in the order of the parts,
                         // whichever of the two came last, so that the same call gives the same bits.

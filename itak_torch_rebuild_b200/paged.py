@@ -30,10 +30,22 @@ _ERROR_LEN = 256
 
 # A decode step's kernels run for a few microseconds, so the descriptors are packed in one go (filling a ctypes structure
 # takes six times as long); the layouts are those of _lib's structures.
-_PACK_ROPE = struct.Struct("8Q6I2if4x").pack
-_PACK_BATCH = struct.Struct("4Q4I").pack
-_PACK_APPEND = struct.Struct("9Q3Iif4x").pack
-_PACK_ATTENTION = struct.Struct("7Q3Iif4x").pack
+def _packer(layout: str):
+    pack = struct.Struct(layout).pack
+
+    def packed(*values) -> bytes:
+        try:
+            return pack(*values)
+        except (struct.error, OverflowError) as e:  # a value that its field cannot hold
+            _refuse(f"an argument is out of range: {e}")
+
+    return packed
+
+
+_PACK_ROPE = _packer("8Q6I2if4x")
+_PACK_BATCH = _packer("4Q4I")
+_PACK_APPEND = _packer("9Q3Iif4x")
+_PACK_ATTENTION = _packer("7Q3Iif4x")
 for _s, _f in ((_lib.RopeDesc, "8Q6I2if4x"), (_lib.PagedBatch, "4Q4I"), (_lib.PagedAppendDesc, "9Q3Iif4x"),
                (_lib.PagedAttentionDesc, "7Q3Iif4x")):
     assert C.sizeof(_s) == struct.calcsize(_f), _s
@@ -65,12 +77,6 @@ def _explain(fn, *args):
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _u32(**values):
-    for name, v in values.items():
-        if not 0 <= v <= 0xffffffff:
-            _refuse(f"{name} must be in 0..2^32 - 1, got {v}")
 
 
 def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
@@ -139,7 +145,6 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     o0, o1, o2 = out.stride()
     if x2 != 1 or o2 != 1:
         _refuse("the channels of x and out must be contiguous")
-    _u32(pairing=pairing)
     d = _PACK_ROPE(x.data_ptr(), out.data_ptr(), at, table, x0, x1, o0, o1, rows, heads, head_dim, 2 * inv_freq.shape[0], pairing,
                    1 if inverse else 0, dtype, dev, magnitude)
     fn = _entry("itk_rope_apply", 1)
@@ -233,7 +238,6 @@ class PagedKv:
         freq = rotary = 0
         if inv_freq is not None:
             freq, rotary = _vector(inv_freq, "inv_freq", torch.float64, None, dev), 2 * inv_freq.shape[0]
-        _u32(pairing=pairing)
         batch = self._batch(table, row_start, kv_len, rows, status)
         if rows == 0:  # torch gives empty tensors no address
             return q_out
@@ -268,7 +272,6 @@ class PagedKv:
             if lse.dtype is not torch.float32 or lse.get_device() != dev or lse.shape != (rows, q_heads) or not lse.is_contiguous():
                 _refuse(f"lse must be a contiguous {torch.float32} [{rows}][{q_heads}] tensor on device {dev}, got {lse.dtype} {tuple(lse.shape)} on {lse.device}")
             lse_at = lse.data_ptr()
-        _u32(window=window, max_rows=max_rows)
         stream = _raw_stream(dev) if stream is None else stream
         if workspace is None:
             if torch.cuda.is_current_stream_capturing():

@@ -585,7 +585,7 @@ def test_pool_objects_refuse_what_they_cannot_describe():
     i32 = dict(dtype=torch.int32, device="cuda")
     q, tab, st, ln = torch.zeros(2, 4, 64, dtype=F16, device="cuda"), torch.zeros(2, 3, **i32), torch.zeros(3, **i32), torch.zeros(2, **i32)
     for kw in (dict(q=q.bfloat16()), dict(q=q[..., :32]), dict(q=q.float().double()), dict(tab=tab.long()), dict(tab=tab[:1]), dict(st=st[:2]), dict(ln=ln.cpu()),
-               dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), dict(out=q[:1]), dict(lse=torch.zeros(2, 3, device="cuda")), dict(window=-1),
+               dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), dict(out=q[:1]), dict(lse=torch.zeros(2, 3, device="cuda")), dict(window=-1), dict(window=2 ** 32), dict(scale=1e300),
                dict(status=torch.zeros(1, device="cuda")), dict(workspace=torch.zeros(10, device="cuda")), dict(q=torch.zeros(2, 3, 64, dtype=F16, device="cuda"))):
         a = dict(q=q, tab=tab, st=st, ln=ln)
         a.update(kw)

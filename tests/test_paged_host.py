@@ -124,7 +124,7 @@ def rope(**kw):
     (dict(magnitude=math.inf), "magnitude"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(positions=None), "null"),
     (dict(inv_freq=None), "null"), (dict(x=P + 2), "aligned"), (dict(out_row_stride=255), "overlap"),
     (dict(out_head_stride=0), "overlap"), (dict(out_head_stride=32), "overlap"), (dict(x_row_stride=1 << 40), "large"),
-    (dict(out=P, out_row_stride=512), "in place"),
+    (dict(out=P, out_row_stride=512), "in place"), (dict(positions=P + 2), "aligned"), (dict(inv_freq=P + 4), "aligned"),
 ])
 def test_rotation_refusals(lib, kw, part):
     err = C.create_string_buffer(256)
@@ -172,13 +172,14 @@ POOL = [
     (dict(head_dim=264, row_stride=264), None, "multiple of 8"), (dict(page_size=0), None, "power of two"),
     (dict(page_size=24), None, "power of two"), (dict(page_size=1 << 17), None, "power of two"), (dict(dtype=_lib.ROW_F32), None, "pages hold"),
     (dict(k=None), None, "null"), (dict(v=P + 8), None, "16-byte"), (dict(row_stride=65), None, "multiples of 8"),
-    (dict(row_stride=56), None, "overlap"), (dict(head_stride=15 * 64), None, "overlap"), (dict(page_stride=31 * 64), None, "overlap"),
+    (dict(n_pages=1 << 31), None, "n_pages"), (dict(row_stride=56), None, "overlap"), (dict(head_stride=15 * 64), None, "overlap"), (dict(page_stride=31 * 64), None, "overlap"),
 ]
 BATCH = [
     (dict(table=None), None, "null"), (dict(row_start=None), None, "null"), (dict(kv_len=None), None, "null"),
     (dict(n_seqs=0), _lib.ERR_ZERO_DIMENSION, "n_seqs"), (dict(n_seqs=1025), _lib.ERR_CAPACITY, "sequences"),
     (dict(table_width=0), _lib.ERR_ZERO_DIMENSION, "table_width"), (dict(table_stride=1), None, "table_stride"),
-    (dict(total_rows=1 << 31), None, "total_rows"),
+    (dict(total_rows=1 << 31), None, "total_rows"), (dict(table=P + 2), None, "aligned"), (dict(row_start=P + 1), None, "aligned"),
+    (dict(kv_len=P + 2), None, "aligned"), (dict(status=P + 2), None, "aligned"),
 ]
 
 
@@ -196,7 +197,7 @@ def test_pool_and_batch_refusals(lib, call, which, kw, code, part):
     (dict(k_new=None), "null"), (dict(v_new=None), "null"), (dict(q_out=None), "go together"), (dict(q=None), "go together"),
     (dict(q_heads=0), "go together"), (dict(rotary_dim=33), "rotary_dim"), (dict(rotary_dim=66), "rotary_dim"), (dict(pairing=2), "pairing"),
     (dict(magnitude=math.nan), "magnitude"), (dict(dtype=_lib.ROW_BF16), "bf16 rows"), (dict(dtype=9), "element type"),
-    (dict(k_new=P + 1), "aligned"), (dict(q_out_row_stride=255), "overlap"), (dict(q_row_stride=512), "in place"),
+    (dict(k_new=P + 1), "aligned"), (dict(inv_freq=P + 4), "aligned"), (dict(q_out_row_stride=255), "overlap"), (dict(q_row_stride=512), "in place"),
 ])
 def test_append_refusals(lib, kw, part):
     err = C.create_string_buffer(256)
@@ -207,7 +208,7 @@ def test_append_refusals(lib, kw, part):
 @pytest.mark.parametrize("kw,code,part", [
     (dict(q_heads=0), _lib.ERR_ZERO_DIMENSION, "num_q_heads"), (dict(q_heads=3), _lib.ERR_NON_DIVISIBLE_HEADS, "divide evenly"),
     (dict(q=None), None, "null"), (dict(out=None), None, "null"), (dict(workspace=None), None, "null"), (dict(workspace=P + 16), None, "256-byte"),
-    (dict(q=P + 8), None, "16-byte"), (dict(scale=math.nan), None, "scale"), (dict(q_row_stride=260), None, "multiples of 8"),
+    (dict(q=P + 8), None, "16-byte"), (dict(lse=P + 2), None, "aligned"), (dict(scale=math.nan), None, "scale"), (dict(q_row_stride=260), None, "multiples of 8"),
     (dict(out_row_stride=248), None, "overlap"), (dict(dtype=_lib.ROW_BF16), None, "bf16 rows"),
 ])
 def test_attention_refusals(lib, kw, code, part):
