@@ -64,7 +64,7 @@ constexpr float kRescaleStep = 8.f;
 // one of them the join; a cut that would leave kSnap tiles at a cell's beginning or end moves there.
 constexpr uint32_t kCellCost = 3, kSnap = 1;
 constexpr uint32_t kSmemBytes = 232448;   // all that a block can have
-constexpr uint32_t kTailBytes = 3072;     // mbarriers, the roles' items, the streams' exchange
+constexpr uint32_t kTailBytes = 3u << 10;    // mbarriers, the roles' items, the streams' exchange
 constexpr long long kWaitClocks = 2000000000ll;  // about a second
 
 template <typename T>
