@@ -30,22 +30,11 @@ _ERROR_LEN = 256
 
 # A decode step's kernels run for a few microseconds, so the descriptors are packed in one go (filling a ctypes structure
 # takes six times as long); the layouts are those of _lib's structures.
-def _packer(layout: str):
-    pack = struct.Struct(layout).pack
-
-    def packed(*values) -> bytes:
-        try:
-            return pack(*values)
-        except (struct.error, OverflowError) as e:  # a value that its field cannot hold
-            _refuse(f"an argument is out of range: {e}")
-
-    return packed
-
-
-_PACK_ROPE = _packer("8Q6I2if4x")
-_PACK_BATCH = _packer("4Q4I")
-_PACK_APPEND = _packer("9Q3Iif4x")
-_PACK_ATTENTION = _packer("7Q3Iif4x")
+_PACK_ROPE = struct.Struct("8Q6I2if4x").pack
+_PACK_BATCH = struct.Struct("4Q4I").pack
+_PACK_APPEND = struct.Struct("9Q3Iif4x").pack
+_PACK_ATTENTION = struct.Struct("7Q3Iif4x").pack
+_OUT_OF_RANGE = (struct.error, OverflowError)  # a value that its field cannot hold
 for _s, _f in ((_lib.RopeDesc, "8Q6I2if4x"), (_lib.PagedBatch, "4Q4I"), (_lib.PagedAppendDesc, "9Q3Iif4x"),
                (_lib.PagedAttentionDesc, "7Q3Iif4x")):
     assert C.sizeof(_s) == struct.calcsize(_f), _s
@@ -79,6 +68,16 @@ def _explain(fn, *args):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _capturing(device: int, stream: int) -> bool:
+    """Whether ``stream`` of ``device`` is being captured, the current stream or not (the default one never is)."""
+    if stream == 0:
+        return False
+    if device == torch.cuda.current_device() and stream == _raw_stream(device):
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
     """The row stride of a ``[rows][heads][head_dim]`` tensor whose heads are contiguous."""
     if t.dtype is not dtype or t.get_device() != device:
@@ -95,7 +94,7 @@ def _vector(t: torch.Tensor, what: str, dtype, n: Optional[int], device: int) ->
     """The address of a contiguous vector of ``n`` elements (any number: ``None``)."""
     if t.dtype is not dtype or t.get_device() != device:
         _refuse(f"{what} must be {dtype} on device {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+    if t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
         _refuse(f"{what} must be a contiguous vector{'' if n is None else f' of {n} elements'}, got {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -145,8 +144,11 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     o0, o1, o2 = out.stride()
     if x2 != 1 or o2 != 1:
         _refuse("the channels of x and out must be contiguous")
-    d = _PACK_ROPE(x.data_ptr(), out.data_ptr(), at, table, x0, x1, o0, o1, rows, heads, head_dim, 2 * inv_freq.shape[0], pairing,
-                   1 if inverse else 0, dtype, dev, magnitude)
+    try:
+        d = _PACK_ROPE(x.data_ptr(), out.data_ptr(), at, table, x0, x1, o0, o1, rows, heads, head_dim, 2 * inv_freq.numel(), pairing,
+                       1 if inverse else 0, dtype, dev, magnitude)
+    except _OUT_OF_RANGE as e:
+        _refuse(f"an argument is out of range: {e}")
     fn = _entry("itk_rope_apply", 1)
     stream = _raw_stream(dev) if stream is None else stream
     if fn(d, stream, None, 0) != _lib.OK:
@@ -196,19 +198,24 @@ class PagedKv:
                                       self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], self._index))
 
     def _batch(self, table, row_start, kv_len, total_rows, status) -> bytes:
-        dev, n = self._index, kv_len.shape[0]
-        lens = _vector(kv_len, "kv_len", torch.int32, None, dev)
-        starts = _vector(row_start, "row_start", torch.int32, n + 1, dev)
-        if table.dtype is not torch.int32 or table.get_device() != dev:
-            _refuse(f"table must be {torch.int32} on device {dev}, got {table.dtype} on {table.device}")
-        if table.dim() != 2 or table.shape[0] != n or (table.stride(1) != 1 and table.shape[1] > 1):
-            _refuse(f"table must be [{n}][pages of a sequence] with contiguous rows, got {tuple(table.shape)}")
+        dev, n, i32 = self._index, kv_len.numel(), torch.int32
+        # one test of what is right; what is wrong is looked for afterwards
+        if (kv_len.dtype is not i32 or row_start.dtype is not i32 or table.dtype is not i32 or kv_len.get_device() != dev
+                or row_start.get_device() != dev or table.get_device() != dev or kv_len.dim() != 1 or row_start.dim() != 1
+                or table.dim() != 2 or row_start.numel() != n + 1 or not kv_len.is_contiguous() or not row_start.is_contiguous()):
+            _vector(kv_len, "kv_len", i32, None, dev)
+            _vector(row_start, "row_start", i32, n + 1, dev)
+            _refuse(f"table must be {i32} [{n}][pages of a sequence] on device {dev}, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        rows, width = table.shape
+        stride, inner = table.stride()
+        if rows != n or (inner != 1 and width > 1):
+            _refuse(f"table must be [{n}][pages of a sequence] with contiguous rows, got {(rows, width)}")
         word = 0
         if status is not None:
-            word = _vector(status, "status", torch.int32, None, dev)
+            word = _vector(status, "status", i32, None, dev)
             if status.numel() < 1:
                 _refuse("status must hold one element")
-        return _PACK_BATCH(table.data_ptr(), starts, lens, word, n, table.shape[1], table.stride(0), total_rows)
+        return _PACK_BATCH(table.data_ptr(), row_start.data_ptr(), kv_len.data_ptr(), word, n, width, stride, total_rows)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *,
                q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
@@ -218,8 +225,8 @@ class PagedKv:
         given.  f32 rows go into f16 pages, 16-bit rows into pages of their type (``itk_paged_append``)."""
         dev, d, dtype = self._index, self.head_dim, k.dtype
         row_dtype = _ROW_DTYPES.get(dtype)
-        if row_dtype is None:
-            _refuse(f"rows must be f32, f16 or bf16, got {dtype}")
+        if row_dtype is None or k.dim() != 3:
+            _refuse(f"rows must be f32, f16 or bf16 [rows][{self.kv_heads}][{d}], got {dtype} {tuple(k.shape)}")
         rows = k.shape[0]
         k_row = _rows(k, "k", rows, self.kv_heads, d, dtype, dev)
         v_row = _rows(v, "v", rows, self.kv_heads, d, dtype, dev)
@@ -237,12 +244,15 @@ class PagedKv:
             _refuse("q, q_out and q_heads go together")
         freq = rotary = 0
         if inv_freq is not None:
-            freq, rotary = _vector(inv_freq, "inv_freq", torch.float64, None, dev), 2 * inv_freq.shape[0]
+            freq, rotary = _vector(inv_freq, "inv_freq", torch.float64, None, dev), 2 * inv_freq.numel()
         batch = self._batch(table, row_start, kv_len, rows, status)
         if rows == 0:  # torch gives empty tensors no address
             return q_out
-        a = _PACK_APPEND(q_at, q_out_at, k.data_ptr(), v.data_ptr(), freq, q_row, q_out_row, k_row, v_row, q_heads, rotary, pairing,
-                         row_dtype, magnitude)
+        try:
+            a = _PACK_APPEND(q_at, q_out_at, k.data_ptr(), v.data_ptr(), freq, q_row, q_out_row, k_row, v_row, q_heads, rotary, pairing,
+                             row_dtype, magnitude)
+        except _OUT_OF_RANGE as e:
+            _refuse(f"an argument is out of range: {e}")
         fn = _entry("itk_paged_append", 3)
         stream = _raw_stream(dev) if stream is None else stream
         if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
@@ -274,7 +284,7 @@ class PagedKv:
             lse_at = lse.data_ptr()
         stream = _raw_stream(dev) if stream is None else stream
         if workspace is None:
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(dev, stream):
                 _refuse("a call that is being captured needs a workspace of its own (attention_workspace)")
             workspace = _workspaces.get((dev, stream))
             if workspace is None:
@@ -284,8 +294,11 @@ class PagedKv:
         batch = self._batch(table, row_start, kv_len, rows, status)
         if rows == 0:  # torch gives empty tensors no address
             return out
-        a = _PACK_ATTENTION(q.data_ptr(), out.data_ptr(), lse_at, workspace.data_ptr(), workspace.numel(), q_row, out_row, q_heads,
-                            max_rows, window, row_dtype, self._scale if scale is None else scale)
+        try:
+            a = _PACK_ATTENTION(q.data_ptr(), out.data_ptr(), lse_at, workspace.data_ptr(), workspace.numel(), q_row, out_row, q_heads,
+                                max_rows, window, row_dtype, self._scale if scale is None else scale)
+        except _OUT_OF_RANGE as e:
+            _refuse(f"an argument is out of range: {e}")
         fn = _entry("itk_paged_attention", 3)
         if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
             _explain(fn, self._kv, batch, a, stream)

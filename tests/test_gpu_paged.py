@@ -495,6 +495,29 @@ def test_a_captured_call_needs_a_workspace_of_its_own():
     assert "workspace" in e.value.msg
 
 
+def test_a_stream_given_by_number_that_is_being_captured_needs_a_workspace_too():
+    b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
+    out = torch.empty_like(b.q)
+    captured, current = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for s in (captured, current):  # each has a workspace of the module's
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=captured):
+        with torch.cuda.stream(current), pytest.raises(CudaComputeError) as e:
+            PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out, stream=captured.cuda_stream)
+    assert "workspace" in e.value.msg
+
+
+def test_rows_of_another_number_of_dimensions_are_refused():
+    b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
+    for k in (b.q[0, 0, 0], b.q[0], b.q[None]):
+        with pytest.raises(CudaComputeError):
+            PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len)
+        with pytest.raises(CudaComputeError):
+            PagedOf(b).attention(k, b.table, b.row_start, b.kv_len, max_rows=1)
+
+
 def test_a_workspace_that_is_too_small_is_refused():
     b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
     ws = paged.attention_workspace("cuda:0")
