@@ -19,9 +19,9 @@
 //           type (half a step of the output's own type, and averaged over the keys).  f32 rows: x = h + l with two
 //           halfs, so that 8 pairs take the 16 rows and scores and outputs come out f32-grade.
 //
-// Measured (us, share of the copy rate): one layer of 8 x 32768 keys, 64 / 8 heads of 128, f32 rows: 174 (0.96); 16 sequences
+// Measured (us, share of the copy rate): one layer of 8 x 32768 keys, 64 / 8 heads of 128, f32 rows: 167-177 (0.94-1.0); 16 sequences
 // of 256-8192 keys, bf16: 52 (0.82: 4.3 us until the first tile is there, 5-8 us of cell ends behind the stream); one sequence of
-// 4096 keys: 11.8, a chain of dependent steps (lengths, page numbers, keys, the warps' exchange, ticket, join).
+// 4096 keys: 11.4, a chain of dependent steps (lengths, page numbers, keys, the warps' exchange, ticket, join).
 #include <type_traits>
 
 #include "attn_common.cuh"
