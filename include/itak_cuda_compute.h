@@ -554,8 +554,9 @@ typedef struct itk_paged_kv {
  * included: its row i sits at position kv_len[s] - rows + i.  The key of position p is row p % page_size of page
  * table[s * table_stride + p / page_size].  All arrays are on the device and read when the work runs.
  * Contents are checked there: a page number outside the pool is never followed (its keys read as zeros, a row that
- * would be stored there is dropped) and raises bit 0 of *status; a length that the table has no columns for is cut to
- * them (bit 1); new rows that reach before position 0 see nothing and are not stored (bit 2); starts that run backwards
+ * would be stored there is dropped) and raises bit 0 of *status; of a sequence that is longer than its row of the table
+ * (or than 2^30 keys) positions stay what kv_len says, new rows behind the last column are not stored and keys there are
+ * not seen (bit 1; lengths count as 2^31 - 1 at most); new rows that reach before position 0 see nothing and are not stored (bit 2); starts that run backwards
  * or past total_rows are cut (bit 3).  Bit 4: a wait inside the tensor-core kernel ran out and the call's outputs are
  * not valid.  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] are neither
  * read nor written. */

@@ -25,6 +25,7 @@ namespace paged {
 constexpr uint32_t kMaxSeqs = 1024;
 constexpr uint32_t kMaxHeadDim = 256;
 constexpr uint32_t kMaxLen = 1u << 30;  // keys of one sequence
+constexpr uint32_t kMaxStated = 0x7fffffffu;  // stated lengths count as this at most
 
 // Bits of itk_paged_batch::status.
 constexpr uint32_t kBadPage = 1u, kLongSeq = 2u, kBeforeStart = 4u, kBadStarts = 8u, kWaitRanOut = 16u;
@@ -49,21 +50,28 @@ __device__ __forceinline__ void raise(const Batch& b, uint32_t bits) {
     if (b.status) atomicOr(b.status, bits);
 }
 
-// One sequence of the batch, with everything that does not fit cut off (see itk_paged_batch for what is reported).
+// Keys that a row of the table has places for.
+__device__ __forceinline__ uint32_t room_of(const Batch& b, uint32_t page_shift) {
+    return static_cast<uint32_t>(min(static_cast<uint64_t>(b.table_width) << page_shift, static_cast<uint64_t>(kMaxLen)));
+}
+
+// One sequence of the batch, with the rows that the packed tensors do not hold cut off (see itk_paged_batch for what is
+// reported).  Positions go by the stated length, whatever the table has room for: rows that moved to fit would lie over
+// keys that live there.  Of its keys there are min(len, room).
 struct Seq {
     uint32_t row0, rows;  // packed rows
-    uint32_t len;         // keys
+    uint32_t len;         // stated keys
     int32_t pos0;         // position of the first row; negative when the new rows reach before position 0
 };
 __device__ __forceinline__ Seq seq_of(const Batch& b, uint32_t s, uint32_t page_shift) {
     const uint32_t lo = b.row_start[s], hi = b.row_start[s + 1];
     const uint32_t stated = b.kv_len[s];
-    const uint64_t room = min(static_cast<uint64_t>(b.table_width) << page_shift, static_cast<uint64_t>(kMaxLen));
+    const uint32_t room = room_of(b, page_shift);
     Seq q;
     q.row0 = min(lo, b.total_rows);
     const uint32_t end = min(hi, b.total_rows);
     q.rows = end > q.row0 ? end - q.row0 : 0u;
-    q.len = static_cast<uint32_t>(min(static_cast<uint64_t>(stated), room));
+    q.len = min(stated, kMaxStated);
     q.pos0 = static_cast<int32_t>(q.len) - static_cast<int32_t>(q.rows);
     uint32_t bits = 0;
     if (hi < lo || hi > b.total_rows) bits |= kBadStarts;

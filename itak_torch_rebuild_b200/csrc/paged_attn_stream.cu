@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
 
 // A sequence as the walk over the batch sees it.
 struct SeqInfo {
-    uint32_t row0, rows, len;
+    uint32_t row0, rows, len;  // len: as stated; there are min(len, room) keys
 };
 
 // Where a walk over a CTA's run stands: a cell and, inside it, the 64-key tiles [t, t_end) that are left to do.
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
     const uint32_t n_seqs = p.batch.n_seqs, G = gridDim.x, cta = blockIdx.x;
     const uint32_t group = p.group, head_dim = p.pool.head_dim, shift = p.pool.page_shift;
+    const uint32_t room = room_of(p.batch, shift);
 
     after_predecessor();
 
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
     auto geometry = [&](uint32_t rows, uint32_t len, uint32_t& lo_t, uint32_t& tiles, uint32_t& blocks) {
         const int32_t pos0 = static_cast<int32_t>(len) - static_cast<int32_t>(rows);
         lo_t = p.window != 0 && pos0 >= 0 && static_cast<uint32_t>(pos0) >= p.window ? (pos0 + 1 - p.window) / kTile : 0u;
-        const uint32_t hi_t = (len + kTile - 1) / kTile;
+        const uint32_t hi_t = (min(len, room) + kTile - 1) / kTile;
         tiles = hi_t > lo_t ? hi_t - lo_t : 1u;
         blocks = (rows * group + PB - 1) / PB;
     };
@@ -204,11 +205,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
         const uint32_t r0 = c.b * PB / group, r1 = (min(c.rows * group, (c.b + 1) * PB) - 1) / group;
         const int32_t pos0 = static_cast<int32_t>(c.len) - static_cast<int32_t>(c.rows);
         const int32_t first = pos0 + static_cast<int32_t>(r0), last = pos0 + static_cast<int32_t>(r1);
-        c.hi = last >= 0 ? static_cast<uint32_t>(last) + 1u : 0u;
+        c.hi = last >= 0 ? min(static_cast<uint32_t>(last) + 1u, room) : 0u;
         c.lo = p.window != 0 && first >= 0 && static_cast<uint32_t>(first) >= p.window ? first + 1 - p.window : 0u;
         c.t = max(lo_t + tile, c.lo / kTile);
         c.t_end = min(lo_t + min(tile + n, c.T), (c.hi + kTile - 1) / kTile);
-        if (c.t >= c.t_end) {  // nothing to see here: one empty step, so that the cell is still finished
+        if (c.t >= c.t_end || c.lo >= c.hi) {  // nothing to see here: one empty step, so that the cell is still finished
             c.t = 0;
             c.t_end = 1;
             c.lo = c.hi = 0;
@@ -456,12 +457,13 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const int32_t low = p.window != 0 ? at[t][j] - static_cast<int32_t>(min(p.window, 0x7fffffffu)) : -1;
+                    const int32_t up = min(at[t][j], static_cast<int32_t>(C.hi) - 1);  // (a row's position may lie behind the last key)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int32_t key = static_cast<int32_t>(key0 + 8 * n + 2 * tq + e);
-                            if (key > at[t][j] || key <= low) w[j][n][e] = -INFINITY;
+                            if (key > up || key <= low) w[j][n][e] = -INFINITY;
                         }
                     top[j] = fmaxf(fmaxf(w[j][0][0], w[j][0][1]), fmaxf(w[j][1][0], w[j][1][1]));
                     top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));

@@ -98,7 +98,7 @@ struct Shape {
 };
 
 struct SeqInfo {
-    uint32_t row0, rows, len;
+    uint32_t row0, rows, len;  // len: as stated; there are min(len, room) keys
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -155,20 +155,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN when 
 struct KeyRange {
     uint32_t lo, hi, t0, t1;
 };
-__device__ __forceinline__ KeyRange keys_of(const SeqInfo& q, uint32_t p0, uint32_t p1, uint32_t group, uint32_t window) {
+__device__ __forceinline__ KeyRange keys_of(const SeqInfo& q, uint32_t p0, uint32_t p1, uint32_t group, uint32_t window, uint32_t room) {
     const int32_t pos0 = static_cast<int32_t>(q.len) - static_cast<int32_t>(q.rows);
     const int32_t first = pos0 + static_cast<int32_t>(p0 / group), last = pos0 + static_cast<int32_t>((p1 - 1) / group);
     KeyRange r;
-    r.hi = last >= 0 ? static_cast<uint32_t>(last) + 1u : 0u;
+    r.hi = last >= 0 ? min(static_cast<uint32_t>(last) + 1u, room) : 0u;
     r.lo = window != 0 && first >= 0 && static_cast<uint32_t>(first) >= window ? first + 1 - window : 0u;
-    if (r.hi == 0) r.lo = 0;
+    if (r.lo >= r.hi) r.lo = r.hi = 0;
     r.t0 = r.lo / kTile;
     r.t1 = (r.hi + kTile - 1) / kTile;
     return r;
 }
 // Tiles a cell takes in a run: at least one, so that a block that sees nothing is still written.
-__device__ __forceinline__ uint32_t cell_tiles(const SeqInfo& q, uint32_t block, uint32_t group, uint32_t window) {
-    const KeyRange r = keys_of(q, block * kBlockPairs, min(q.rows * group, (block + 1) * kBlockPairs), group, window);
+__device__ __forceinline__ uint32_t cell_tiles(const SeqInfo& q, uint32_t block, uint32_t group, uint32_t window, uint32_t room) {
+    const KeyRange r = keys_of(q, block * kBlockPairs, min(q.rows * group, (block + 1) * kBlockPairs), group, window, room);
     return max(r.t1 - r.t0, 1u);
 }
 
@@ -189,6 +189,7 @@ struct Item {
 struct Run {
     const AttnParams& p;
     uint64_t end;
+    uint32_t room;
 
     __device__ __forceinline__ void open_seq(Item& it) const {
         Batch b = p.batch;
@@ -201,7 +202,7 @@ struct Run {
         const uint32_t all = it.q.rows * p.group, p0 = it.block * kBlockPairs, p1 = min(all, p0 + kBlockPairs);
         it.pairs = p1 - p0;
         it.twin = it.pairs <= kTile ? 1u : 0u;
-        const KeyRange r = keys_of(it.q, p0, p1, p.group, p.window);
+        const KeyRange r = keys_of(it.q, p0, p1, p.group, p.window, room);
         it.T = max(r.t1 - r.t0, 1u);
         it.off = off;
         it.n = static_cast<uint32_t>(min(end - it.pos, static_cast<uint64_t>(it.T - off)));
@@ -218,7 +219,7 @@ struct Run {
             it.step = 1;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const KeyRange k = keys_of(it.q, p0 + i * kTile, i == 0 ? p0 + kTile : p1, p.group, p.window);
+                const KeyRange k = keys_of(it.q, p0 + i * kTile, i == 0 ? p0 + kTile : p1, p.group, p.window, room);
                 it.a[i] = max(it.t0, k.t0);
                 it.e[i] = min(it.t1, k.t1);
             }
@@ -278,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n_seqs = p.batch.n_seqs, group = p.group, window = p.window, cta = blockIdx.x;
+    const uint32_t room = room_of(p.batch, p.pool.page_shift);
 
     // ---- set-up and the batch summed up --------------------------------------------------------------------------------
     if (tid == 0) {
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         uint64_t sum = kLater;
         if (blocks <= kOwnBlocks) {
             sum = 0;
-            for (uint32_t i = 0; i < blocks; ++i) sum += cell_tiles(q, i, group, window) + kCellCost;
+            for (uint32_t i = 0; i < blocks; ++i) sum += cell_tiles(q, i, group, window, room) + kCellCost;
         }
         per_head[s] = sum;
     }
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const SeqInfo q = info[s];
         const uint32_t blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
         uint64_t sum = 0;
-        for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window) + kCellCost;
+        for (uint32_t i = lane; i < blocks; i += 32) sum += cell_tiles(q, i, group, window, room) + kCellCost;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         __syncwarp();
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             blocks = (q.rows * group + kBlockPairs - 1) / kBlockPairs;
             uint32_t tiles = 0;  // of that block
             for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {  // the block that holds position `left` of the KV head
-                const uint32_t mine = b0 + lane < blocks ? cell_tiles(q, b0 + lane, group, window) + kCellCost : 0u;
+                const uint32_t mine = b0 + lane < blocks ? cell_tiles(q, b0 + lane, group, window, room) + kCellCost : 0u;
                 uint32_t incl = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     __syncthreads();
     const uint64_t run0 = items[0].pos, run1 = items[1].pos;
     const bool works = run0 < run1;
-    const Run run{p, run1};
+    const Run run{p, run1, room};
     __syncthreads();
     if (works && warp == 0) {
         if (lane == 0) run.open_cell(items[0], items[0].off);
@@ -740,9 +742,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const bool live = in < it.pairs;
             const uint32_t pair = it.block * kBlockPairs + (live ? in : 0u);
             const int32_t pos0 = static_cast<int32_t>(it.q.len) - static_cast<int32_t>(it.q.rows);
-            const int32_t at = live ? pos0 + static_cast<int32_t>(pair / group) : -1;
-            // keys (low, at] are seen
-            const int32_t low = window != 0 ? at - static_cast<int32_t>(min(window, 0x7fffffffu)) : -1;
+            const int32_t pos = live ? pos0 + static_cast<int32_t>(pair / group) : -1;
+            // keys (low, at] are seen (a position may lie behind the last key)
+            const int32_t low = window != 0 ? pos - static_cast<int32_t>(min(window, 0x7fffffffu)) : -1, at = min(pos, static_cast<int32_t>(room) - 1);
             float m = -INFINITY, l = 0.f;
             float acc[SPLIT ? D : 1];  // f32 rows: the output so far
 #pragma unroll

@@ -265,10 +265,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
     if (row < sq.row0 || row - sq.row0 >= sq.rows) return;
     const int32_t pos = sq.pos0 + static_cast<int32_t>(row - sq.row0);
     if (pos < 0) return;
-    // pos < len <= table_width * page_size
-    const uint32_t page = p.batch.table[static_cast<size_t>(seq) * p.batch.table_stride + (static_cast<uint32_t>(pos) >> p.pool.page_shift)];
-    const bool stored = page < p.pool.n_pages;
-    if (!stored && tid == 0) raise(p.batch, kBadPage);
+    // A row behind the table's last column has no place (reported with its sequence); its query is turned all the same.
+    const bool placed = static_cast<uint32_t>(pos) < room_of(p.batch, p.pool.page_shift);
+    const uint32_t page = placed ? p.batch.table[static_cast<size_t>(seq) * p.batch.table_stride + (static_cast<uint32_t>(pos) >> p.pool.page_shift)] : 0u;
+    const bool stored = placed && page < p.pool.n_pages;
+    if (placed && !stored && tid == 0) raise(p.batch, kBadPage);
     const uint64_t at = page * p.pool.page_stride + (static_cast<uint32_t>(pos) & ((1u << p.pool.page_shift) - 1u)) * p.pool.row_stride;
     P* const kp = static_cast<P*>(p.pool.k) + at;
     P* const vp = static_cast<P*>(p.pool.v) + at;

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from itak_torch_rebuild_b200 import CudaComputeError, _lib, paged
-from pagedref import PAGE, U, Batch, rotate, rotation_bound, within
+from pagedref import PAGE, U, Batch, attend, attend_bound, rotate, rotation_bound, within
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -233,6 +233,73 @@ def test_append_drops_what_the_pool_does_not_hold():
     assert before.shape == b.k.shape
 
 
+def rows_of(b, pool):
+    """A pool's bits as [page][row][heads][D], on the host."""
+    pool = pool.cpu().view(torch.int16)
+    return (pool.transpose(1, 2) if b.layout == "head" else pool).clone()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pairing,rot,lead", [(0, 0, 0), (1, 32, 0), (1, 6, 0), (0, 16, 1)])
+@pytest.mark.parametrize("layout", ["head", "token"])
+def test_rows_behind_the_table_are_dropped_where_they_stand(t, pairing, rot, lead, layout):
+    """A sequence longer than its row of the table: positions go by the stated length, the rows that still have a place are
+    stored there, the others nowhere - least of all over the keys before them.  Queries are turned at their positions.
+    ``lead``: rows that start off a 16-byte boundary."""
+    d, page = 32, 8
+    b = Batch([3, 3, 2, 1], [24, 24, 24, 24], 4, 2, d, t, page, layout)
+    stated = [26, 1000, 24, -1]
+    b.kv_len.copy_(torch.tensor(stated))
+    f, fd, _ = table(rot) if rot else (None, None, 1.0)
+    wide = torch.randn(b.total, 8 * d + lead).to(t).cuda()
+    qkv = wide[:, lead:].unflatten(1, (8, d))
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    want_k, want_v = rows_of(b, b.k), rows_of(b, b.v)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q_out = PagedOf(b).append(k, v, b.table, b.row_start, b.kv_len, q=q, inv_freq=fd, pairing=pairing, status=status)
+    assert int(status) == 2
+    got_k, got_v = rows_of(b, b.k), rows_of(b, b.v)
+    for s, i, p in ((0, 0, 23), (2, 0, 22), (2, 1, 23)):
+        row, at, off = b.starts[s] + i, int(b.table_h[s, p // page]), p % page
+        assert torch.equal(got_v[at, off], v[row].cpu().to(PAGE[t]).view(torch.int16))
+        if rot:
+            extra, _ = rotation_bound(k[row:row + 1].cpu(), f, pairing, 1.0, PAGE[t])
+            within(got_k[at, off].view(PAGE[t])[None], rotate(k[row:row + 1].cpu(), [p], f, pairing), extra, PAGE[t])
+        else:
+            assert torch.equal(got_k[at, off], k[row].cpu().to(PAGE[t]).view(torch.int16))
+        want_k[at, off], want_v[at, off] = got_k[at, off], got_v[at, off]
+    assert torch.equal(got_k, want_k) and torch.equal(got_v, want_v), "a row outside the batch was written"
+    for s in (0, 1, 2):
+        lo, r = b.starts[s], b.rows[s]
+        if rot:
+            extra, _ = rotation_bound(q[lo:lo + r].cpu(), f, pairing, 1.0, t)
+            within(q_out[lo:lo + r], rotate(q[lo:lo + r].cpu(), [stated[s] - r + i for i in range(r)], f, pairing), extra, t)
+        else:
+            assert torch.equal(q_out[lo:lo + r], q[lo:lo + r])
+
+
+@pytest.mark.parametrize("starts,lens,bits,kept", [
+    ([0, 3, 5], [1000, 1], 2 | 4, [(1, 4, 0)]),                 # (sequence, packed row, position)
+    ([3, 0, 5], [20, 2], 4 | 8, [(1, 3, 0), (1, 4, 1)]),
+    ([0, 3, 1000], [20, 2], 8, [(0, 0, 17), (0, 1, 18), (0, 2, 19), (1, 3, 0), (1, 4, 1)]),
+    ([7, 7, 7], [20, 2], 8, []),
+    ([0, 3, 5], [2 ** 31 - 1, 24], 2, [(1, 3, 22), (1, 4, 23)]),
+])
+def test_append_of_malformed_batches_writes_what_belongs(starts, lens, bits, kept):
+    b = Batch([3, 2], [24, 24], 2, 1, 16, F16, 8, "head")
+    k = torch.randn(b.total, 1, 16).half().cuda()
+    want = [rows_of(b, b.k), rows_of(b, b.v)]
+    b.row_start.copy_(torch.tensor(starts))
+    b.kv_len.copy_(torch.tensor(lens))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, status=status)
+    assert int(status) == bits
+    for s, row, p in kept:
+        for pool in want:
+            pool[int(b.table_h[s, p // 8]), p % 8] = k[row].cpu().view(torch.int16)
+    assert torch.equal(rows_of(b, b.k), want[0]) and torch.equal(rows_of(b, b.v), want[1])
+
+
 # ---- attention --------------------------------------------------------------------------------------------------------
 
 
@@ -386,6 +453,35 @@ def test_malformed_batches_are_cut_and_reported(rows):
     out = PagedOf(b).attention(*args(), max_rows=rows, status=status)
     assert int(status) & 8
     b.check(out)  # cut to the rows there are
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [1, 7, 150])
+@pytest.mark.parametrize("over", [1, 5, 70, 10 ** 9])
+@pytest.mark.parametrize("window", [0, 3, 66, 200])
+def test_attention_of_a_sequence_longer_than_its_table(t, rows, over, window):
+    """Positions go by the stated length; the keys behind the table's last column are not there."""
+    room = 240
+    b = Batch([rows, 2], [room, 90], 4, 2, 64, t, 16, "head")
+    b.kv_len[0] = room + over
+    out, lse = torch.full((b.total, 4, 64), 7.0, dtype=t, device="cuda"), torch.full((b.total, 4), 7.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows, window=window, out=out, lse=lse, status=status)
+    assert int(status) == 2
+    b.check(out, lse, window=window, only=(1,))
+    scale = float(np.float32(1.0 / math.sqrt(b.d)))
+    for r in range(rows):
+        p = room + over - rows + r
+        behind = max(0, p - (room - 1))  # a row that stands behind the last key sees what one at the last key would, less that
+        got, got_lse = out[r:r + 1], lse[r:r + 1].double().cpu()
+        if window and window <= behind:
+            assert bool((got == 0).all()) and bool((got_lse == -math.inf).all())
+            continue
+        want, want_lse, mean, slack = attend(b.q_h[r:r + 1].double(), b.keys[0].double(), b.values[0].double(), p - behind, scale,
+                                             window - behind if window else 0)
+        within(got, want, attend_bound(mean, slack, room, b.d, t), t)
+        tol = (b.d + 16) * 2.0 ** -24 * slack + 2.0 ** -20 * slack + (room / 16 + 64) * 2.0 ** -24 + 8 * 2.0 ** -24 * want_lse.abs()
+        assert bool(((got_lse - want_lse).abs() <= tol).all())
 
 
 def test_a_wrong_bound_of_the_rows_changes_nothing_but_the_kernel():
