@@ -692,6 +692,7 @@ int itk_backend_create(const itk_config* cfg, itk_backend** out) {
     auto cuda_refuse = [&](cudaError_t e, const char* what) {
         std::string msg = std::string(what) + ": " + cudaGetErrorString(e);
         itk_backend_destroy(b);
+        cudaGetLastError();  // reported here, not by the thread's next launch
         return refuse(ITK_ERR_CUDA, msg);
     };
     cudaError_t e = cudaSetDevice(cfg->device);

@@ -211,13 +211,20 @@ struct ErrorText {
     }
 };
 
+// An error that is reported to the caller is not left pending in the thread as well, where a later call would take it for
+// its own: a launch that ran must not be reported as one that failed, or its caller may rotate rows in place twice.
+inline cudaError_t handled(cudaError_t e) {
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
+}
+
 // Makes `device` current for the call and puts the caller's back.
 class DeviceScope {
 public:
     explicit DeviceScope(int device) {
-        err = cudaGetDevice(&prev_);
+        err = handled(cudaGetDevice(&prev_));
         if (err == cudaSuccess && prev_ != device) {
-            err = cudaSetDevice(device);
+            err = handled(cudaSetDevice(device));
             changed_ = err == cudaSuccess;
         }
     }
@@ -246,6 +253,7 @@ private:
     std::atomic<uint64_t> bits_{0};
 };
 
+// The launch's own result, whatever was pending before it.
 template <typename... Params, typename... Args>
 cudaError_t launch_dependent(void (*kernel)(Params...), uint32_t grid, uint32_t threads, size_t smem, cudaStream_t s, const Args&... args) {
     cudaLaunchAttribute attr{};
@@ -258,9 +266,7 @@ cudaError_t launch_dependent(void (*kernel)(Params...), uint32_t grid, uint32_t 
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    const cudaError_t last = cudaGetLastError();
-    return e != cudaSuccess ? e : last;
+    return handled(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 constexpr uint64_t kMaxStride = 1ull << 38;

@@ -14,7 +14,7 @@ cudaError_t multiprocessors(int device, uint32_t* sms) {
     static std::atomic<uint32_t> known[64];
     if (device >= 0 && device < 64 && (*sms = known[device].load(std::memory_order_relaxed)) != 0) return cudaSuccess;
     int n = 0;
-    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+    const cudaError_t e = handled(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
     if (e != cudaSuccess) return e;
     *sms = static_cast<uint32_t>(n);
     if (device >= 0 && device < 64) known[device].store(*sms, std::memory_order_relaxed);

@@ -674,8 +674,8 @@ cudaError_t launch_as(const AttnParams& p, uint32_t sms, cudaStream_t s) {
     auto kernel = paged_stream_kernel<T, D, STAGES, MT>;
     static OncePerDevice prepared;
     if (!prepared.done(p.device)) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, STAGES>(MT, kMaxSeqs)));
+        const cudaError_t e = handled(
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, STAGES>(MT, kMaxSeqs))));
         if (e != cudaSuccess) return e;
         prepared.mark(p.device);
     }

@@ -1204,11 +1204,11 @@ cudaError_t launch_as(const AttnParams& p, int32_t page_dtype, uint32_t sms, cud
     static OncePerDevice prepared;
     if (!prepared.done(p.device)) {
         cudaFuncAttributes attr;
-        cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+        cudaError_t e = handled(cudaFuncGetAttributes(&attr, kernel));
         if (e != cudaSuccess) return e;
         // The warpgroups' shares are drawn from what the block was launched with: fewer, and setmaxnreg would wait for good.
         if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<T, D>::kSmem));
+        e = handled(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<T, D>::kSmem)));
         if (e != cudaSuccess) return e;
         prepared.mark(p.device);
     }

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
 from typing import Optional, Sequence
 
 import numpy as np
@@ -57,12 +58,21 @@ def _refuse(msg: str, code: int = _lib.ERR_INVALID_ARGUMENT):
     raise CudaComputeError(code, msg)
 
 
-def _explain(fn, *args):
-    """A refused call has done nothing: it is made again with a buffer for its reason."""
-    err = C.create_string_buffer(_ERROR_LEN)
-    rc = fn(*args, err, _ERROR_LEN)
+class _Reason(threading.local):
+    """A thread's buffer for the reason of a refusal, handed to every call: a call is made once, whatever it returns."""
+
+    def __init__(self):
+        self.text = C.create_string_buffer(_ERROR_LEN)
+
+
+_reason = _Reason()
+
+
+def _call(fn, *args):
+    text = _reason.text
+    rc = fn(*args, text, _ERROR_LEN)
     if rc != _lib.OK:
-        raise CudaComputeError(rc, err.value.decode("utf-8", "replace"))
+        raise CudaComputeError(rc, text.value.decode("utf-8", "replace"))
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -149,10 +159,7 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                        1 if inverse else 0, dtype, dev, magnitude)
     except _OUT_OF_RANGE as e:
         _refuse(f"an argument is out of range: {e}")
-    fn = _entry("itk_rope_apply", 1)
-    stream = _raw_stream(dev) if stream is None else stream
-    if fn(d, stream, None, 0) != _lib.OK:
-        _explain(fn, d, stream)
+    _call(_entry("itk_rope_apply", 1), d, _raw_stream(dev) if stream is None else stream)
     return out
 
 
@@ -253,10 +260,7 @@ class PagedKv:
                              row_dtype, magnitude)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        fn = _entry("itk_paged_append", 3)
-        stream = _raw_stream(dev) if stream is None else stream
-        if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
-            _explain(fn, self._kv, batch, a, stream)
+        _call(_entry("itk_paged_append", 3), self._kv, batch, a, _raw_stream(dev) if stream is None else stream)
         return q_out
 
     def attention(self, q: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *, max_rows: int,
@@ -299,7 +303,5 @@ class PagedKv:
                                 max_rows, window, row_dtype, self._scale if scale is None else scale)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        fn = _entry("itk_paged_attention", 3)
-        if fn(self._kv, batch, a, stream, None, 0) != _lib.OK:
-            _explain(fn, self._kv, batch, a, stream)
+        _call(_entry("itk_paged_attention", 3), self._kv, batch, a, stream)
         return out

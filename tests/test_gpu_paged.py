@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from itak_torch_rebuild_b200 import CudaComputeError, _lib, paged
+from itak_torch_rebuild_b200 import CudaCompute, CudaComputeError, KvDtype, _lib, paged
 from pagedref import PAGE, U, Batch, attend, attend_bound, rotate, rotation_bound, within
 
 pytestmark = pytest.mark.gpu
@@ -109,6 +109,35 @@ def test_rotation_refuses_on_the_python_side():
         kw.update(bad)
         with pytest.raises(CudaComputeError):
             paged.rope_apply(kw.pop("x"), kw.pop("positions"), kw.pop("inv_freq"), **kw)
+
+
+def leave_an_error_behind(how):
+    lib = _lib.load()
+    if how == "a device that is not there":
+        assert lib.itk_paged_attention_workspace(torch.cuda.device_count() + 7) == 0
+    elif how == "a call on a device that is not there":
+        d = _lib.RopeDesc(1 << 20, 1 << 21, 1 << 20, 1 << 20, 64, 64, 64, 64, 1, 1, 64, 64, 0, 0, _lib.ROW_F32, torch.cuda.device_count() + 7, 1.0)
+        assert lib.itk_rope_apply(C.byref(d), None, None, 0) == _lib.ERR_CUDA
+    else:  # 8 TiB of slots
+        with pytest.raises(CudaComputeError):
+            CudaCompute(8, 8, 8, 128, n_slots=64, max_context=1 << 22, chunk_cap=8, kv_dtype=KvDtype.F32)
+
+
+@pytest.mark.parametrize("how", ["a device that is not there", "a call on a device that is not there", "a cache that does not fit"])
+def test_an_earlier_error_does_not_turn_rows_twice(how):
+    """A refused call of this library before one that rotates in place: the rows are turned once, and nothing is raised."""
+    f, fd, _ = table(64)
+    x, pos = torch.randn(4, 2, 64), torch.tensor([3, 50, 700, 9000], dtype=torch.int32)
+    extra, _ = rotation_bound(x, f, 0, 1.0, F32)
+    y = x.cuda()
+    leave_an_error_behind(how)
+    paged.rope_apply(y, pos.cuda(), fd, out=y)
+    within(y, rotate(x, pos, f, 0), extra, F32)
+    b = Batch([4], [9], 2, 1, 64, F32, 8, "head")
+    q, k = x.cuda(), torch.randn(4, 1, 64).cuda()
+    leave_an_error_behind(how)
+    PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len, q=q, q_out=q, inv_freq=fd)
+    within(q, rotate(x, [5, 6, 7, 8], f, 0), extra, F32)
 
 
 # ---- append -----------------------------------------------------------------------------------------------------------

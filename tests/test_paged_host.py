@@ -228,3 +228,30 @@ def test_missing_descriptors(lib):
         assert fn(None, None, None, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
         assert fn(C.byref(kv()), None, None, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
         assert fn(C.byref(kv()), C.byref(batch()), None, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
+
+
+def test_a_failed_call_is_made_once():
+    """A call that reports an error may have run (an error of an asynchronous launch before it): it is not made again."""
+    made = []
+
+    def entry(*args):
+        made.append(args)
+        args[-2].value = b"launch failed: something before it"
+        return _lib.ERR_CUDA if len(made) == 1 else _lib.OK
+
+    with pytest.raises(CudaComputeError) as e:
+        paged._call(entry, b"descriptor", 7)
+    assert e.value.code == _lib.ERR_CUDA and e.value.msg == "launch failed: something before it"
+    assert len(made) == 1 and made[0][:2] == (b"descriptor", 7)
+    paged._call(entry, b"descriptor", 7)
+    assert len(made) == 2
+
+
+@pytest.mark.parametrize("name,args", [("itk_rope_apply", 1), ("itk_paged_append", 3), ("itk_paged_attention", 3)])
+def test_every_entry_point_is_called_once_and_keeps_its_reason(lib, name, args, monkeypatch):
+    """The library's own refusals through the packed descriptors' path, its first call already carrying the buffer."""
+    fn = paged._entry(name, args)
+    made = []
+    with pytest.raises(CudaComputeError) as e:
+        paged._call(lambda *a: made.append(a) or fn(*a), *[None] * args, None)
+    assert len(made) == 1 and "null pointer" in e.value.msg
