@@ -496,7 +496,8 @@ typedef enum itk_row_dtype { ITK_ROW_F32 = 0, ITK_ROW_F16 = 1, ITK_ROW_BF16 = 2 
  *   ITK_ROPE_BANDS   by turns over the original context, t_i = original_context * inv_freq[i] / 2 pi: pairs of more
  *                    than `high` turns kept, of fewer than `low` divided by factor, between them mixed in t_i
  *   ITK_ROPE_RAMP    by pair number: kept up to the pair of `high` turns (rounded down), divided by factor from the
- *                    pair of `low` turns (rounded up), mixed linearly between; magnitude 0.1 ln(factor) + 1
+ *                    pair of `low` turns (rounded up; behind the last pair where that still makes more, up to number
+ *                    rotary_dim - 1), mixed linearly between; magnitude 0.1 ln(factor) + 1
  *   ITK_ROPE_PAIRS   inv_freq[i] / pair_factors[i]
  * `magnitude` multiplies sine and cosine; 0 asks for the scaling's own (1 except for RAMP).  Host arithmetic in f64, no
  * device needed; inv_freq receives rotary_dim / 2 values, which the caller copies to the device once. */

@@ -451,10 +451,11 @@ extern "C" int itk_rope_table(const itk_rope_config* c, double* inv_freq, float*
     const double rot = c->rotary_dim, factor = c->factor, two_pi = 6.283185307179586476925;
     double base = c->base;
     if (c->scaling == ITK_ROPE_BASE) base *= pow(factor, rot / (rot - 2.0));
-    // RAMP: the pair that makes t turns over the original context, base^(-2i / rot) * original_context = 2 pi t
+    // RAMP: the pair that makes t turns over the original context, base^(-2i / rot) * original_context = 2 pi t.  The pair of
+    // `low` turns may lie behind the last one (up to rot - 1): then the ramp ends before it has come down to 1 / factor.
     const double pair_span = rot / (2.0 * log(base));
     const double ramp_lo = banded ? fmax(0.0, floor(pair_span * log(c->original_context / (c->high * two_pi)))) : 0.0;
-    const double ramp_hi = banded ? fmin(half - 1.0, ceil(pair_span * log(c->original_context / (c->low * two_pi)))) : 0.0;
+    const double ramp_hi = banded ? fmin(rot - 1.0, ceil(pair_span * log(c->original_context / (c->low * two_pi)))) : 0.0;
     for (uint32_t i = 0; i < half; ++i) {
         double f = pow(base, -2.0 * i / rot);
         double keep = 1.0;

@@ -65,6 +65,25 @@ def test_ramp_table_and_magnitude(lib):
     assert paged.rope_table(rot, 10000.0, scaling="ramp", factor=factor, original_context=ctx, low=low, high=high, magnitude=1.5)[1] == 1.5
 
 
+@pytest.mark.parametrize("rot,base,ctx,behind", [(128, 10000.0, 65536.0, True), (128, 10000.0, 131072.0, True), (64, 10000.0, 65536.0, True),
+                                                 (64, 10000.0, 1e9, True), (128, 10000.0, 32768.0, False), (4, 500000.0, 8192.0, True),
+                                                 (2, 500000.0, 8192.0, True), (128, 500000.0, 8192.0, False)])
+def test_ramp_whose_upper_pair_lies_behind_the_last(lib, rot, base, ctx, behind):
+    """Slow pairs that make more than `low` turns over the original context: the ramp's upper end is not moved to the last
+    pair, only to rotary_dim - 1."""
+    factor, low, high = 8.0, 1.0, 32.0
+    f, _ = paged.rope_table(rot, base, scaling="ramp", factor=factor, original_context=ctx, low=low, high=high)
+    a = max(0.0, math.floor(rot * math.log(ctx / (high * 2 * math.pi)) / (2 * math.log(base))))
+    b = min(rot - 1.0, math.ceil(rot * math.log(ctx / (low * 2 * math.pi)) / (2 * math.log(base))))
+    assert (b > rot / 2 - 1) == behind
+    for j in range(rot // 2):
+        plain = base ** (-2 * j / rot)
+        gone = min(1.0, max(0.0, (j - a) / max(b - a, 1e-3)))
+        assert f[j] == pytest.approx(plain * (1 - gone) + plain / factor * gone, rel=1e-13), j
+    if behind:
+        assert f[-1] > base ** (2.0 / rot - 1.0) / factor * 1.0000001
+
+
 def test_pair_factors(lib):
     pf = np.linspace(1, 9, 32)
     f, _ = paged.rope_table(64, BASE, scaling="pairs", pair_factors=pf)
