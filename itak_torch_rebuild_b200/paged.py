@@ -3,8 +3,9 @@
 ``PagedKv`` names a pair of page pools the caller owns; ``append`` stores a ragged batch's new rows (K rotated on the
 way) and ``attention`` attends them.  ``rope_table`` makes a rotation's frequencies, plain or scaled for long contexts,
 and ``rope_apply`` rotates rows on their own, forward or as a gradient.  Every call queues work on the current stream of
-the tensors' device (or on ``stream``), allocates nothing on the device but a default ``out`` and, once per stream, a
-workspace, and raises :class:`CudaComputeError` with the library's text when it is refused.
+the tensors' device (or on ``stream``, a handle), allocates nothing on the device but a default ``out`` (of the stream that
+writes it, as torch counts it) and, once per stream, a workspace, and raises :class:`CudaComputeError` with the library's text
+when it is refused.  Tensors that a call on ``stream`` shares with other streams are the caller's to order, as in torch.
 
 A batch: sequence ``s`` owns the packed rows ``[row_start[s], row_start[s + 1])`` and ``kv_len[s]`` keys, its new rows
 included; the key of position ``p`` is row ``p % page_size`` of page ``table[s][p // page_size]``.  ``table``,
@@ -78,14 +79,36 @@ def _call(fn, *args):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# Handles with a meaning of their own: the default stream (two names), and "the calling thread's", one handle for many streams.
+_DEFAULT_STREAMS = (0, 1)
+_PER_THREAD_STREAM = 2
+
+
+def _stream_object(device: int, stream: int):
+    """The torch stream of a handle."""
+    if stream in _DEFAULT_STREAMS:
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(stream, device=device)
+
+
 def _capturing(device: int, stream: int) -> bool:
     """Whether ``stream`` of ``device`` is being captured, the current stream or not (the default one never is)."""
-    if stream == 0:
+    if stream in _DEFAULT_STREAMS:
         return False
     if device == torch.cuda.current_device() and stream == _raw_stream(device):
         return torch.cuda.is_current_stream_capturing()
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+    with torch.cuda.stream(_stream_object(device, stream)):
         return torch.cuda.is_current_stream_capturing()
+
+
+def _new_rows(shape, dtype, device: int, stream: Optional[int]) -> torch.Tensor:
+    """Memory for a result of a call on ``stream`` (``None``: the current one).  It has to be the allocator's memory of that
+    stream: a block of another stream's may still be read there by work queued before it was freed, and may be handed out
+    again there while ``stream`` writes it."""
+    if stream is None or stream == _raw_stream(device):
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(_stream_object(device, stream)):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
@@ -144,7 +167,7 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         _refuse(f"x must be an f32, f16 or bf16 [rows][heads][head_dim] tensor on a CUDA device, got {x.dtype} {tuple(x.shape)} on {x.device}")
     shape = x.shape
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = _new_rows(shape, x.dtype, dev, stream)
     elif out.dtype is not x.dtype or out.get_device() != dev or out.shape != shape:
         _refuse(f"out must be {x.dtype} {tuple(shape)} on {x.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
     rows, heads, head_dim = shape
@@ -244,7 +267,7 @@ class PagedKv:
             q_heads = q.shape[1]
             q_row = _rows(q, "q", rows, q_heads, d, dtype, dev)
             if q_out is None:
-                q_out = torch.empty((rows, q_heads, d), dtype=dtype, device=self.device)
+                q_out = _new_rows((rows, q_heads, d), dtype, dev, stream)
             q_out_row = _rows(q_out, "q_out", rows, q_heads, d, dtype, dev)
             q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
@@ -279,7 +302,7 @@ class PagedKv:
         rows, q_heads, _ = q.shape
         q_row = _rows(q, "q", rows, q_heads, d, dtype, dev)
         if out is None:
-            out = torch.empty((rows, q_heads, d), dtype=dtype, device=self.device)
+            out = _new_rows((rows, q_heads, d), dtype, dev, stream)
         out_row = _rows(out, "out", rows, q_heads, d, dtype, dev)
         lse_at = 0
         if lse is not None:

@@ -593,6 +593,43 @@ def test_another_stream_and_one_given_by_number(rows):
     assert torch.equal(out, out2)
 
 
+def calls_with_a_result_of_their_own():
+    f, fd, _ = table(64)
+    x, pos = torch.randn(48, 4, 64, device="cuda"), torch.arange(48, dtype=torch.int32, device="cuda")
+    b = Batch([16] * 3, [21, 200, 77], 4, 2, 64, F32, 16, "head")
+    k = torch.randn(48, 2, 64, device="cuda")
+    kv, batch = PagedOf(b), (b.table, b.row_start, b.kv_len)
+    return {"rope": lambda **kw: paged.rope_apply(x, pos, fd, **kw),
+            "append": lambda **kw: kv.append(k, k, *batch, q=x, inv_freq=fd, **kw),
+            "attention": lambda **kw: kv.attention(x, *batch, max_rows=1, **kw)}
+
+
+@pytest.mark.parametrize("name", ["rope", "append", "attention"])
+def test_a_result_that_another_stream_writes_is_that_streams_memory(name):
+    """A block that work queued on the current stream still reads, freed behind that work, is not what a call on another
+    stream writes its result to - nor is the result's block handed out on the current stream while that one writes."""
+    call = calls_with_a_result_of_their_own()[name]
+    want = call()  # (also the first call of its kind)
+    s = torch.cuda.Stream()
+    call(stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    held = torch.full_like(want, 5.0)
+    read = torch.empty_like(held)
+    torch.cuda._sleep(1 << 26)  # some 30 ms before the block is read
+    read.copy_(held)
+    at = held.data_ptr()
+    del held
+    got = call(stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((read == 5.0).all()), "a block that was still being read was written"
+    assert torch.equal(got, want) and got.data_ptr() != at
+    at = got.data_ptr()
+    del got
+    assert torch.empty_like(want).data_ptr() != at  # it went back to the other stream
+    # the same stream by number: as without it
+    assert torch.equal(call(stream=torch.cuda.current_stream().cuda_stream), want)
+
+
 def test_two_streams_at_once():
     b = [Batch([1] * 4, [900, 40, 333, 64], 8, 2, 128, F16, 16, "head", seed=i) for i in range(2)]
     streams = [torch.cuda.Stream() for _ in b]
