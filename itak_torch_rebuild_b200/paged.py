@@ -105,6 +105,8 @@ def _new_rows(shape, dtype, device: int, stream: Optional[int]) -> torch.Tensor:
     """Memory for a result of a call on ``stream`` (``None``: the current one).  It has to be the allocator's memory of that
     stream: a block of another stream's may still be read there by work queued before it was freed, and may be handed out
     again there while ``stream`` writes it."""
+    if stream == _PER_THREAD_STREAM:  # one handle, a stream for every thread: the allocator could not tell them apart
+        _refuse("a call on the per-thread default stream needs its result's memory given")
     if stream is None or stream == _raw_stream(device):
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(_stream_object(device, stream)):
@@ -191,12 +193,14 @@ _workspaces: dict = {}
 
 def attention_workspace(device) -> torch.Tensor:
     """A workspace for ``PagedKv.attention`` calls on ``device``, cleared.  Calls that may run at the same time - on two
-    streams, or from two graphs that are replayed on two streams - need one each."""
+    streams, or from two graphs that are replayed on two streams - need one each.  Make it before a capture begins."""
     device = torch.device(device)
     n = _lib.load().itk_paged_attention_workspace(device.index or 0)
     if n == 0:
         raise CudaComputeError(_lib.ERR_CUDA, f"no workspace for {device}: the device cannot be used")
     with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():  # its clearing would become part of the graph, its memory the graph's
+            _refuse("a workspace cannot be made while the current stream is being captured")
         ws = torch.zeros(n, dtype=torch.uint8, device=device)
         torch.cuda.current_stream().synchronize()  # whatever stream uses it first
     return ws
@@ -294,7 +298,9 @@ class PagedKv:
         within ``window`` keys when it is not 0 (``itk_paged_attention``).  ``max_rows`` bounds the rows of one sequence
         and only chooses between kernels; ``scale`` is ``1 / sqrt(head_dim)`` unless given; ``lse`` ``[rows][q_heads]``
         f32 receives the log-sum-exp.  Without ``workspace`` calls of one stream share one of this module's; a call
-        that is being captured must be given its own (``attention_workspace``)."""
+        that is being captured, or that runs on the per-thread default stream, must be given its own
+        (``attention_workspace``).  A stream that is destroyed is to be synchronised first: its handle, and the workspace
+        that goes with it, may become another stream's."""
         dev, d, dtype = self._index, self.head_dim, q.dtype
         row_dtype = _ROW_DTYPES.get(dtype)
         if row_dtype is None or q.dim() != 3:
@@ -311,6 +317,8 @@ class PagedKv:
             lse_at = lse.data_ptr()
         stream = _raw_stream(dev) if stream is None else stream
         if workspace is None:
+            if stream == _PER_THREAD_STREAM:  # one handle, a stream for every thread
+                _refuse("a call on the per-thread default stream needs a workspace of its own (attention_workspace)")
             if _capturing(dev, stream):
                 _refuse("a call that is being captured needs a workspace of its own (attention_workspace)")
             workspace = _workspaces.get((dev, stream))

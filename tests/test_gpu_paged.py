@@ -1,6 +1,7 @@
 """The paged operators on the device against their definitions in 64 bits (``pagedref``), with tolerances derived there."""
 import ctypes as C
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -669,6 +670,57 @@ def test_a_stream_given_by_number_that_is_being_captured_needs_a_workspace_too()
         with torch.cuda.stream(current), pytest.raises(CudaComputeError) as e:
             PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out, stream=captured.cuda_stream)
     assert "workspace" in e.value.msg
+
+
+def test_the_per_thread_default_stream_shares_nothing_of_the_modules():
+    """Its handle is one number for the streams of all threads: neither a workspace nor the allocator may go by it."""
+    b = Batch([1, 1], [400, 90], 4, 2, 64, F16, 16, "head")
+    args, per_thread = (b.q, b.table, b.row_start, b.kv_len), 2
+    ws = [paged.attention_workspace("cuda:0") for _ in range(4)]
+    outs = [torch.empty_like(b.q) for _ in ws]
+    with pytest.raises(CudaComputeError) as e:
+        PagedOf(b).attention(*args, max_rows=1, out=outs[0], stream=per_thread)
+    assert "workspace" in e.value.msg
+    for call in (lambda: PagedOf(b).attention(*args, max_rows=1, workspace=ws[0], stream=per_thread),
+                 lambda: paged.rope_apply(b.q, torch.zeros(2, dtype=torch.int32, device="cuda"), table(64)[1], stream=per_thread),
+                 lambda: PagedOf(b).append(b.q[:, :2], b.q[:, 2:], b.table, b.row_start, b.kv_len, q=b.q, stream=per_thread)):
+        with pytest.raises(CudaComputeError) as e:
+            call()
+        assert "memory" in e.value.msg
+    torch.cuda.synchronize()
+
+    def thread(i):
+        for _ in range(20):
+            PagedOf(b).attention(*args, max_rows=1, out=outs[i], workspace=ws[i], stream=per_thread)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(len(ws))]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    torch.cuda.synchronize()
+    for o in outs:
+        b.check(o)
+
+
+def test_a_workspace_is_not_made_inside_a_capture():
+    b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
+    out = torch.empty_like(b.q)
+    fresh = torch.cuda.Stream()  # (a stream whose workspace is not there yet)
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    paged._workspaces.pop((0, fresh.cuda_stream), None)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.add_(1)
+        for call in (lambda: paged.attention_workspace("cuda:0"),
+                     lambda: PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1, out=out, stream=fresh.cuda_stream)):
+            with pytest.raises(CudaComputeError) as e:
+                call()
+            assert "captured" in e.value.msg
+    g.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1).all())  # the capture went on
 
 
 def test_rows_of_another_number_of_dimensions_are_refused():
