@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint32_t bar_q = bar_o + 16;              // [stream] the cell's queries are in shared memory
     const uint32_t bar_land = bar_q + 16;           // a V tile that needs zero rows has landed
     const uint32_t bar_done = bar_land + 8;         // everything issued to the tensor core is complete
-    constexpr uint32_t kWordAt = 16 * NST + 96, kItemsAt = kWordAt + 24, kItems = 7;
+    const uint32_t bar_t = bar_done + 8;            // [stream] the products' thread has come to the cell
+    constexpr uint32_t kWordAt = 16 * NST + 112, kItemsAt = kWordAt + 24, kItems = 7;
     static_assert(kItemsAt + kItems * sizeof(Item) + 256 * sizeof(float2) <= kTailBytes, "tail");
     uint32_t* const word = reinterpret_cast<uint32_t*>(tail_ptr + kWordAt);  // [0] tensor memory, [1] joined flag
     volatile uint32_t* const abort_flag = word + 2;
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             tc::mbar_init(bar_p + 16 * i + 8, 128);
             tc::mbar_init(bar_o + 8 * i, 1);
             tc::mbar_init(bar_q + 8 * i, 128);
+            tc::mbar_init(bar_t + 8 * i, 1);
             issued[i] = 0;
         }
         tc::mbar_init(bar_land, 1);
@@ -588,7 +590,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         if constexpr (SPLIT) tc::mma_f16_ss(tS, q + Sh::kStage / 16 + off, k + off, kIdS, 1u);
                     }
                 };
-                ok = wait(bar_q + 8 * i, n_items & 1u);
+                // A twin cell's queries are the first warpgroup's for both streams.  No queries are handed over before both
+                // streams that read the ones before have come here (bar_t), so no phase can be passed over: stream 1 has its own
+                // barrier's phase of a twin cell only after warpgroup 0 has met warpgroup 1 at the end of the cell before.
+                ok = wait(bar_q + 8 * i, n_items & 1u) && (twin == 0 || i == 0 || wait(bar_q, n_items & 1u));
+                if (ok) mbar_arrive(bar_t + 8 * i);
                 const uint32_t xa = it.a[1 - i], xe = it.e[1 - i];
                 const uint32_t rounds = xa < xe ? (xe - xa + step - 1) / step + 1 : 0u;  // of the other stream: 0, 1, ...
                 // One copy of the code: the first round has no weights to use yet, the last no scores to make.
@@ -660,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);  // the queries carry a negative scale's sign
         const bool flip = p.scale_log2 < 0.f;
         const uint32_t head_dim = p.pool.head_dim;
-        uint32_t n_s = 0, n_o = 0;  // scores seen, last products seen
+        uint32_t n_s = 0, n_o = 0, n_t = 0;  // scores seen, last products seen, cells ended
         bool dead = !works;         // a wait ran out: walk on through the barriers, touch nothing
         Item &it = items[i], &nx = items[2 + i];  // the warpgroup's cell and the one after it
         auto group_sync = [&]() {
@@ -729,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         auto hand_over_queries = [&]() {
             asm volatile("cp.async.wait_all;\n" ::: "memory");
             tc::fence_proxy_async();
+            tc::fence_before_sync();  // the next products overwrite what was read out of tensor memory
             mbar_arrive(bar_q + 8 * i);
         };
         if (works) {
@@ -1142,6 +1149,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
             }
+            // A stream without a tile in the cell has waited for nothing of its products' thread so far: queries handed over
+            // two cells ahead of it would complete a phase that it tells by its parity.
+            dead = dead || !wait(bar_t + 8 * i, n_t & 1u);
+            dead = __any_sync(0xffffffffu, dead);
+            ++n_t;
             if (twin) {  // the other stream's accumulator and the exchange are done with
                 tc::fence_before_sync();
                 both_sync();

@@ -146,3 +146,129 @@ class Batch:
                 # the score's error, the sum's, and log2 and its product in f32
                 tol = (self.d + 16) * 2.0 ** -24 * slack + 2.0 ** -20 * slack + (n / 16 + 64) * 2.0 ** -24 + 8 * 2.0 ** -24 * want_lse.abs()
                 assert bool(((got - want_lse).abs()[seen] <= tol[seen]).all()), float((got - want_lse).abs()[seen].max())
+
+
+# ---- the same for batches of some thousand keys, on the device ----------------------------------------------------------
+
+def attend_many(q, keys, values, pos0, scale, window):
+    """``attend`` with all rows and heads of a sequence at once, on the tensors' own device."""
+    rows, hq, d = q.shape
+    n, hkv, _ = keys.shape
+    k, v = (x.double().transpose(0, 1).repeat_interleave(hq // hkv, 0) for x in (keys, values))  # [Hq][n][D]
+    qh = q.double().transpose(0, 1)
+    p = torch.arange(pos0, pos0 + rows, device=q.device)[:, None]
+    key = torch.arange(n, device=q.device)
+    seen = (key <= p) & (key > p - window) if window else key <= p
+    s = (qh @ k.transpose(1, 2) * scale).masked_fill(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    w = torch.exp(s - top.masked_fill(top == -math.inf, 0.0))
+    total = w.sum(-1, keepdim=True)
+    w = torch.where(total > 0, w / total, torch.zeros_like(w))
+    lse = (top + total.log()).squeeze(-1)
+    slack = (qh.abs() @ k.abs().transpose(1, 2)).masked_fill(~seen, 0.0).amax(-1) * abs(scale)
+    return (w @ v).transpose(0, 1), lse.transpose(0, 1), (w @ v.abs()).transpose(0, 1), slack.transpose(0, 1)
+
+
+class DeviceBatch:
+    """A ragged batch made on the device, pages scattered over a pool whose unused rows hold NaN.  ``shape``: what to do with
+    (q, keys, values) of a sequence before they are stored."""
+
+    def __init__(self, rows, lens, hq, hkv, d, t, page, layout, seed=0, shape=None):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.rows, self.lens, self.hq, self.hkv, self.d, self.t, self.page, self.layout = rows, lens, hq, hkv, d, t, page, layout
+        pt, i32 = PAGE[t], dict(dtype=torch.int32, device="cuda")
+        held = [-(-n // page) for n in lens]
+        self.n_pages = sum(held) + 2
+        order = torch.randperm(self.n_pages, generator=g, device="cuda").to(torch.int32)
+        self.table = torch.full((len(rows), max(1, max(held))), -1, **i32)
+        self.starts = np.cumsum([0] + rows).tolist()
+        self.total = self.starts[-1]
+        self.k, self.v = (torch.full((self.n_pages, page, hkv, d), math.nan, dtype=pt, device="cuda") for _ in range(2))
+        self.q = torch.empty(self.total, hq, d, dtype=t, device="cuda")
+        self.keys, self.values = [], []
+        for s, (r, n) in enumerate(zip(rows, lens)):
+            at = sum(held[:s])
+            self.table[s, :held[s]] = order[at:at + held[s]]
+            q, k, v = (torch.randn(m, h, d, generator=g, device="cuda") for m, h in ((r, hq), (n, hkv), (n, hkv)))
+            if shape is not None:
+                q, k, v = shape(q, k, v)
+            self.q[self.starts[s]:self.starts[s] + r] = q.to(t)
+            self.keys.append(k.to(pt))
+            self.values.append(v.to(pt))
+            p = torch.arange(n, device="cuda")
+            place = (self.table[s].long()[p // page], p % page)
+            self.k[place], self.v[place] = self.keys[s], self.values[s]
+        if layout == "head":
+            self.k, self.v = (x.transpose(1, 2).contiguous() for x in (self.k, self.v))
+        self.row_start = torch.tensor(self.starts, **i32)
+        self.kv_len = torch.tensor(lens, **i32)
+
+    def check(self, out, lse, window=0, scale=None):
+        scale = float(np.float32(1.0 / math.sqrt(self.d) if scale is None else scale))
+        for s, (r, n) in enumerate(zip(self.rows, self.lens)):
+            if r == 0:
+                continue
+            lo = self.starts[s]
+            want, want_lse, mean, slack = (x.cpu() for x in attend_many(self.q[lo:lo + r], self.keys[s], self.values[s], n - r, scale, window))
+            within(out[lo:lo + r], want, attend_bound(mean, slack, n, self.d, self.t), self.t)
+            got = lse[lo:lo + r].double().cpu()
+            seen = torch.isfinite(want_lse)
+            assert torch.equal(torch.isfinite(got), seen) and bool((got[~seen] == -math.inf).all())
+            tol = (self.d + 16) * 2.0 ** -24 * slack + 2.0 ** -20 * slack + (n / 16 + 64) * 2.0 ** -24 + 8 * 2.0 ** -24 * want_lse.abs()
+            assert bool(((got - want_lse).abs()[seen] <= tol[seen]).all()), float((got - want_lse).abs()[seen].max())
+
+
+# How the attention kernels cut a launch into runs, one per CTA, restated from their sources: what a test's batch makes them do.
+
+def plan_tc(rows, lens, group, kv_heads, window, sms):
+    """The tensor-memory kernel's pieces: (CTA, pairs of the cell's block, tiles of the piece, tiles of the cell)."""
+    tile, block, cost, snap = 128, 256, 3, 1
+    cells = []  # (pairs, tiles), in the launch's order
+    for r, n in zip(rows, lens):
+        of_head = []
+        for p0 in range(0, r * group, block):
+            p1 = min(r * group, p0 + block)
+            first, last = n - r + p0 // group, n - r + (p1 - 1) // group
+            hi = max(0, last + 1)
+            lo = first + 1 - window if window and first >= window else 0
+            of_head.append((p1 - p0, max(1, -(-hi // tile) - lo // tile) if hi > lo else 1))
+        cells += of_head * kv_heads
+    starts = np.cumsum([0] + [t + cost for _, t in cells]).tolist()
+    total = starts[-1]
+    per = max(1, -(-total // sms))
+    snap = min(snap, per // 2)
+
+    def cut(pos):
+        if pos >= total:
+            return total
+        c = int(np.searchsorted(starts, pos, side="right")) - 1
+        left = pos - starts[c]
+        return starts[c] if left <= snap else starts[c + 1] if left + snap >= cells[c][1] else pos
+
+    pieces = []
+    for cta in range(sms):
+        lo, hi = cut(cta * per), cut((cta + 1) * per)
+        for c in range(len(cells)):
+            a, b = max(lo, starts[c]), min(hi, starts[c] + cells[c][1])
+            if a < b:
+                pieces.append((cta, cells[c][0], b - a, cells[c][1]))
+    return pieces
+
+
+def plan_stream(rows, lens, group, kv_heads, window, block, ctas):
+    """The streaming kernel's pieces: (CTA, tiles of the piece, tiles of the cell); ``block``: pairs of a cell."""
+    tile, cost, least = 64, 3, 2
+    cells = []
+    for r, n in zip(rows, lens):
+        pos0 = n - r
+        lo = (pos0 + 1 - window) // tile if window and pos0 >= window else 0
+        cells += [max(1, -(-n // tile) - lo)] * (-(-r * group // block) * kv_heads)
+    starts = np.cumsum([0] + [t + cost for t in cells]).tolist()
+    per = max(least, -(-starts[-1] // ctas))
+    pieces = []
+    for cta in range(ctas):
+        for c in range(len(cells)):
+            a, b = max(cta * per, starts[c]), min((cta + 1) * per, starts[c] + cells[c])
+            if a < b:
+                pieces.append((cta, b - a, cells[c]))
+    return pieces

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from itak_torch_rebuild_b200 import CudaCompute, CudaComputeError, KvDtype, _lib, paged
-from pagedref import PAGE, U, Batch, attend, attend_bound, rotate, rotation_bound, within
+from pagedref import PAGE, U, Batch, DeviceBatch, attend, attend_bound, plan_stream, plan_tc, rotate, rotation_bound, within
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -575,6 +575,44 @@ def test_results_do_not_change_between_runs():
     first = PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=300)
     for _ in range(3):
         assert torch.equal(PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=300), first)
+
+
+# ---- batches that give a CTA many tiles, or many cells ------------------------------------------------------------------------
+
+
+def run_device_batch(b, window=0, scale=None):
+    out = torch.full((b.total, b.hq, b.d), 7.0, dtype=b.t, device="cuda")
+    lse = torch.full((b.total, b.hq), 7.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), window=window, scale=scale, out=out, lse=lse, status=status)
+    assert int(status) == 0
+    b.check(out, lse, window, scale)
+    return out, lse
+
+
+def processors():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (4, 1, 128), (3, 1, 96)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_many_short_cells_one_behind_the_other(t, hq, hkv, d, window):
+    """Cells of one to three tiles, dozens in a CTA: blocks that both streams share (one of them often without a tile), blocks
+    of their own, and rows that see nothing of a stream's share, in every order."""
+    rng = np.random.default_rng(d + window)
+    n_seqs = 600
+    rows = [int(x) for x in rng.choice([1, 3, 20, 31, 40, 65, 100, 150], n_seqs)]
+    lens = [r + int(x) for r, x in zip(rows, rng.choice([0, 0, 5, 27, 100, 128, 260], n_seqs))]
+    pieces = plan_tc(rows, lens, hq // hkv, hkv, window, processors())
+    assert max(np.bincount([p[0] for p in pieces])) >= 5
+    assert {1, 2} <= {p[2] for p in pieces if p[1] <= 128} and {1, 2} <= {p[2] for p in pieces if p[1] > 128}
+    b = DeviceBatch(rows, lens, hq, hkv, d, t, 16, "head", seed=d)
+    first = run_device_batch(b, window)
+    for _ in range(5):
+        out, lse = torch.empty_like(first[0]), torch.empty_like(first[1])
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), window=window, out=out, lse=lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
 # ---- streams, graphs, workspaces ----------------------------------------------------------------------------------------
