@@ -221,7 +221,7 @@ class DeviceBatch:
 # How the attention kernels cut a launch into runs, one per CTA, restated from their sources: what a test's batch makes them do.
 
 def plan_tc(rows, lens, group, kv_heads, window, sms):
-    """The tensor-memory kernel's pieces: (CTA, pairs of the cell's block, tiles of the piece, tiles of the cell)."""
+    """The tensor-memory kernel's pieces: (CTA, pairs of the cell's block, tiles of the piece, tiles of the cell, cell)."""
     tile, block, cost, snap = 128, 256, 3, 1
     cells = []  # (pairs, tiles), in the launch's order
     for r, n in zip(rows, lens):
@@ -251,7 +251,7 @@ def plan_tc(rows, lens, group, kv_heads, window, sms):
         for c in range(len(cells)):
             a, b = max(lo, starts[c]), min(hi, starts[c] + cells[c][1])
             if a < b:
-                pieces.append((cta, cells[c][0], b - a, cells[c][1]))
+                pieces.append((cta, cells[c][0], b - a, cells[c][1], c))
     return pieces
 
 

@@ -615,6 +615,72 @@ def test_many_short_cells_one_behind_the_other(t, hq, hkv, d, window):
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
+def growing(q, k, v):
+    """Scores that climb along the keys, by several of the lazy steps, for the even rows; that fall for the odd ones; and that
+    swing for every third one."""
+    rows, n = q.shape[0], k.shape[0]
+    x = torch.linspace(0, 1, n, device="cuda")[:, None, None]
+    axis = torch.zeros(q.shape[-1], device="cuda")
+    swing, climb = axis.clone(), axis.clone()
+    climb[0::2], swing[1::2] = 1.0, 1.0
+    k = 0.3 * k + 6.0 * (x * climb + torch.sin(25 * x) * swing)
+    r = torch.arange(rows, device="cuda")[:, None, None]
+    q = 0.3 * q + torch.where(r % 3 == 2, 1.0, 0.0) * swing + torch.where(r % 2 == 0, 1.0, -1.0) * torch.where(r % 3 == 2, 0.0, 1.0) * climb
+    return q, k, v
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d,page,layout", [(64, 16, "token"), (128, 64, "head"), (128, 8, "head"), (40, 256, "token")])
+@pytest.mark.parametrize("shape", [None, growing])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_runs_of_many_tiles_on_the_tensor_memory_kernel(t, d, page, layout, shape, window):
+    """Batches that give a CTA's streams many tiles of a cell, of blocks that both share (two sequences of few rows) and of
+    blocks of their own, cells that two, three and more CTAs have a part of, and several cells in a CTA."""
+    rows, lens = [300, 40, 1, 129, 33, 260, 0, 64], [4100, 12000, 3000, 1500, 9001, 2049, 500, 6000]
+    if window:
+        rows, lens = 3 * rows, 3 * lens
+    hq, hkv = 8, 4
+    pieces = plan_tc(rows, lens, hq // hkv, hkv, window, processors())
+    own, shared = [p for p in pieces if p[1] > 128], [p for p in pieces if p[1] <= 128]
+    assert max(p[2] for p in own) >= 6 and max(p[2] for p in shared) >= 8
+    parts = np.bincount([p[4] for p in pieces])
+    assert {1, 2} <= set(parts) and (window or max(parts) >= 4)
+    assert any(p[2] < p[3] for p in own) and any(p[2] < p[3] for p in shared)
+    assert max(np.bincount([p[0] for p in pieces])) >= 2
+    b = DeviceBatch(rows, lens, hq, hkv, d, t, page, layout, seed=d + page, shape=shape)
+    first = run_device_batch(b, window)
+    for _ in range(3):
+        out, lse = torch.empty_like(first[0]), torch.empty_like(first[1])
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), window=window, out=out, lse=lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_whole_cells_of_many_tiles(t, d):
+    """More cells than CTAs, each of 20 tiles: nothing is joined, every stream runs its cells' tiles through."""
+    rows, lens = [160] * 40, [2560 - 37 * i for i in range(40)]
+    pieces = plan_tc(rows, lens, 2, 4, 0, processors())
+    assert max(p[2] for p in pieces) >= 16 and any(p[2] == p[3] >= 10 for p in pieces if p[1] > 128) and any(p[2] == p[3] >= 10 for p in pieces if p[1] <= 128)
+    run_device_batch(DeviceBatch(rows, lens, 8, 4, d, t, 32, "head", seed=d, shape=growing))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("shape", [None, growing])
+@pytest.mark.parametrize("window", [0, 2100])
+def test_runs_of_many_tiles_on_the_streaming_kernel(t, d, rows, shape, window):
+    """The same for its narrow and its wide block: 8 and 24 pairs, dozens of tiles of a cell in a CTA."""
+    hq, hkv = 64, 8
+    lens = [4000 + 311 * i for i in range(16)]
+    narrow = 8 if t is F32 else 16
+    block = 2 * narrow if rows * hq // hkv > narrow and d <= 128 else narrow
+    pieces = plan_stream([rows] * 16, lens, hq // hkv, hkv, window, block, (2 if d <= 128 else 1) * processors())
+    assert max(p[1] for p in pieces) >= 14 and any(p[1] < p[2] for p in pieces)
+    run_device_batch(DeviceBatch([rows] * 16, lens, hq, hkv, d, t, 16, "token", seed=d, shape=shape), window)
+
+
 # ---- streams, graphs, workspaces ----------------------------------------------------------------------------------------
 
 
