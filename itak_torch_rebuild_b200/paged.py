@@ -50,7 +50,7 @@ def _entry(name: str, descriptors: int):
     if fn is None:
         fn = _lib.load()[name]
         fn.restype = C.c_int
-        fn.argtypes = [C.c_char_p] * descriptors + [C.c_void_p, C.c_char_p, C.c_size_t]
+        fn.argtypes = [C.c_char_p] * descriptors + [C.c_void_p, C.c_void_p, C.c_size_t]
         _calls[name] = fn
     return fn
 
@@ -60,20 +60,18 @@ def _refuse(msg: str, code: int = _lib.ERR_INVALID_ARGUMENT):
 
 
 class _Reason(threading.local):
-    """A thread's buffer for the reason of a refusal, handed to every call: a call is made once, whatever it returns."""
+    """A thread's buffer for the reason of a refusal, handed to every call (by its address, which is what a call costs least
+    with): a call is made once, whatever it returns."""
 
     def __init__(self):
         self.text = C.create_string_buffer(_ERROR_LEN)
+        self.at = C.addressof(self.text)
+
+    def refuse(self, rc: int):
+        raise CudaComputeError(rc, self.text.value.decode("utf-8", "replace"))
 
 
 _reason = _Reason()
-
-
-def _call(fn, *args):
-    text = _reason.text
-    rc = fn(*args, text, _ERROR_LEN)
-    if rc != _lib.OK:
-        raise CudaComputeError(rc, text.value.decode("utf-8", "replace"))
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -184,7 +182,9 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                        1 if inverse else 0, dtype, dev, magnitude)
     except _OUT_OF_RANGE as e:
         _refuse(f"an argument is out of range: {e}")
-    _call(_entry("itk_rope_apply", 1), d, _raw_stream(dev) if stream is None else stream)
+    rc = _entry("itk_rope_apply", 1)(d, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
+    if rc != _lib.OK:
+        _reason.refuse(rc)
     return out
 
 
@@ -287,7 +287,9 @@ class PagedKv:
                              row_dtype, magnitude)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        _call(_entry("itk_paged_append", 3), self._kv, batch, a, _raw_stream(dev) if stream is None else stream)
+        rc = _entry("itk_paged_append", 3)(self._kv, batch, a, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
+        if rc != _lib.OK:
+            _reason.refuse(rc)
         return q_out
 
     def attention(self, q: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *, max_rows: int,
@@ -334,5 +336,7 @@ class PagedKv:
                                 max_rows, window, row_dtype, self._scale if scale is None else scale)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        _call(_entry("itk_paged_attention", 3), self._kv, batch, a, stream)
+        rc = _entry("itk_paged_attention", 3)(self._kv, batch, a, stream, _reason.at, _ERROR_LEN)
+        if rc != _lib.OK:
+            _reason.refuse(rc)
         return out

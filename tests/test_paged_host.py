@@ -4,6 +4,7 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
 import __graft_entry__ as entry
 from itak_torch_rebuild_b200 import CudaComputeError, _lib, paged
@@ -249,28 +250,50 @@ def test_missing_descriptors(lib):
         assert fn(C.byref(kv()), C.byref(batch()), None, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
 
 
-def test_a_failed_call_is_made_once():
-    """A call that reports an error may have run (an error of an asynchronous launch before it): it is not made again."""
+class OnCard:
+    """Stands in for a tensor on a device that is not there, as far as the calls look at it."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("name", ["itk_rope_apply", "itk_paged_append", "itk_paged_attention"])
+def test_a_failed_call_is_made_once(lib, name, monkeypatch):
+    """A call that reports an error may have run (an asynchronous launch before it failed): it is not made again, and its
+    reason is the one it gave."""
     made = []
 
     def entry(*args):
         made.append(args)
-        args[-2].value = b"launch failed: something before it"
+        C.memmove(args[-2], b"launch failed: something before it\0", 35)
         return _lib.ERR_CUDA if len(made) == 1 else _lib.OK
 
+    monkeypatch.setattr(paged, "_entry", lambda which, n: entry if which == name else pytest.fail(which))
+    i32 = lambda *shape: OnCard(torch.zeros(*shape, dtype=torch.int32))
+    x, f = OnCard(torch.zeros(4, 2, 64)), OnCard(torch.zeros(32, dtype=torch.float64))
+    kv = paged.PagedKv.__new__(paged.PagedKv)
+    kv._index, kv.head_dim, kv.kv_heads, kv._kv, kv._scale = 0, 64, 2, b"", 0.125
+    batch = (i32(1, 3), i32(2), i32(1))
+    call = {"itk_rope_apply": lambda: paged.rope_apply(x, i32(4), f, out=x, stream=7),
+            "itk_paged_append": lambda: kv.append(x, x, *batch, q=x, q_out=x, inv_freq=f, stream=7),
+            "itk_paged_attention": lambda: kv.attention(x, *batch, max_rows=4, out=x, workspace=OnCard(torch.zeros(8, dtype=torch.uint8)), stream=7)}[name]
     with pytest.raises(CudaComputeError) as e:
-        paged._call(entry, b"descriptor", 7)
+        call()
     assert e.value.code == _lib.ERR_CUDA and e.value.msg == "launch failed: something before it"
-    assert len(made) == 1 and made[0][:2] == (b"descriptor", 7)
-    paged._call(entry, b"descriptor", 7)
+    assert len(made) == 1
+    call()
     assert len(made) == 2
 
 
 @pytest.mark.parametrize("name,args", [("itk_rope_apply", 1), ("itk_paged_append", 3), ("itk_paged_attention", 3)])
-def test_every_entry_point_is_called_once_and_keeps_its_reason(lib, name, args, monkeypatch):
-    """The library's own refusals through the packed descriptors' path, its first call already carrying the buffer."""
-    fn = paged._entry(name, args)
-    made = []
+def test_the_library_writes_its_reason_where_the_call_says(lib, name, args):
+    assert paged._entry(name, args)(*[None] * args, None, paged._reason.at, 256) == _lib.ERR_INVALID_ARGUMENT
     with pytest.raises(CudaComputeError) as e:
-        paged._call(lambda *a: made.append(a) or fn(*a), *[None] * args, None)
-    assert len(made) == 1 and "null pointer" in e.value.msg
+        paged._reason.refuse(_lib.ERR_INVALID_ARGUMENT)
+    assert "null pointer" in e.value.msg
