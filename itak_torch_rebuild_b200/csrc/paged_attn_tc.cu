@@ -662,7 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const uint32_t i = warp >> 2, r = tid & 127;
         const uint32_t lane_base = ((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_base + i * kTile, tO = tmem + lane_base + kTmemO + i * D;
-        const uint32_t tOther = tmem + lane_base + kTmemO + (1 - i) * D;
         const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);  // the queries carry a negative scale's sign
         const bool flip = p.scale_log2 < 0.f;
         const uint32_t head_dim = p.pool.head_dim;
@@ -927,34 +926,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
 
             // ---- the cell's end ----------------------------------------------------------------------------------------
             const bool whole = it.n == it.T, twin = it.twin != 0;
-            float f0 = 1.f, f1 = 0.f;  // weights of the own and the other stream's rows
-            bool other_any = false;
+            float f0 = 1.f, f1 = 0.f;  // twin: weights of stream 0's and stream 1's rows
+            const bool any0 = twin ? it.a[0] < it.e[0] : any, any1 = twin && it.a[1] < it.e[1];
             if (twin) {
-                // Rows are the same in both streams and sit in the same lanes: each warpgroup takes half of the channels.
-                other_any = it.a[1 - i] < it.e[1 - i];
+                // Rows are the same in both streams and sit in the same lanes: each warpgroup takes half of the channels.  Both
+                // add stream 0 and stream 1 in this order: the sum that one hands to a join has to be the other's, to the
+                // bit, or a result's bits would depend on which CTA comes last.
                 exchange[tid] = make_float2(m, l);
                 tc::fence_before_sync();
                 both_sync();
                 tc::fence_after_sync();
                 const float2 x = exchange[tid ^ 128];
-                const float M = m != m || x.x != x.x ? NAN : fmaxf(m, x.x);
-                f0 = m == -INFINITY ? 0.f : fast_exp2(m - M);
-                f1 = x.x == -INFINITY ? 0.f : fast_exp2(x.x - M);
-                l = l * f0 + x.y * f1;
+                const float m0 = i == 0 ? m : x.x, m1 = i == 0 ? x.x : m, l0 = i == 0 ? l : x.y, l1 = i == 0 ? x.y : l;
+                const float M = m0 != m0 || m1 != m1 ? NAN : fmaxf(m0, m1);
+                f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - M);
+                f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - M);
+                l = fmaf(l0, f0, l1 * f1);
                 m = M;
             }
             const uint32_t row = it.q.row0 + pair / group, head = it.kvh * group + pair % group;
             const uint32_t c0 = twin ? i * (D / 2) : 0u, c1 = twin ? c0 + D / 2 : D;  // channels of this thread
             const int64_t dst = live ? static_cast<int64_t>(row * p.out_row + head * head_dim) : -1;
+            const uint32_t tO0 = twin ? tmem + lane_base + kTmemO : tO, tO1 = tmem + lane_base + kTmemO + D;
             auto output16 = [&](uint32_t ch, float (&f)[16]) {
                 uint32_t o[16], y[16] = {};
-                tc::tmem_ld16(tO + ch, o);
-                if (twin) tc::tmem_ld16(tOther + ch, y);
+                tc::tmem_ld16(tO0 + ch, o);
+                if (twin) tc::tmem_ld16(tO1 + ch, y);
                 tc::tmem_wait_ld();
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
-                    f[u] = any ? __uint_as_float(o[u]) : 0.f;
-                    if (twin) f[u] = f[u] * f0 + (other_any ? __uint_as_float(y[u]) * f1 : 0.f);
+                    f[u] = any0 ? __uint_as_float(o[u]) : 0.f;
+                    if (twin) f[u] = fmaf(f[u], f0, any1 ? __uint_as_float(y[u]) * f1 : 0.f);
                 }
             };
             // A finished row goes out by way of shared memory, so that a warp stores whole rows: thread by thread, 32 rows at

@@ -655,6 +655,32 @@ def test_runs_of_many_tiles_on_the_tensor_memory_kernel(t, d, page, layout, shap
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
+def halves_alike(q, k, v):
+    half = v.shape[-1] // 2
+    return q, k, torch.cat((v[..., :half], v[..., :half]), -1)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,parts", [([4000, 2300, 9001], {5, 8, 18}), ([1500, 700] * 12, {1, 2})])
+def test_both_halves_of_the_channels_are_weighed_alike(t, d, lens, parts):
+    """Blocks that both streams share are finished by two warpgroups, half of the channels each, and joined by whichever CTA
+    comes last: values whose halves are the same give halves that are the same, to the bit - a sum that the two held
+    differently would also make the bits of a result depend on who came last."""
+    rows = ([33, 40, 50] * 8)[:len(lens)]
+    pieces = plan_tc(rows, lens, 2, 4, 0, processors())
+    assert all(p[1] <= 128 for p in pieces)
+    if processors() == 148:
+        assert parts <= set(np.bincount([p[4] for p in pieces]))
+    b = DeviceBatch(rows, lens, 8, 4, d, t, 16, "head", seed=d, shape=halves_alike)
+    first = run_device_batch(b)
+    assert torch.equal(first[0][..., :d // 2], first[0][..., d // 2:])
+    for _ in range(20):
+        out, lse = torch.empty_like(first[0]), torch.empty_like(first[1])
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), out=out, lse=lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 def test_whole_cells_of_many_tiles(t, d):
