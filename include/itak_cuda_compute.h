@@ -558,8 +558,8 @@ typedef struct itk_paged_kv {
  * would be stored there is dropped) and raises bit 0 of *status; of a sequence that is longer than its row of the table
  * (or than 2^30 keys) positions stay what kv_len says, new rows behind the last column are not stored and keys there are
  * not seen (bit 1; lengths count as 2^31 - 1 at most); new rows that reach before position 0 see nothing and are not stored (bit 2); starts that run backwards
- * or past total_rows are cut (bit 3).  Bit 4: a wait inside the tensor-core kernel ran out and the call's outputs are
- * not valid.  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] are neither
+ * or past total_rows are cut (bit 3).  Bit 4: a wait inside the tensor-core kernel ran out (see
+ * itk_paged_attention_wait_limit).  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] are neither
  * read nor written. */
 typedef struct itk_paged_batch {
     const uint32_t* table;     /* [n_seqs][table_stride], table_width columns used */
@@ -600,8 +600,7 @@ int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* batch, const
  * what lies outside a sequence's keys never reaches a result.
  *
  * `workspace`: device memory of itk_paged_attention_workspace() bytes, 256-byte aligned, that must be zero before its
- * first use; every call leaves what it needs of it zero again (after a call that raised bit 4 of *status the caller clears
- * it).  Calls that may run at the same time need one each.
+ * first use; every call leaves what it needs of it zero again.  Calls that may run at the same time need one each.
  *
  * The same call gives the same bits: partial results of a key range that several CTAs shared are joined in one order. */
 typedef struct itk_paged_attention_desc {
@@ -619,6 +618,11 @@ typedef struct itk_paged_attention_desc {
 } itk_paged_attention_desc;
 int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch* batch, const itk_paged_attention_desc* d,
                         void* cuda_stream, char* error_text, size_t error_text_len);
+/* Bound of every wait inside the tensor-core kernel of the calls that follow, in units of 1024 SM clocks, for the whole
+ * process; 0 = the default (about a second), at most 2^22.  No wait is known that could take that long: the bound is there so
+ * that a fault ends the call.  Where a wait runs out, the rows (and lse) that its part of the launch still had to do come
+ * out as NaN, bit 4 of *status is raised, and the workspace is fit for the next call. */
+int itk_paged_attention_wait_limit(uint32_t kclocks);
 /* Bytes of workspace that serve every itk_paged_attention call on `device` whatever its batch; 0 without a device. */
 uint64_t itk_paged_attention_workspace(int32_t device);
 

@@ -286,6 +286,7 @@ SIGNATURES = {
     "itk_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(PagedAttentionDesc), _vp,
                                       C.c_char_p, _sz]),
     "itk_paged_attention_workspace": (_u64, [C.c_int32]),
+    "itk_paged_attention_wait_limit": (C.c_int, [_u32]),
     "itk_rope_rows": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_float, _vp, C.c_char_p, _sz]),
     "itk_decode_attention_noalloc": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32p, _u32p, _vp, _vp, _u32, _vp,
                                                C.c_char_p, _sz]),

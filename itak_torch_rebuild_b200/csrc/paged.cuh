@@ -95,6 +95,7 @@ struct AttnParams {
     unsigned int* tickets;  // zero between launches
     float* part_ml;         // [part][row][2]: running maximum (log2 domain) and sum
     float* part_o;          // [part][row][D]: unnormalised outputs
+    long long wait_clocks;  // bound of the tensor-memory kernel's waits, SM clocks
 };
 
 // Takes a ticket: orders the block's stores before it (all of them precede a barrier that the caller has passed) and what

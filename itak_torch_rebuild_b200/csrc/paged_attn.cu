@@ -21,6 +21,10 @@ cudaError_t multiprocessors(int device, uint32_t* sms) {
     return cudaSuccess;
 }
 
+// The bound of the tensor-memory kernel's waits: about a second unless itk_paged_attention_wait_limit says otherwise.
+constexpr long long kWaitClocks = 2000000000ll;
+std::atomic<uint32_t> wait_kclocks{0};
+
 constexpr uint64_t kAlign = 256;
 uint64_t round_up(uint64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
@@ -49,6 +53,12 @@ extern "C" uint64_t itk_paged_attention_workspace(int32_t device) {
     uint32_t sms = 0;
     if (itk::paged::multiprocessors(device, &sms) != cudaSuccess) return 0;
     return itk::paged::layout_of(sms).bytes;
+}
+
+extern "C" int itk_paged_attention_wait_limit(uint32_t kclocks) {
+    if (kclocks > 1u << 22) return ITK_ERR_INVALID_ARGUMENT;
+    itk::paged::wait_kclocks.store(kclocks, std::memory_order_relaxed);
+    return 0;
 }
 
 extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch* batch, const itk_paged_attention_desc* d,
@@ -97,6 +107,8 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     p.tickets = reinterpret_cast<unsigned int*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + l.ml);
     p.part_o = reinterpret_cast<float*>(ws + l.o);
+    const uint32_t limit = wait_kclocks.load(std::memory_order_relaxed);
+    p.wait_clocks = limit != 0 ? static_cast<long long>(limit) << 10 : kWaitClocks;
     // Few (row, head) pairs per KV head stream, many go to tensor memory.  Measured at 2055-2487 keys, 32 / 8 heads of 128
     // channels (streaming : tensor memory, us):
     //   16-bit rows, 16 pairs   16 sequences 37 : 53     2 sequences 17 : 19

@@ -65,7 +65,7 @@ constexpr float kRescaleStep = 8.f;
 constexpr uint32_t kCellCost = 3, kSnap = 1;
 constexpr uint32_t kSmemBytes = 232448;   // all that a block can have
 constexpr uint32_t kTailBytes = 3u << 10;    // mbarriers, the roles' items, the streams' exchange
-constexpr long long kWaitClocks = 2000000000ll;  // about a second
+constexpr long long kRestClocks = 2000000000ll;  // about a second, for what is in flight to come to rest when a call ends early
 
 template <typename T>
 struct RowTraits;
@@ -254,7 +254,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* const smem = smem_raw;
     if ((smem_u32(smem) & 1023u) != 0) {  // (the tiles' swizzle goes by address bits; never so far)
+        after_predecessor();
         if (threadIdx.x == 0) raise(p.batch, kWaitRanOut);
+        const uint32_t rows = min(p.batch.row_start[p.batch.n_seqs], p.batch.total_rows);
+        for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
+            for (uint32_t c = threadIdx.x; c < p.q_heads * p.pool.head_dim; c += kThreads) static_cast<T*>(p.out)[row * p.out_row + c] = from_f32<T>(NAN);
+            if (p.lse)
+                for (uint32_t h = threadIdx.x; h < p.q_heads; h += kThreads) p.lse[static_cast<uint64_t>(row) * p.q_heads + h] = NAN;
+        }
         return;
     }
     const uint32_t qbuf = smem_u32(smem), ring = qbuf + 2 * Sh::kQ, tail = ring + NST * Sh::kStage;
@@ -444,13 +451,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     tc::fence_after_sync();
     const uint32_t tmem = word[0];
     // Waits that ran out end the call: every role leaves (or, the softmax threads, walks on through their barriers without
-    // waiting), once what the role has in flight has come to rest.
+    // waiting), once what the role has in flight has come to rest.  A warp of the softmax that has given up is `dead`: its rows,
+    // of this cell and of all that follow in the run, become NaN - by way of a maximum and sum of NaN, which every join hands
+    // on - and its tickets are taken all the same, so that the workspace is as the next launch wants it.
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
         if (tc::mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
         while (!tc::mbar_try_wait(bar, parity)) {
             if (*abort_flag != 0) return false;
-            if (clock64() - t0 > kWaitClocks) {
+            if (clock64() - t0 > p.wait_clocks) {
                 *abort_flag = 1;
                 raise(p.batch, kWaitRanOut);
                 return false;
@@ -468,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const uint32_t slot = lane / NP, panel = lane % NP;  // lane's page within the tile, and its 64 channels
             const uint32_t row_at = slot << box_shift;           // its first row in the tile
             uint32_t cnt = 0, landed = 0;
-            bool ok = true;
+            bool ok = true, landing = false;
             Item& it = items[6];
             do {
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
@@ -503,9 +512,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             tma_load(dst + panel * Sh::kPanel + row_at * 128, v == 0 ? &kmap : &vmap, signal, panel * 64,
                                      static_cast<int32_t>(key & ((1u << shift) - 1u)), static_cast<int32_t>(it.kvh), static_cast<int32_t>(page));
                         if (v == 1 && cut) {
+                            landing = true;
                             if (!wait(bar_land, landed & 1u)) ok = false;
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
+                            landing = false;
                             ++landed;
                             unsigned char* const rows = smem + (dst - qbuf);
                             const uint32_t gone = kTile - (b - a);
@@ -527,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             } while (ok && it.more);
             if (!ok) {  // copies in flight land before the block's shared memory goes
                 for (uint32_t n = cnt > NST ? cnt - NST : 0u; n < cnt; ++n)
-                    tc::mbar_wait_bounded(bar_full + 8 * (n % NST), (n / NST) & 1u, kWaitClocks);
-                tc::mbar_wait_bounded(bar_land, landed & 1u, kWaitClocks);
+                    tc::mbar_wait_bounded(bar_full + 8 * (n % NST), (n / NST) & 1u, kRestClocks);
+                if (landing) tc::mbar_wait_bounded(bar_land, landed & 1u, kRestClocks);
             }
         } else if ((warp == kMmaWarp || warp == kMmaWarp + 2) && works && lane == 0) {
             // ---------------- products of one stream ---------------------------------------------------------------------
@@ -550,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const long long t0 = clock64();
                 while (static_cast<int32_t>(issued[1 - i] - n) <= 0) {
                     if (*abort_flag != 0) return false;
-                    if (clock64() - t0 > kWaitClocks) {
+                    if (clock64() - t0 > p.wait_clocks) {
                         *abort_flag = 1;
                         raise(p.batch, kWaitRanOut);
                         return false;
@@ -653,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 run.next(it);
             } while (ok && it.more);
             tc::mma_commit(bar_done);
-            tc::mbar_wait_bounded(bar_done, 0u, kWaitClocks);
+            tc::mbar_wait_bounded(bar_done, 0u, kRestClocks);
         }
         __syncwarp();
     } else {
@@ -925,6 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             }
 
             // ---- the cell's end ----------------------------------------------------------------------------------------
+            if (dead) m = l = NAN;
             const bool whole = it.n == it.T, twin = it.twin != 0;
             float f0 = 1.f, f1 = 0.f;  // twin: weights of stream 0's and stream 1's rows
             const bool any0 = twin ? it.a[0] < it.e[0] : any, any1 = twin && it.a[1] < it.e[1];
@@ -949,10 +961,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             const int64_t dst = live ? static_cast<int64_t>(row * p.out_row + head * head_dim) : -1;
             const uint32_t tO0 = twin ? tmem + lane_base + kTmemO : tO, tO1 = tmem + lane_base + kTmemO + D;
             auto output16 = [&](uint32_t ch, float (&f)[16]) {
-                uint32_t o[16], y[16] = {};
-                tc::tmem_ld16(tO0 + ch, o);
-                if (twin) tc::tmem_ld16(tO1 + ch, y);
-                tc::tmem_wait_ld();
+                uint32_t o[16] = {}, y[16] = {};
+                if (!dead) {
+                    tc::tmem_ld16(tO0 + ch, o);
+                    if (twin) tc::tmem_ld16(tO1 + ch, y);
+                    tc::tmem_wait_ld();
+                }
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
                     f[u] = any0 ? __uint_as_float(o[u]) : 0.f;
@@ -994,23 +1008,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             };
             auto inverse = [](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };
             if (whole) {
-                if (!dead) {
-                    const float inv = inverse(l);
+                const float inv = inverse(l);
 #pragma unroll 1
-                    for (uint32_t ch = c0; ch < c1; ch += 16) {
-                        float f[16];
-                        output16(ch, f);
-                        stage16(ch, f, inv);
-                    }
-                    send_rows();
-                    if (live && (i == 0 || !twin)) put_lse(row, head, m, l);
+                for (uint32_t ch = c0; ch < c1; ch += 16) {
+                    float f[16];
+                    output16(ch, f);
+                    stage16(ch, f, inv);
                 }
+                send_rows();
+                if (live && (i == 0 || !twin)) put_lse(row, head, m, l);
             } else {
                 // The part goes out channels by rows: a warp's store is 512 contiguous bytes.
                 const uint32_t part = it.off == 0 ? 2 * cta + 1 : 2 * cta;
                 float4* const all = reinterpret_cast<float4*>(p.part_o);
                 float2* const pml = reinterpret_cast<float2*>(p.part_ml);
-                if (!dead) {
+                {
 #pragma unroll 1
                     for (uint32_t ch = c0; ch < c1; ch += 16) {
                         float f[16];
@@ -1038,7 +1050,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 // The parts lie in slots 2 first + 1 (where the cell begins), 2 (first + 1), 2 (first + 2), ...
                 const uint32_t n_parts = last - first + 1;
                 auto slot_of = [&](uint32_t k) { return static_cast<size_t>(2 * (first + k) + (k == 0 ? 1 : 0)); };
-                if (word[1] != 0u && !dead) {
+                if (word[1] != 0u) {
                     if (n_parts == 2) {
                         // Every thread joins its own row, its own part still in tensor memory - in the order of the parts,
                         // whichever of the two came last, so that the same call gives the same bits.

@@ -206,6 +206,21 @@ def attention_workspace(device) -> torch.Tensor:
     return ws
 
 
+def release_workspaces():
+    """Gives up this module's own workspaces (39 MB for every stream that has called without one), once their devices have
+    come to rest.  Later calls make new ones."""
+    for device in {device for device, _ in _workspaces}:
+        torch.cuda.synchronize(device)
+    _workspaces.clear()
+
+
+def wait_limit(kclocks: int = 0):
+    """Bounds the waits inside the tensor-core kernel, in units of 1024 SM clocks (0: about a second;
+    ``itk_paged_attention_wait_limit``).  Where one runs out, rows come out as NaN and bit 4 of ``status`` is raised."""
+    if not 0 <= kclocks <= 0xffffffff or _lib.load().itk_paged_attention_wait_limit(kclocks) != _lib.OK:
+        _refuse(f"the bound of a wait is 0..2^22 x 1024 clocks, got {kclocks}")
+
+
 class PagedKv:
     """A pair of page pools: ``k`` and ``v`` 4-dimensional f16 or bf16 tensors of the same shape and strides,
     ``[pages][kv_heads][page_size][head_dim]`` with ``layout="head"`` or ``[pages][page_size][kv_heads][head_dim]`` with

@@ -707,6 +707,52 @@ def test_runs_of_many_tiles_on_the_streaming_kernel(t, d, rows, shape, window):
     run_device_batch(DeviceBatch([rows] * 16, lens, hq, hkv, d, t, 16, "token", seed=d, shape=shape), window)
 
 
+@pytest.fixture
+def short_waits():
+    yield paged.wait_limit
+    torch.cuda.synchronize()
+    paged.wait_limit(0)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_wait_that_runs_out_shows(short_waits, t, d):
+    """With bounds far below what a tile takes: rows come out as they would have or as NaN, never as something else, the
+    status says so, and the workspace serves the next call."""
+    rows, lens = [300, 40, 1, 129, 33, 260, 0, 64] * 2, [1100, 4000, 300, 500, 2001, 1049, 500, 900] * 2
+    b = DeviceBatch(rows, lens, 8, 4, d, t, 16, "head", seed=d)
+    pieces = plan_tc(rows, lens, 2, 4, 0, processors())
+    parts = np.bincount([p[4] for p in pieces])
+    assert {1, 2} <= set(parts) and max(parts) >= 3 and max(np.bincount([p[0] for p in pieces])) >= 2
+    ws, status = paged.attention_workspace("cuda:0"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    n_tickets = 4 * 2 * processors()
+
+    def run():
+        out, lse = torch.full((b.total, 8, d), 7.0, dtype=t, device="cuda"), torch.full((b.total, 8), 7.0, device="cuda")
+        PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=300, out=out, lse=lse, workspace=ws, status=status)
+        torch.cuda.synchronize()
+        assert bool((ws[:n_tickets] == 0).all())
+        return out, lse
+
+    want = run()
+    assert int(status) == 0
+    lost = []
+    for limit in (1, 3, 8):
+        short_waits(limit)
+        status.zero_()
+        out, lse = run()
+        gone = torch.isnan(lse)
+        lost.append(int(gone.sum()))
+        assert int(status) in ((16,) if lost[-1] else (0, 16))
+        assert bool(torch.isnan(out[gone]).all())
+        assert torch.equal(out[~gone], want[0][~gone]) and torch.equal(lse[~gone], want[1][~gone])
+    assert lost[0] > 0
+    short_waits(0)
+    status.zero_()
+    again = run()
+    assert int(status) == 0 and torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
 # ---- streams, graphs, workspaces ----------------------------------------------------------------------------------------
 
 
@@ -860,6 +906,16 @@ def test_rows_of_another_number_of_dimensions_are_refused():
             PagedOf(b).append(k, k, b.table, b.row_start, b.kv_len)
         with pytest.raises(CudaComputeError):
             PagedOf(b).attention(k, b.table, b.row_start, b.kv_len, max_rows=1)
+
+
+def test_the_modules_workspaces_are_given_up():
+    b = Batch([1], [400], 4, 2, 64, F16, 16, "head")
+    PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1)
+    assert paged._workspaces
+    paged.release_workspaces()
+    assert not paged._workspaces
+    b.check(PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=1))
+    assert len(paged._workspaces) == 1
 
 
 def test_a_workspace_that_is_too_small_is_refused():

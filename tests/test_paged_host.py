@@ -250,6 +250,15 @@ def test_missing_descriptors(lib):
         assert fn(C.byref(kv()), C.byref(batch()), None, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
 
 
+def test_wait_limits(lib):
+    for bad in (-1, (1 << 22) + 1, 1 << 32):
+        with pytest.raises(CudaComputeError) as e:
+            paged.wait_limit(bad)
+        assert e.value.code == _lib.ERR_INVALID_ARGUMENT
+    for fine in (1, 1 << 22, 0):
+        paged.wait_limit(fine)
+
+
 class OnCard:
     """Stands in for a tensor on a device that is not there, as far as the calls look at it."""
 
