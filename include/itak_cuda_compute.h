@@ -595,7 +595,10 @@ int itk_paged_append(const itk_paged_kv* kv, const itk_paged_batch* batch, const
  * not NULL the natural logarithm of each row's sum of exponentials.  A row that sees nothing gives zeros and -infinity.
  * Any number of rows per sequence: one (decode), a few (a block to verify) or a prompt's chunk; max_rows is the caller's
  * bound of it and only chooses between kernels - results hold whatever the device-side row counts are.
- * Head dimensions, page sizes and row types as above.  Queries of f32 rows stay below 65504 in magnitude.
+ * Head dimensions, page sizes and row types as above.  Scores, maxima, sums and outputs are f32; what is rounded to fewer
+ * bits: with 16-bit rows each softmax weight, to the pages' type, before it meets its V row (the sum takes it unrounded); with
+ * f32 rows queries and weights, to two halfs (2^-22 of a weight, and never more than 2^-32 of the row's largest where that is
+ * more).  Queries of f32 rows stay below 65504 in magnitude.
  * A value that is not finite in a visible V row may reach every row of the batch block it is visible to some of;
  * what lies outside a sequence's keys never reaches a result.
  *

@@ -81,6 +81,19 @@ __device__ __forceinline__ Seq seq_of(const Batch& b, uint32_t s, uint32_t page_
     return q;
 }
 
+// Softmax weights are kept 2^kLift times larger than 2^(c s - m) where they are rounded to halfs: with a running maximum that lags
+// by up to 2^8 they reach 2^15, and small ones stay clear of the type's subnormal steps - 2^-32 of the row's largest instead of
+// 2^-25, which over 2^15 keys under one that outshines them would add up to 1e-3 of a result.  The sum scales alike, and
+// is scaled back for the log-sum-exp.  bf16 has the range of f32 and needs none.
+template <typename P>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 7.f;
+template <typename P>
+constexpr float kUnlift = 1.f;
+template <>
+constexpr float kUnlift<__half> = 1.f / 128.f;
+
 // What an attention launch gets (both kernels).
 struct AttnParams {
     Pool pool;

@@ -1,7 +1,7 @@
 // Attention of a ragged batch over the pages of its sequences, for calls with few (row, head) pairs per KV head: decode
 // steps and short verify blocks - and, at any cost in speed, every shape the tensor-memory kernel does not take.
 //
-// For one row at position p and one head:  out = sum_k w_k v_k / sum_k w_k,  w_k = 2^(c q.k - m),  c = scale * log2(e),
+// For one row at position p and one head:  out = sum_k w_k v_k / sum_k w_k,  w_k = 2^(c q.k - m) (times a constant, see kLift),  c = scale * log2(e),
 // over the keys p - window < k <= p, with the running maximum m and the sums kept in f32 in one pass over the keys.
 //
 // Bound: HBM.  Every K and V row of a (sequence, KV head) is read once for all the pairs of the KV head's group (up to
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
                 }
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    const float base = m[t][j] == -INFINITY ? 0.f : m[t][j];
+                    const float base = m[t][j] == -INFINITY ? 0.f : m[t][j] - kLift<P>;
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
                 }
                 if (c4 == 0 && p.lse)
                     p.lse[static_cast<uint64_t>(C.row0 + row) * p.q_heads + head] =
-                        sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+                        sum > 0.f || sum != sum ? (top + log2f(sum * kUnlift<P>)) * 0.69314718055994530942f : -INFINITY;
             };
             const uint32_t pairs = min(C.rows * group - C.b * PB, PB);
 #pragma unroll

@@ -1,7 +1,8 @@
 // Attention of a ragged batch over the pages of its sequences on the 5th-generation tensor cores, for calls with many
 // (row, head) pairs per KV head: prompt chunks, and verify blocks beyond the streaming kernel's 16 pairs.
 //
-//   S = Q K^T,  P = 2^(c S - m),  O += P V,  out = O / sum P,   c = scale * log2(e), one pass over the keys.
+//   S = Q K^T,  P = 2^(c S - m),  O += P V,  out = O / sum P,   c = scale * log2(e), one pass over the keys (P times a
+//   constant where the pages are halfs, see kLift).
 //
 // A cell is (sequence, KV head, block of 256 pairs); a pair is a query row and one of the heads of the KV head's group, so
 // that all heads of a group share the K and V tiles.  One CTA per SM walks an equal, contiguous run of the launch's
@@ -849,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         l *= f;
                     }
                     if (!(mx < INFINITY)) m = NAN;  // a NaN or +infinity among the scores: the row is NaN from here on
-                    const float nm = m == -INFINITY ? 0.f : -m;
+                    const float nm = m == -INFINITY ? 0.f : kLift<P> - m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -894,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         l *= f;
                     }
                     if (!(mx < INFINITY)) m = NAN;
-                    const uint64_t c2 = pair_of(c, c), nm2 = pair_of(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+                    const uint64_t c2 = pair_of(c, c), nm2 = pair_of(m == -INFINITY ? 0.f : kLift<P> - m, m == -INFINITY ? 0.f : kLift<P> - m);
                     uint64_t sum2[2] = {0u, 0u};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -1004,7 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             auto put_lse = [&](uint32_t lrow, uint32_t lhead, float top, float sum) {
                 if (p.lse)
                     p.lse[static_cast<uint64_t>(lrow) * p.q_heads + lhead] =
-                        sum > 0.f || sum != sum ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+                        sum > 0.f || sum != sum ? (top + log2f(sum * kUnlift<P>)) * 0.69314718055994530942f : -INFINITY;
             };
             auto inverse = [](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };
             if (whole) {

@@ -580,13 +580,13 @@ def test_results_do_not_change_between_runs():
 # ---- batches that give a CTA many tiles, or many cells ------------------------------------------------------------------------
 
 
-def run_device_batch(b, window=0, scale=None):
+def run_device_batch(b, window=0, scale=None, **kw):
     out = torch.full((b.total, b.hq, b.d), 7.0, dtype=b.t, device="cuda")
     lse = torch.full((b.total, b.hq), 7.0, device="cuda")
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     PagedOf(b).attention(b.q, b.table, b.row_start, b.kv_len, max_rows=max(b.rows), window=window, scale=scale, out=out, lse=lse, status=status)
     assert int(status) == 0
-    b.check(out, lse, window, scale)
+    b.check(out, lse, window, scale, **kw)
     return out, lse
 
 
@@ -705,6 +705,25 @@ def test_runs_of_many_tiles_on_the_streaming_kernel(t, d, rows, shape, window):
     pieces = plan_stream([rows] * 16, lens, hq // hkv, hkv, window, block, (2 if d <= 128 else 1) * processors())
     assert max(p[1] for p in pieces) >= 14 and any(p[1] < p[2] for p in pieces)
     run_device_batch(DeviceBatch([rows] * 16, lens, hq, hkv, d, t, 16, "token", seed=d, shape=shape), window)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("below", [9.3, 13.2, 16.4, 18.7, 21.55])
+def test_one_key_far_above_many_small_ones(t, d, rows, below):
+    """A key whose weight is 2^below times that of each of some thousand others, which all count the same way: a step of the
+    weights' type, times their number, must not show.  Half pages keep a weight to 2^-25 in a scale where the largest is 2^7 at
+    least, 2^-32 of it; bf16 has no such step."""
+    def sink(q, k, v):
+        q, k, v = torch.zeros_like(q), torch.zeros_like(k), torch.ones_like(v)
+        # the first key's score above the others': 4 k times 2^-x, a scale of ln(2) and a common factor
+        q[..., 0], k[..., 0] = 4.0, -below / 4.0
+        k[0, :, 0], v[0] = 0.0, 0.0
+        return q, k, v
+
+    b = DeviceBatch([rows] * 2, [8192, 3001], 4, 2, d, t, 16, "head", shape=sink)
+    run_device_batch(b, scale=math.log(2.0), step=0.0 if t is BF16 else 2.0 ** -32)
 
 
 @pytest.fixture
