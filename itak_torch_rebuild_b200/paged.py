@@ -7,6 +7,10 @@ the tensors' device (or on ``stream``, a handle), allocates nothing on the devic
 writes it, as torch counts it) and, once per stream, a workspace, and raises :class:`CudaComputeError` with the library's text
 when it is refused.  Tensors that a call on ``stream`` shares with other streams are the caller's to order, as in torch.
 
+No gradient passes through these calls: while gradients are enabled they refuse tensors that require one (``rope_apply`` with
+``inverse=True`` is the rotation's gradient, for a backward pass of the caller's).  What they write counts as written in place,
+so that autograd notices when a backward pass still wants the old values.
+
 A batch: sequence ``s`` owns the packed rows ``[row_start[s], row_start[s + 1])`` and ``kv_len[s]`` keys, its new rows
 included; the key of position ``p`` is row ``p % page_size`` of page ``table[s][p // page_size]``.  ``table``,
 ``row_start`` and ``kv_len`` are int32 tensors on the device, read when the work runs, so a captured graph follows them.
@@ -45,13 +49,11 @@ _calls: dict = {}
 
 
 def _entry(name: str, descriptors: int):
-    """The library's entry point taking packed descriptors."""
-    fn = _calls.get(name)
-    if fn is None:
-        fn = _lib.load()[name]
-        fn.restype = C.c_int
-        fn.argtypes = [C.c_char_p] * descriptors + [C.c_void_p, C.c_void_p, C.c_size_t]
-        _calls[name] = fn
+    """The library's entry point taking packed descriptors, looked up once (``_calls``)."""
+    fn = _lib.load()[name]
+    fn.restype = C.c_int
+    fn.argtypes = [C.c_char_p] * descriptors + [C.c_void_p, C.c_void_p, C.c_size_t]
+    _calls[name] = fn
     return fn
 
 
@@ -111,6 +113,17 @@ def _new_rows(shape, dtype, device: int, stream: Optional[int]) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+# Counts tensors as written to, for autograd's check of what it has saved.
+_written = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
+
+_grad_enabled = torch.is_grad_enabled
+
+
+def _no_gradient():
+    _refuse("no gradient passes through this call: detach its tensors, or call it under torch.no_grad()")
+
+
 def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
     """The row stride of a ``[rows][heads][head_dim]`` tensor whose heads are contiguous."""
     if t.dtype is not dtype or t.get_device() != device:
@@ -165,7 +178,9 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     dtype, dev = _ROW_DTYPES.get(x.dtype), x.get_device()
     if dtype is None or dev < 0 or x.dim() != 3:
         _refuse(f"x must be an f32, f16 or bf16 [rows][heads][head_dim] tensor on a CUDA device, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    shape = x.shape
+    if _grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+        _no_gradient()
+    shape, given = x.shape, out is not None
     if out is None:
         out = _new_rows(shape, x.dtype, dev, stream)
     elif out.dtype is not x.dtype or out.get_device() != dev or out.shape != shape:
@@ -182,9 +197,11 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                        1 if inverse else 0, dtype, dev, magnitude)
     except _OUT_OF_RANGE as e:
         _refuse(f"an argument is out of range: {e}")
-    rc = _entry("itk_rope_apply", 1)(d, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
+    rc = (_calls.get("itk_rope_apply") or _entry("itk_rope_apply", 1))(d, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
     if rc != _lib.OK:
         _reason.refuse(rc)
+    if given:
+        _written([out])
     return out
 
 
@@ -276,6 +293,9 @@ class PagedKv:
         row_dtype = _ROW_DTYPES.get(dtype)
         if row_dtype is None or k.dim() != 3:
             _refuse(f"rows must be f32, f16 or bf16 [rows][{self.kv_heads}][{d}], got {dtype} {tuple(k.shape)}")
+        if _grad_enabled() and (k.requires_grad or v.requires_grad or self.k.requires_grad or self.v.requires_grad
+                                or (q is not None and q.requires_grad) or (q_out is not None and q_out.requires_grad)):
+            _no_gradient()
         rows = k.shape[0]
         k_row = _rows(k, "k", rows, self.kv_heads, d, dtype, dev)
         v_row = _rows(v, "v", rows, self.kv_heads, d, dtype, dev)
@@ -302,9 +322,10 @@ class PagedKv:
                              row_dtype, magnitude)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        rc = _entry("itk_paged_append", 3)(self._kv, batch, a, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
+        rc = (_calls.get("itk_paged_append") or _entry("itk_paged_append", 3))(self._kv, batch, a, _raw_stream(dev) if stream is None else stream, _reason.at, _ERROR_LEN)
         if rc != _lib.OK:
             _reason.refuse(rc)
+        _written([self.k, self.v] if q_out is None else [self.k, self.v, q_out])
         return q_out
 
     def attention(self, q: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *, max_rows: int,
@@ -322,6 +343,9 @@ class PagedKv:
         row_dtype = _ROW_DTYPES.get(dtype)
         if row_dtype is None or q.dim() != 3:
             _refuse(f"rows must be f32, f16 or bf16 [rows][heads][{d}], got {dtype} {tuple(q.shape)}")
+        if _grad_enabled() and (q.requires_grad or self.k.requires_grad or self.v.requires_grad
+                                or (out is not None and out.requires_grad) or (lse is not None and lse.requires_grad)):
+            _no_gradient()
         rows, q_heads, _ = q.shape
         q_row = _rows(q, "q", rows, q_heads, d, dtype, dev)
         if out is None:
@@ -351,7 +375,8 @@ class PagedKv:
                                 max_rows, window, row_dtype, self._scale if scale is None else scale)
         except _OUT_OF_RANGE as e:
             _refuse(f"an argument is out of range: {e}")
-        rc = _entry("itk_paged_attention", 3)(self._kv, batch, a, stream, _reason.at, _ERROR_LEN)
+        rc = (_calls.get("itk_paged_attention") or _entry("itk_paged_attention", 3))(self._kv, batch, a, stream, _reason.at, _ERROR_LEN)
         if rc != _lib.OK:
             _reason.refuse(rc)
+        _written([out] if lse is None else [out, lse])
         return out

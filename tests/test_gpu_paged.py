@@ -918,6 +918,35 @@ def test_a_workspace_is_not_made_inside_a_capture():
     assert bool((x == 1).all())  # the capture went on
 
 
+@pytest.mark.parametrize("name", ["rope", "append", "attention"])
+def test_autograd_is_not_passed_by_in_silence(name):
+    """A tensor that requires a gradient is refused rather than detached; one that autograd has saved counts as changed."""
+    f, fd, _ = table(64)
+    pos = torch.arange(4, dtype=torch.int32, device="cuda")
+    b = Batch([4], [9], 2, 2, 64, F32, 8, "head")
+    kv, batch = PagedOf(b), (b.table, b.row_start, b.kv_len)
+    x, k = torch.randn(4, 2, 64, device="cuda"), torch.randn(4, 2, 64, device="cuda")
+    call = {"rope": lambda x, out: paged.rope_apply(x, pos, fd, out=out),
+            "append": lambda x, out: kv.append(k, k, *batch, q=x, q_out=out, inv_freq=fd),
+            "attention": lambda x, out: kv.attention(x, *batch, max_rows=4, out=out)}[name]
+    leaf = x.clone().requires_grad_()
+    for kw in (dict(x=leaf, out=torch.empty_like(x)), dict(x=leaf * 2, out=torch.empty_like(x)), dict(x=x, out=leaf)):
+        with pytest.raises(CudaComputeError) as e:
+            call(**kw)
+        assert "gradient" in e.value.msg
+    with torch.no_grad():
+        want = call(leaf, torch.empty_like(x)).clone()
+    assert not want.requires_grad and torch.equal(want, call(x, torch.empty_like(x)))
+    with torch.inference_mode():
+        assert torch.equal(want, call(x, torch.empty_like(x)))
+    w = torch.ones(4, 2, 64, device="cuda", requires_grad=True)
+    out = x.clone()
+    y = (w * out).sum()  # saves out
+    call(x, out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_rows_of_another_number_of_dimensions_are_refused():
     b = Batch([1], [40], 4, 2, 64, F16, 16, "head")
     for k in (b.q[0, 0, 0], b.q[0], b.q[None]):

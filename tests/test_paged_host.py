@@ -272,6 +272,47 @@ class OnCard:
         return 0
 
 
+def calls_on_card():
+    """The three calls on stand-ins, by the name of their entry point: call(**tensors), and the tensors it writes."""
+    i32 = lambda *shape: OnCard(torch.zeros(*shape, dtype=torch.int32))
+    f = OnCard(torch.zeros(32, dtype=torch.float64))
+    kv = paged.PagedKv.__new__(paged.PagedKv)
+    kv._index, kv.head_dim, kv.kv_heads, kv._kv, kv._scale = 0, 64, 2, b"", 0.125
+    rows = {n: OnCard(torch.zeros(4, 2, 64)) for n in ("x", "out", "q", "q_out", "k", "v", "k_pool", "v_pool")}
+    rows["lse"] = OnCard(torch.zeros(4, 2))
+    kv.k, kv.v = rows["k_pool"], rows["v_pool"]
+    batch, ws = (i32(1, 3), i32(2), i32(1)), OnCard(torch.zeros(8, dtype=torch.uint8))
+    return rows, {
+        "itk_rope_apply": (lambda: paged.rope_apply(rows["x"], i32(4), f, out=rows["out"], stream=7), ["out"], ["x", "out"]),
+        "itk_paged_append": (lambda: kv.append(rows["k"], rows["v"], *batch, q=rows["q"], q_out=rows["q_out"], inv_freq=f, stream=7),
+                             ["k_pool", "v_pool", "q_out"], ["k", "v", "q", "q_out", "k_pool", "v_pool"]),
+        "itk_paged_attention": (lambda: kv.attention(rows["q"], *batch, max_rows=4, out=rows["out"], lse=rows["lse"], workspace=ws, stream=7),
+                                ["out", "lse"], ["q", "out", "lse", "k_pool", "v_pool"]),
+    }
+
+
+@pytest.mark.parametrize("name", ["itk_rope_apply", "itk_paged_append", "itk_paged_attention"])
+def test_tensors_that_require_a_gradient_are_refused_while_gradients_are_enabled(name, monkeypatch):
+    made, written = [], []
+    monkeypatch.setattr(paged, "_calls", {name: lambda *args: made.append(name) or _lib.OK})
+    monkeypatch.setattr(paged, "_written", lambda ts: written.extend(ts))
+    rows, calls = calls_on_card()
+    call, writes, takes = calls[name]
+    call()
+    assert made == [name] and written == [rows[n] for n in writes]
+    for n in takes:
+        rows[n].t.requires_grad_()
+        with pytest.raises(CudaComputeError) as e:
+            call()
+        assert e.value.code == _lib.ERR_INVALID_ARGUMENT and "gradient" in e.value.msg and len(made) == 1
+        rows[n].t.requires_grad_(False)
+    for n in takes:
+        rows[n].t.requires_grad_()
+    with torch.no_grad():
+        call()
+    assert len(made) == 2
+
+
 @pytest.mark.parametrize("name", ["itk_rope_apply", "itk_paged_append", "itk_paged_attention"])
 def test_a_failed_call_is_made_once(lib, name, monkeypatch):
     """A call that reports an error may have run (an asynchronous launch before it failed): it is not made again, and its
@@ -283,15 +324,9 @@ def test_a_failed_call_is_made_once(lib, name, monkeypatch):
         C.memmove(args[-2], b"launch failed: something before it\0", 35)
         return _lib.ERR_CUDA if len(made) == 1 else _lib.OK
 
-    monkeypatch.setattr(paged, "_entry", lambda which, n: entry if which == name else pytest.fail(which))
-    i32 = lambda *shape: OnCard(torch.zeros(*shape, dtype=torch.int32))
-    x, f = OnCard(torch.zeros(4, 2, 64)), OnCard(torch.zeros(32, dtype=torch.float64))
-    kv = paged.PagedKv.__new__(paged.PagedKv)
-    kv._index, kv.head_dim, kv.kv_heads, kv._kv, kv._scale = 0, 64, 2, b"", 0.125
-    batch = (i32(1, 3), i32(2), i32(1))
-    call = {"itk_rope_apply": lambda: paged.rope_apply(x, i32(4), f, out=x, stream=7),
-            "itk_paged_append": lambda: kv.append(x, x, *batch, q=x, q_out=x, inv_freq=f, stream=7),
-            "itk_paged_attention": lambda: kv.attention(x, *batch, max_rows=4, out=x, workspace=OnCard(torch.zeros(8, dtype=torch.uint8)), stream=7)}[name]
+    monkeypatch.setattr(paged, "_calls", {name: entry})
+    monkeypatch.setattr(paged, "_written", lambda ts: None)
+    call = calls_on_card()[1][name][0]
     with pytest.raises(CudaComputeError) as e:
         call()
     assert e.value.code == _lib.ERR_CUDA and e.value.msg == "launch failed: something before it"
