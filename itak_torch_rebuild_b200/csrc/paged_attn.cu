@@ -73,9 +73,11 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     if (d->q_heads == 0) return e.refuse(ITK_ERR_ZERO_DIMENSION, "num_q_heads must be positive, got 0");
     if (d->q_heads % kv->kv_heads != 0)
         return e.refuse(ITK_ERR_NON_DIVISIBLE_HEADS, "%llu query heads do not divide evenly across %llu KV heads", d->q_heads, kv->kv_heads);
+    if (d->q_heads > 65535) return e.invalid("q_heads %llu is too large", d->q_heads);
     if (static_cast<uint64_t>(batch->total_rows) * d->q_heads > 0x7fffffffull)
         return e.invalid("total_rows x q_heads = %llu is too large", static_cast<uint64_t>(batch->total_rows) * d->q_heads);
-    if (!isfinite(d->scale)) return e.invalid("the scale must be finite");
+    const float scale_log2 = static_cast<float>(static_cast<double>(d->scale) * 1.4426950408889634074);
+    if (!isfinite(scale_log2)) return e.invalid("the scale must be finite, and below 2e38");
     if (!d->q || !d->out || !d->workspace) return e.invalid("null pointer argument");
     if (!aligned_to(d->lse, 4)) return e.invalid("lse must be aligned to 4 bytes");
     if (!aligned16(d->q) || !aligned16(d->out)) return e.invalid("q and out must start on a 16-byte boundary");
@@ -102,7 +104,7 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     p.q_heads = d->q_heads;
     p.group = d->q_heads / kv->kv_heads;
     p.window = d->window;
-    p.scale_log2 = static_cast<float>(static_cast<double>(d->scale) * 1.4426950408889634074);
+    p.scale_log2 = scale_log2;
     unsigned char* ws = static_cast<unsigned char*>(d->workspace);
     p.tickets = reinterpret_cast<unsigned int*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + l.ml);

@@ -237,6 +237,14 @@ def test_attention_refusals(lib, kw, code, part):
     assert rc == (code or _lib.ERR_INVALID_ARGUMENT) and part in err.value.decode(), err.value
 
 
+@pytest.mark.parametrize("kw,part", [(dict(q_heads=65536), "q_heads"), (dict(q_heads=1 << 30), "q_heads"), (dict(scale=3e38), "scale"), (dict(scale=-math.inf), "scale")])
+def test_attention_refuses_what_its_kernels_cannot_count(lib, kw, part):
+    """Heads whose channels would pass 32 bits, and a scale that is infinite in the base the kernels work in."""
+    err = C.create_string_buffer(256)
+    rc = lib.itk_paged_attention(C.byref(kv()), C.byref(batch(total_rows=1)), C.byref(attention(**kw)), None, err, 256)
+    assert rc == _lib.ERR_INVALID_ARGUMENT and part in err.value.decode(), err.value
+
+
 def test_too_many_pairs(lib):
     err = C.create_string_buffer(256)
     rc = lib.itk_paged_attention(C.byref(kv()), C.byref(batch(total_rows=1 << 30)), C.byref(attention()), None, err, 256)
