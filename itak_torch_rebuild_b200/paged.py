@@ -262,6 +262,8 @@ class PagedKv:
         self._scale = 1.0 / math.sqrt(max(self.head_dim, 1))
         self._kv = bytes(_lib.PagedKv(k.data_ptr(), v.data_ptr(), st[0], st[heads_at], st[rows_at], self.n_pages, self.page_size,
                                       self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], self._index))
+        if max(k.shape) > 0xffffffff:  # (a ctypes field would cut it)
+            _refuse(f"the pools' shape {tuple(k.shape)} is out of range")
 
     def _batch(self, table, row_start, kv_len, total_rows, status) -> bytes:
         dev, n, i32 = self._index, kv_len.numel(), torch.int32
@@ -281,7 +283,10 @@ class PagedKv:
             word = _vector(status, "status", i32, None, dev)
             if status.numel() < 1:
                 _refuse("status must hold one element")
-        return _PACK_BATCH(table.data_ptr(), row_start.data_ptr(), kv_len.data_ptr(), word, n, width, stride, total_rows)
+        try:
+            return _PACK_BATCH(table.data_ptr(), row_start.data_ptr(), kv_len.data_ptr(), word, n, width, stride if n > 1 else width, total_rows)
+        except _OUT_OF_RANGE as e:
+            _refuse(f"a size of the batch is out of range: {e}")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, *,
                q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,

@@ -245,6 +245,30 @@ def test_attention_refuses_what_its_kernels_cannot_count(lib, kw, part):
     assert rc == _lib.ERR_INVALID_ARGUMENT and part in err.value.decode(), err.value
 
 
+@pytest.mark.parametrize("name", ["itk_paged_append", "itk_paged_attention"])
+def test_sizes_that_their_fields_cannot_hold_are_refused_by_name(name, monkeypatch):
+    """A table whose rows lie 2^33 elements apart, and one whose only row does (nothing is stepped over)."""
+    packed = []
+    monkeypatch.setattr(paged, "_calls", {name: lambda *args: packed.append(_lib.PagedBatch.from_buffer_copy(args[1])) or _lib.OK})
+    monkeypatch.setattr(paged, "_written", lambda ts: None)
+    kv = paged.PagedKv.__new__(paged.PagedKv)
+    kv._index, kv.head_dim, kv.kv_heads, kv._kv, kv._scale = 0, 64, 2, b"", 0.125
+    kv.k = kv.v = x = OnCard(torch.zeros(4, 2, 64))
+    ws = OnCard(torch.zeros(8, dtype=torch.uint8))
+
+    def call(n):
+        table = OnCard(torch.zeros(n, 3, dtype=torch.int32))
+        table.stride = lambda: (1 << 33, 1)
+        batch = (table, OnCard(torch.zeros(n + 1, dtype=torch.int32)), OnCard(torch.zeros(n, dtype=torch.int32)))
+        return kv.append(x, x, *batch, stream=7) if name == "itk_paged_append" else kv.attention(x, *batch, max_rows=1, out=x, workspace=ws, stream=7)
+
+    with pytest.raises(CudaComputeError) as e:
+        call(2)
+    assert "out of range" in e.value.msg and not packed
+    call(1)
+    assert packed[0].table_stride == packed[0].table_width == 3
+
+
 def test_too_many_pairs(lib):
     err = C.create_string_buffer(256)
     rc = lib.itk_paged_attention(C.byref(kv()), C.byref(batch(total_rows=1 << 30)), C.byref(attention()), None, err, 256)
