@@ -125,7 +125,7 @@ def _no_gradient():
 
 
 def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtype, device: int) -> int:
-    """The row stride of a ``[rows][heads][head_dim]`` tensor whose heads are contiguous."""
+    """The row stride of a ``[rows][heads][head_dim]`` tensor whose heads are contiguous (of a single row: torch gives it any)."""
     if t.dtype is not dtype or t.get_device() != device:
         _refuse(f"{what} must be {dtype} on device {device}, got {t.dtype} on {t.device}")
     if t.shape != (rows, heads, head_dim):
@@ -133,7 +133,7 @@ def _rows(t: torch.Tensor, what: str, rows: int, heads: int, head_dim: int, dtyp
     s0, s1, s2 = t.stride()
     if s2 != 1 or (s1 != head_dim and heads > 1):
         _refuse(f"the heads of {what} must be contiguous, got strides {(s0, s1, s2)}")
-    return s0
+    return s0 if rows > 1 else heads * head_dim
 
 
 def _vector(t: torch.Tensor, what: str, dtype, n: Optional[int], device: int) -> int:
@@ -246,24 +246,26 @@ class PagedKv:
     def __init__(self, k: torch.Tensor, v: torch.Tensor, *, layout: str = "head"):
         if layout not in ("head", "token"):
             _refuse(f"layout is 'head' or 'token', got {layout!r}")
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+        # a dimension of one element is never stepped over, and torch gives it any stride
+        steps = [[s if n > 1 else 0 for n, s in zip(x.shape, x.stride())] for x in (k, v)]
+        if k.dim() != 4 or k.shape != v.shape or steps[0] != steps[1]:
             _refuse(f"the pools must be two 4-dimensional tensors of one shape and one set of strides, got {tuple(k.shape)} and {tuple(v.shape)}")
         if k.device.type != "cuda" or k.dtype not in (torch.float16, torch.bfloat16):
             _refuse(f"the pools must be f16 or bf16 tensors on a CUDA device, got {k.dtype} on {k.device}")
         if v.device != k.device or v.dtype is not k.dtype:
             _refuse(f"the pools must be of one type on one device, got {k.dtype} on {k.device} and {v.dtype} on {v.device}")
-        st = k.stride()
-        if st[3] != 1:
+        st = steps[0]
+        if st[3] != 1 and k.shape[3] > 1:
             _refuse("the channels of a page must be contiguous")
         self.k, self.v, self.layout, self.device, self.dtype = k, v, layout, k.device, k.dtype
         heads_at, rows_at = (1, 2) if layout == "head" else (2, 1)
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = k.shape[0], k.shape[heads_at], k.shape[rows_at], k.shape[3]
         self._index = k.get_device()
         self._scale = 1.0 / math.sqrt(max(self.head_dim, 1))
-        self._kv = bytes(_lib.PagedKv(k.data_ptr(), v.data_ptr(), st[0], st[heads_at], st[rows_at], self.n_pages, self.page_size,
-                                      self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], self._index))
         if max(k.shape) > 0xffffffff:  # (a ctypes field would cut it)
             _refuse(f"the pools' shape {tuple(k.shape)} is out of range")
+        self._kv = bytes(_lib.PagedKv(k.data_ptr(), v.data_ptr(), st[0], st[heads_at], st[rows_at], self.n_pages, self.page_size,
+                                      self.kv_heads, self.head_dim, _ROW_DTYPES[k.dtype], self._index))
 
     def _batch(self, table, row_start, kv_len, total_rows, status) -> bytes:
         dev, n, i32 = self._index, kv_len.numel(), torch.int32

@@ -547,6 +547,25 @@ def test_strided_rows_and_pages(t):
     assert bool((out[:, 0] == 7.0).all()) and bool((out[:, 5] == 7.0).all())
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_strides_that_are_never_stepped_over_do_not_count(t):
+    """A single row of Q, K, V and the result in rows of odd length, a pool with one head, one page and pages of one row."""
+    for page, hkv in ((16, 1), (1, 2)):
+        b = Batch([1], [1 if page == 1 else 9], 4, hkv, 64, t, page, "head", spare=0)
+        one = lambda x: torch.empty(x.shape[1] * 64 + 3, dtype=t, device="cuda")[:x.shape[1] * 64].view(1, -1, 64).as_strided(x.shape, (x.shape[1] * 64 + 3, 64, 1))
+        q, out, k = one(b.q), one(b.q), one(b.q[:, :hkv])
+        q.copy_(b.q)
+        odd = lambda x: x.as_strided(x.shape, [s if n > 1 else 4097 for n, s in zip(x.shape, x.stride())])
+        kv = paged.PagedKv(odd(b.k), b.v)
+        kv.attention(q, b.table, b.row_start, b.kv_len, max_rows=1, out=out)
+        b.check(out)
+        k.copy_(torch.randn(1, hkv, 64))
+        kv.append(k, k, b.table, b.row_start, b.kv_len)
+        place = (int(b.table_h[0, (b.lens[0] - 1) // page]), (b.lens[0] - 1) % page)
+        for pool in (b.k, b.v):
+            assert torch.equal(b.cell(pool, *place), k[0].to(PAGE[t]))
+
+
 def test_a_long_cache_is_addressed_past_32_bits():
     """A pool whose last pages lie beyond 2^32 bytes and 2^31 elements: the same keys there and at its start."""
     page, hkv, d = 64, 8, 128
