@@ -520,7 +520,8 @@ int itk_rope_table(const itk_rope_config* cfg, double* inv_freq, float* magnitud
  * a frequency table, and the gradient.  Pair i joins channels (2i, 2i + 1) (pairing 0) or (i, i + rotary_dim / 2)
  * (pairing 1); channels from rotary_dim on are copied.  With inverse != 0 the angle is negated: the map from the
  * gradient of `out` to the gradient of `x`.  Angles in f64, reduced to a turn before sine and cosine are taken in f32;
- * products in f32; one rounding to the rows' type.  out may be x (same strides); else the two share no element.
+ * products in f32; one rounding to the rows' type.  Positions are unsigned: -1 in a signed array is position 2^32 - 1.
+ * out may be x (same strides); else the two share no element.
  * head_dim up to 256, even. */
 typedef struct itk_rope_desc {
     const void* x;             /* device, element (row, head, channel) at row * x_row_stride + head * x_head_stride + channel */
@@ -559,8 +560,8 @@ typedef struct itk_paged_kv {
  * (or than 2^30 keys) positions stay what kv_len says, new rows behind the last column are not stored and keys there are
  * not seen (bit 1; lengths count as 2^31 - 1 at most); new rows that reach before position 0 see nothing and are not stored (bit 2); starts that run backwards
  * or past total_rows are cut (bit 3).  Bit 4: a wait inside the tensor-core kernel ran out (see
- * itk_paged_attention_wait_limit).  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] are neither
- * read nor written. */
+ * itk_paged_attention_wait_limit).  `status` may be NULL; bits stay until the caller clears them.  Rows behind row_start[n_seqs] do not
+ * count and are not written. */
 typedef struct itk_paged_batch {
     const uint32_t* table;     /* [n_seqs][table_stride], table_width columns used */
     const uint32_t* row_start; /* [n_seqs + 1] */

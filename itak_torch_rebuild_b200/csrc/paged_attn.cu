@@ -111,16 +111,24 @@ extern "C" int itk_paged_attention(const itk_paged_kv* kv, const itk_paged_batch
     p.part_o = reinterpret_cast<float*>(ws + l.o);
     const uint32_t limit = wait_kclocks.load(std::memory_order_relaxed);
     p.wait_clocks = limit != 0 ? static_cast<long long>(limit) << 10 : kWaitClocks;
-    // Few (row, head) pairs per KV head stream, many go to tensor memory.  Measured at 2055-2487 keys, 32 / 8 heads of 128
-    // channels (streaming : tensor memory, us):
-    //   16-bit rows, 16 pairs   16 sequences 37 : 53     2 sequences 17 : 19
-    //                28 pairs   16 sequences 49 : 54     8 sequences 40 : 37     2 sequences 28 : 19
-    //                48 pairs   16 sequences 75 : 54     2 sequences 32 : 21
-    //   f32 rows,    28 pairs   16 sequences 69 : 94     2 sequences 23 : 29
-    //                48 pairs   16 sequences 98 : 96     2 sequences 27 : 31
-    //                64 pairs   16 sequences 125 : 96    2 sequences 30 : 32
+    // Few (row, head) pairs per KV head stream, many go to tensor memory.  Measured at 2055-2900 keys, 32 / 8 heads, caches
+    // larger than L2 (streaming : tensor memory, us):
+    //                            16 sequences    8 sequences    2 sequences
+    //   bf16, D = 128, 16 pairs    37 :  54        26 : 39        17 : 17
+    //                  28 pairs    48 :  54        34 : 40        24 : 18
+    //                  48 pairs    73 :  54        49 : 40        24 : 20
+    //         D =  64, 16 pairs    26 :  35        19 : 26        12 : 15
+    //                  28 pairs    32 :  35        24 : 26        16 : 15
+    //                  48 pairs    51 :  36        34 : 26        17 : 16
+    //   f32,  D = 128, 28 pairs    69 :  93        45 : 63        19 : 27
+    //                  48 pairs    99 :  94        63 : 64        23 : 29
+    //                  64 pairs   126 :  95        76 : 65        26 : 30
+    //         D =  64, 28 pairs    46 :  55        30 : 37        14 : 19
+    //                  48 pairs    64 :  56        40 : 38        16 : 19
+    //                  64 pairs    82 :  56        50 : 38        18 : 20
     // Between 17 and 32 pairs of 16-bit rows what counts is how many CTAs share a cell, since the streaming kernel's joins
-    // are the slower ones: it takes them when there is a cell (sequence and KV head) for two of three multiprocessors.
+    // are the slower ones: it takes them when there is a cell (sequence and KV head) for two of three multiprocessors (the
+    // border lies somewhere below the 64 cells of 8 sequences, above the 16 of two).
     const uint64_t pairs = static_cast<uint64_t>(d->max_rows < batch->total_rows ? d->max_rows : batch->total_rows) * p.group;
     const uint32_t narrow = stream_pairs(d->dtype);
     const bool many_cells = static_cast<uint64_t>(batch->n_seqs) * kv->kv_heads * 3 >= sms * 2ull;

@@ -94,6 +94,8 @@ struct Cursor {
     bool fresh, done;
 };
 
+// Shared memory grows by 20 bytes a sequence: of 128 channels, two CTAs have room on a multiprocessor up to 842 sequences (433
+// with two products), one beyond - right all the same, since no CTA waits for another.
 template <int D, int STAGES>
 __host__ __device__ constexpr size_t pipe_bytes() {
     return static_cast<size_t>(STAGES) * kWarps * 2 * 16 * D * 2;

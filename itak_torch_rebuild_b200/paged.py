@@ -149,7 +149,8 @@ def rope_table(rotary_dim: int, base: float, *, scaling: str = "plain", factor: 
                low: float = 1.0, high: float = 0.0, pair_factors: Optional[Sequence[float]] = None, magnitude: float = 0.0):
     """The frequencies of a rotation: ``(inv_freq, magnitude)``, an f64 array of ``rotary_dim / 2`` angles per position and
     the factor on sine and cosine (``itk_rope_table``).  ``scaling``: ``plain``, ``linear``, ``base``, ``bands``, ``ramp`` (turns
-    ``low`` < ``high`` over ``original_context``) or ``pairs`` (``pair_factors``).  Copy the table to the device once."""
+    ``low`` < ``high`` over ``original_context``) or ``pairs`` (``pair_factors``); all of these are f32 values, the table is f64.
+    Copy it to the device once."""
     if scaling not in _SCALINGS:
         _refuse(f"rope: unknown scaling {scaling!r}")
     pf = None
@@ -172,9 +173,9 @@ def rope_table(rotary_dim: int, base: float, *, scaling: str = "plain", factor: 
 def rope_apply(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, pairing: int = 0, magnitude: float = 1.0,
                inverse: bool = False, out: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
     """Rotates ``x`` ``[rows][heads][head_dim]`` (f32, f16 or bf16; any row and head strides), row ``r`` at
-    ``positions[r]`` (int32).  ``pairing`` 0 joins channels (2i, 2i + 1), 1 joins (i, i + rotary_dim / 2), with
+    ``positions[r]`` (int32, read as unsigned: there are no positions before 0).  ``pairing`` 0 joins channels (2i, 2i + 1), 1 joins (i, i + rotary_dim / 2), with
     ``rotary_dim = 2 * len(inv_freq)``; ``inverse=True`` maps the gradient of the result to the gradient of ``x``.
-    ``out`` may be ``x``."""
+    ``out`` may be ``x``.  At least one row and head."""""
     dtype, dev = _ROW_DTYPES.get(x.dtype), x.get_device()
     if dtype is None or dev < 0 or x.dim() != 3:
         _refuse(f"x must be an f32, f16 or bf16 [rows][heads][head_dim] tensor on a CUDA device, got {x.dtype} {tuple(x.shape)} on {x.device}")
