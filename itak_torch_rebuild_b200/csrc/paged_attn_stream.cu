@@ -492,12 +492,13 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
                 }
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    const float base = m[t][j] == -INFINITY ? 0.f : m[t][j] - kLift<P>;
+                    // (f32 rows: lifted behind the exponential, whose argument would cost the largest weights three of their bits)
+                    const float base = m[t][j] == -INFINITY ? 0.f : SPLIT ? m[t][j] : m[t][j] - kLift<P>;
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            w[j][n][e] = fast_exp2(w[j][n][e] - base);
+                            w[j][n][e] = SPLIT ? fast_exp2(w[j][n][e] - base) * (1.f / kUnlift<P>) : fast_exp2(w[j][n][e] - base);
                             l[t][j] += w[j][n][e];
                         }
                 }

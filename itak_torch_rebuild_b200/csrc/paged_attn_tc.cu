@@ -142,6 +142,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -850,8 +855,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         l *= f;
                     }
                     if (!(mx < INFINITY)) m = NAN;  // a NaN or +infinity among the scores: the row is NaN from here on
-                    const float nm = m == -INFINITY ? 0.f : kLift<P> - m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float nm = m == -INFINITY ? 0.f : -m;
+                    // (lifted behind the exponential: 7 in its argument would cost the largest weights three of their bits)
+                    const uint64_t c2 = pair_of(c, c), nm2 = pair_of(nm, nm), lift2 = pair_of(1.f / kUnlift<P>, 1.f / kUnlift<P>);
+                    uint64_t sum2[2] = {0u, 0u};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t x[32];
@@ -862,20 +869,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             uint32_t y[16];
 #pragma unroll
                             for (int u = 0; u < 8; ++u) {
-                                const float w0 = fast_exp2(fmaf(__uint_as_float(x[16 * g + 2 * u]), c, nm));
-                                const float w1 = fast_exp2(fmaf(__uint_as_float(x[16 * g + 2 * u + 1]), c, nm));
-                                sum[u & 1] += w0;
-                                sum[2 + (u & 1)] += w1;
-                                const __half2 h = __floats2half2_rn(w0, w1);
+                                const float2 e2 = unpair(fma2(pair_of(__uint_as_float(x[16 * g + 2 * u]), __uint_as_float(x[16 * g + 2 * u + 1])), c2, nm2));
+                                const uint64_t w2 = mul2(pair_of(fast_exp2(e2.x), fast_exp2(e2.y)), lift2);
+                                sum2[u & 1] = add2(sum2[u & 1], w2);
+                                const float2 w = unpair(w2);
+                                const __half2 h = __floats2half2_rn(w.x, w.y);
                                 const float2 hf = __half22float2(h);
                                 y[u] = *reinterpret_cast<const uint32_t*>(&h);
-                                y[8 + u] = pack2(__half(), w0 - hf.x, w1 - hf.y);
+                                y[8 + u] = pack2(__half(), w.x - hf.x, w.y - hf.y);
                             }
                             tc::tmem_st16(tS + 32 * j + 16 * g, y);
                         }
                         if (j == 1) stored(0);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 s01 = unpair(add2(sum2[0], sum2[1]));
+                    l += s01.x + s01.y;
                 } else {
                     uint32_t x[4][32];
 #pragma unroll
