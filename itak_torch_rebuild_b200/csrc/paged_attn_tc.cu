@@ -36,7 +36,7 @@
 // clocks on the special-function units.  A round (both products of a tile of one stream) takes about 1600: softmax and
 // products of one stream follow one another, and two streams do not quite cover that chain.  (2^x by a polynomial on the
 // multiply-add pipe for part of the weights made it longer.)  Measured: 4096 bf16 rows at 16384 keys, 32 / 8 heads of 128:
-// 797-900 us by the board's power state, 1.07-1.21 PFLOP/s of 1.66; 4 x 512 rows at 1024-2048 keys: f16 73 us, f32 157 us,
+// 956 us (826 before the power limit sets in), 1.01 PFLOP/s of 1.66; 4 x 512 rows at 1024-2048 keys: f16 73 us, f32 153 us,
 // where a cell's end (3 tiles' time), the joins and 14000 clocks before the first tile count as much as the tiles.
 #include <cuda.h>
 

@@ -9,8 +9,8 @@
 // once, by as many threads as there are pairs, and shared through shared memory by every head; the first heads' data is
 // requested before the angles are known.
 //
-// Measured (share of the copy rate): 8192 x 64 head rows of 128 bf16 channels 46.4 us (0.90); 6 ragged sequences of 611-2048 new
-// tokens, 64 / 8 heads, Q, K and V 57 us (0.89); f32 98 us (0.98); a decode step of 16 sequences 3.5 us.
+// Measured (share of the copy rate): 8192 x 64 head rows of 128 bf16 channels 47 us (0.88), f32 82 us (1.0); 6 ragged sequences
+// of 611-2048 new tokens, 64 / 8 heads, Q, K and V 57-58 us (0.88); a decode step of 16 sequences 3.5 us.
 #include <math.h>
 
 #include "paged.cuh"
