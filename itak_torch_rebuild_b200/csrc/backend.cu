@@ -178,6 +178,7 @@ struct itk_backend {
         return code;
     }
     int cuda_fail(cudaError_t e, const char* what) const {
+        cudaGetLastError();  // reported here, not by the thread's next launch
         return fail(ITK_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
     }
     size_t row_len() const { return static_cast<size_t>(cfg.kv_heads) * cfg.head_dim; }
