@@ -198,6 +198,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 
 // The kernels are launched as programmatic dependents: their blocks take their places while the kernel before them in the
 // stream still runs, and wait here before they touch memory (2 us of a call that follows another).
+// What a predecessor may have written - the table, starts, lengths, rows - is read with plain loads: the path for data that is
+// read-only while a kernel runs is not for them, since this kernel runs while they are written.
 __device__ __forceinline__ void after_predecessor() {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) paged_stream_kerne
         const uint32_t key = L.t * kTile + warp * 16 + (lane & 15);
         const uint32_t inside = min(max(key, L.lo), L.hi - 1u);  // rows outside the block's keys are not read
         if (L.done || L.hi == 0) return 0u;
-        return __ldg(p.batch.table + static_cast<size_t>(L.s) * p.batch.table_stride + (inside >> shift));
+        return p.batch.table[static_cast<size_t>(L.s) * p.batch.table_stride + (inside >> shift)];
     };
     uint32_t page = page_of();
     auto request = [&](uint32_t stage) {

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const uint32_t* const tab = p.batch.table + static_cast<size_t>(it.s) * p.batch.table_stride;
                 const uint32_t lo = it.lo, hi = it.hi;
                 auto holds = [&](uint32_t key) { return row_at < kTile && key < hi && key + (1u << box_shift) > lo; };
-                auto page_of = [&](uint32_t key) { return holds(key) ? __ldg(tab + (key >> shift)) : 0u; };
+                auto page_of = [&](uint32_t key) { return holds(key) ? tab[key >> shift] : 0u; };
                 uint32_t ahead = it.t0 < it.t1 ? page_of(it.t0 * kTile + row_at) : 0u;  // page numbers come a tile ahead
                 for (uint32_t t = it.t0; ok && t < it.t1; ++t) {
                     const uint32_t key = t * kTile + row_at;  // the box holds keys [key, key + box rows)

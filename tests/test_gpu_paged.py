@@ -886,6 +886,41 @@ def test_a_stream_given_by_number_that_is_being_captured_needs_a_workspace_too()
     assert "workspace" in e.value.msg
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("captured", [False, True])
+def test_tables_and_lengths_that_the_kernel_before_wrote(rows, captured):
+    """The kernels take their places while the one before them still runs: what it wrote last is what they read."""
+    b = Batch([rows] * 3, [700, 260, 513], 8, 2, 64, F16, 16, "head")
+    kv, ws = PagedOf(b), paged.attention_workspace("cuda:0")
+    other = b.table.flip(0).contiguous()  # the sequences in the opposite order
+    lens = [b.kv_len.clone(), b.kv_len.flip(0).contiguous()]
+    tables = [b.table.clone(), other]
+    want = [kv.attention(b.q, tables[i], b.row_start, lens[i], max_rows=rows, workspace=ws) for i in (0, 1)]
+    outs = [torch.empty_like(b.q) for _ in range(2)]
+    turn = torch.zeros(1, dtype=torch.int64, device="cuda")
+    both, both_lens = torch.stack(tables), torch.stack(lens)
+
+    def steps():
+        for _ in range(10):
+            for out in outs:
+                b.table.copy_(both.index_select(0, turn)[0] + 0 * b.table)  # (reads what it replaces)
+                b.kv_len.copy_(both_lens.index_select(0, turn)[0])
+                turn.sub_(1).neg_()
+                kv.attention(b.q, b.table, b.row_start, b.kv_len, max_rows=rows, out=out, workspace=ws)
+
+    torch.cuda.synchronize()
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            steps()
+    for _ in range(10):
+        for out in outs:
+            out.zero_()
+        g.replay() if captured else steps()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
 def test_the_per_thread_default_stream_shares_nothing_of_the_modules():
     """Its handle is one number for the streams of all threads: neither a workspace nor the allocator may go by it."""
     b = Batch([1, 1], [400, 90], 4, 2, 64, F16, 16, "head")
